@@ -657,6 +657,60 @@ typedef struct ic_attn_bwd_args {
 } ic_attn_bwd_args;
 int ic_attn_bwd(const ic_attn_bwd_args* b, ic_stream_t stream);
 
+/* ---------------------------------------------------------------- rotary positions and per-head norms of q and k
+ * Rows of the token mixer's queries and keys: the rotation of reference iron_rope.py:49-66 (channel pairs (2j, 2j+1)),
+ * the half layout (pairs (j, m + j)), rotation of a leading part of the row only, and an RMSNorm of every head's row
+ * (utils.py:33-35) in the same pass.
+ *   u = x                                     (w == NULL)
+ *   u = w * x / sqrt(mean_D(x^2) + eps)       (w != NULL)
+ *   y_a = u_a c - u_b s,  y_b = u_a s + u_b c  for the m pairs (a, b);  y = u on the other D - 2m channels
+ * with c = scale * cos(angle), s = scale * sin(angle): either read from cos / sin, or formed from angle =
+ * position * freqs[j], in 64 bits (a far position's angle keeps its fraction).  Arithmetic in fp32, one rounding to the
+ * rows' type at the end.  Rows may be strided (elements; the D channels of a row are contiguous). */
+enum { IC_DT_F32 = 0, IC_DT_BF16 = 1, IC_DT_F16 = 2 };
+enum { IC_ROPE_INTERLEAVED = 0, IC_ROPE_HALF = 1 };
+typedef struct ic_rope_rows {
+  const void* x;              /* [B,H,T,D] rows: element (b,h,t,j) at b*x_sb + h*x_sh + t*x_st + j */
+  void* y;                    /* the same shape, strides y_*; must not overlap x */
+  const void* w;              /* [D] norm weight, or NULL: no norm */
+  int64_t x_sb, x_sh, x_st;
+  int64_t y_sb, y_sh, y_st;
+  int32_t H;                  /* 0: no such rows (only allowed for k) */
+  int32_t w_dtype;            /* IC_DT_* of w (and of the gradient gw) */
+} ic_rope_rows;
+typedef struct ic_rope_args {
+  int32_t B, T, D, m;         /* D <= 512; 2m <= D; B*T < 2^31 */
+  int32_t dtype, layout;      /* IC_DT_* of the rows, IC_ROPE_* */
+  int32_t inverse;            /* 1: rotate by the negative angles (the transposed map); no norm then */
+  int32_t pos64, freq64;      /* positions are int64 (else int32); freqs are fp64 (else fp32) */
+  float scale, eps;
+  const float* cos;           /* [B or 1,T,m], or NULL: from positions and freqs */
+  const float* sin;
+  int64_t cs_sb;              /* elements from one sequence's table to the next (0: shared) */
+  const void* positions;      /* [B or 1,T], or NULL: position t */
+  int64_t pos_sb;
+  const void* freqs;          /* [m] radians per position */
+  ic_rope_rows q, k;          /* both with w or both without */
+} ic_rope_args;
+int ic_rope_fwd(const ic_rope_args* a, ic_stream_t stream);
+/* Backward of ic_rope_fwd with norms (without them it is ic_rope_fwd with inverse = 1 on the gradients).  x is read
+ * again (its norm is recomputed); gw is WRITTEN.  part: [ic_rope_parts(), D] floats of workspace; partial sums of gw
+ * are added in a fixed order (no atomics). */
+typedef struct ic_rope_grad {
+  const void* g;              /* d loss / d y, strides g_* */
+  void* gx;                   /* d loss / d x, strides gx_* */
+  void* gw;                   /* [D], type w_dtype */
+  int64_t g_sb, g_sh, g_st;
+  int64_t gx_sb, gx_sh, gx_st;
+} ic_rope_grad;
+typedef struct ic_rope_bwd_args {
+  ic_rope_args f;             /* the forward's arguments (y unused, inverse = 0) */
+  ic_rope_grad q, k;
+  float* part;
+} ic_rope_bwd_args;
+int ic_rope_parts(void);
+int ic_rope_bwd(const ic_rope_bwd_args* b, ic_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,11 +6,13 @@ gradients are deferred to one ic_*_wgrad launch per backward pass through a tape
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Callable, Dict, List, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ENUMS, check, lib, new, ptr, stream_handle
 
@@ -912,6 +914,204 @@ def attention(q, k, v, valid_len=None, alpha=None, lag_dt: float = 1.0, eps_log:
     vl = None if valid_len is None else valid_len.to(torch.int32).contiguous()
     out, stats = AttnFn.apply(_pad_cols(q, pa), _pad_cols(k, pa), _pad_cols(v, pb), vl, alpha, lag_dt, eps_log)
     return (out if pb == dv else out[..., :dv]), stats
+
+
+# ---------------------------------------------------------------- rotary positions, norms of queries and keys
+DTYPES = {torch.float32: ENUMS["IC_DT_F32"], torch.bfloat16: ENUMS["IC_DT_BF16"], torch.float16: ENUMS["IC_DT_F16"]}
+ROPE_LAYOUTS = {"interleaved": ENUMS["IC_ROPE_INTERLEAVED"], "half": ENUMS["IC_ROPE_HALF"]}
+ROPE_MAX_D = 512
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on(t: torch.Tensor):
+    """The launches below go to the tensors' own device (its current stream), whatever the current device is."""
+    return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _same_device(who: str, first: torch.Tensor, **others) -> None:
+    if not first.is_cuda:
+        raise RuntimeError(f"{who}: needs tensors on a ROCm device (got a CPU tensor)")
+    for n, t in others.items():
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"{who}: {n} is on {t.device}, the rows are on {first.device}")
+
+
+def _rows4(t: torch.Tensor) -> torch.Tensor:
+    """Rows whose channels lie side by side (any strides of the other dimensions)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _empty_in_order(shape, strides, dtype, device) -> torch.Tensor:
+    """A dense [B,H,T,D] tensor whose dimensions lie in memory in the order of the given strides (D innermost): the
+    gradient of a [B,T,H,D]-ordered view comes back in that order."""
+    o = sorted((0, 1, 2), key=lambda i: -strides[i])
+    return torch.empty([shape[i] for i in o] + [shape[3]], dtype=dtype, device=device).permute([o.index(i) for i in (0, 1, 2)] + [3])
+
+
+class _Angles:
+    """Checked angles of a rotation: tables cos / sin, or positions and frequencies."""
+
+    def __init__(self, who, q, cos, sin, positions, freqs, layout, scale):
+        B, _, T, D = q.shape
+        if layout not in ROPE_LAYOUTS:
+            raise ValueError(f"{who}: layout {layout!r} (one of {sorted(ROPE_LAYOUTS)})")
+        if (cos is None) != (sin is None) or (cos is None) == (freqs is None):
+            raise ValueError(f"{who}: angles are given either as cos and sin or as freqs (with positions)")
+        if cos is not None and positions is not None:
+            raise ValueError(f"{who}: positions go with freqs, not with cos / sin")
+        _same_device(who, q, cos=cos, sin=sin, positions=positions, freqs=freqs)
+        if any(t is not None and t.requires_grad for t in (cos, sin, freqs)):
+            raise RuntimeError(f"{who}: no gradient reaches the angles (cos, sin, freqs): detach them")
+        self.scale, self.layout = float(scale), ROPE_LAYOUTS[layout]
+        if cos is not None:
+            for n, t in (("cos", cos), ("sin", sin)):
+                if t.dtype != torch.float32 or t.shape != cos.shape or t.dim() not in (2, 3) or t.shape[-2] != T or (t.dim() == 3 and t.shape[0] not in (1, B)):
+                    raise ValueError(f"{who}: {n} is {t.dtype} {tuple(t.shape)}, needs fp32 [T,m], [1,T,m] or [B,T,m] with B={B}, T={T}")
+            self.m = cos.shape[-1]
+            self.cos, self.sin, self.pos, self.freqs = cos.contiguous(), sin.contiguous(), None, None
+            self.sb = T * self.m if cos.dim() == 3 and cos.shape[0] == B and B > 1 else 0
+        else:
+            if freqs.dim() != 1 or freqs.dtype not in (torch.float32, torch.float64):
+                raise ValueError(f"{who}: freqs is {freqs.dtype} {tuple(freqs.shape)}, needs fp32 or fp64 [m]")
+            self.m = freqs.shape[0]
+            self.sb = 0
+            if positions is not None:
+                if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((T,), (1, T), (B, T)):
+                    raise ValueError(f"{who}: positions is {positions.dtype} {tuple(positions.shape)}, needs int32 or int64 [T], [1,T] or [B,T] with B={B}, T={T}")
+                positions = positions.contiguous()
+                self.sb = T if positions.dim() == 2 and positions.shape[0] == B and B > 1 else 0
+            self.cos = self.sin = None
+            self.pos, self.freqs = positions, freqs.contiguous()
+        if 2 * self.m > D:
+            raise ValueError(f"{who}: {self.m} rotated pairs do not fit rows of {D} channels")
+
+    def fill(self, a) -> None:
+        a.m, a.layout, a.scale = self.m, self.layout, self.scale
+        if self.cos is not None:
+            a.cos, a.sin, a.cs_sb = self.cos.data_ptr(), self.sin.data_ptr(), self.sb
+        else:
+            a.freqs, a.freq64 = self.freqs.data_ptr(), int(self.freqs.dtype == torch.float64)
+            if self.pos is not None:
+                a.positions, a.pos64, a.pos_sb = self.pos.data_ptr(), int(self.pos.dtype == torch.int64), self.sb
+
+
+def _rope_args(ang: _Angles, rows, inverse: int = 0, eps: float = 0.0):
+    """ic_rope_args for [(x, y, weight), ...] (q, and k if there is one)."""
+    B, _, T, D = rows[0][0].shape
+    a = new("ic_rope_args", B=B, T=T, D=D, dtype=DTYPES[rows[0][0].dtype], inverse=inverse, eps=eps)
+    ang.fill(a)
+    for r, (x, y, w) in zip((a.q, a.k), rows):
+        r.H, r.x = x.shape[1], x.data_ptr()
+        r.x_sb, r.x_sh, r.x_st = x.stride()[:3]
+        if y is not None:
+            r.y = y.data_ptr()
+            r.y_sb, r.y_sh, r.y_st = y.stride()[:3]
+        if w is not None:
+            r.w, r.w_dtype = w.data_ptr(), DTYPES[w.dtype]
+    return a
+
+
+class RopeFn(torch.autograd.Function):
+    """Rotated queries (and keys) in one launch (ic_rope_fwd); the backward is the rotation by the negative angles."""
+
+    @staticmethod
+    def forward(ctx, q, k, ang):
+        xs = [_rows4(t) for t in (q, k) if t is not None]
+        ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+        with _on(q):
+            _call("ic_rope_fwd", _rope_args(ang, [(x, y, None) for x, y in zip(xs, ys)]))
+        ctx.like = [x.stride() for x in xs]
+        ctx.ang = ang
+        ctx.save_for_backward(ang.cos, ang.sin, ang.pos, ang.freqs)  # (so that angles changed in place raise)
+        return ys[0], (ys[1] if len(ys) > 1 else None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        ctx.saved_tensors
+        gs = [_rows4(g) for g in (gq, gk)[:len(ctx.like)]]
+        outs = [_empty_in_order(g.shape, st, g.dtype, g.device) for g, st in zip(gs, ctx.like)]
+        with _on(gs[0]):
+            _call("ic_rope_fwd", _rope_args(ctx.ang, [(g, o, None) for g, o in zip(gs, outs)], inverse=1))
+        return outs[0], (outs[1] if len(outs) > 1 else None), None
+
+
+class QKNormRopeFn(torch.autograd.Function):
+    """RMSNorm of every head's row of q and k and the rotation, one launch (ic_rope_fwd with weights); the backward
+    (ic_rope_bwd) reads the rows again instead of keeping their norms."""
+
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, ang, eps):
+        xs = [_rows4(q), _rows4(k)]
+        ws = [wq.contiguous(), wk.contiguous()]
+        ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+        with _on(q):
+            _call("ic_rope_fwd", _rope_args(ang, list(zip(xs, ys, ws)), eps=eps))
+        ctx.ang, ctx.eps = ang, eps
+        ctx.save_for_backward(*xs, *ws, ang.cos, ang.sin, ang.pos, ang.freqs)
+        return ys[0], ys[1]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        xq, xk, wq, wk = ctx.saved_tensors[:4]
+        gs = [_rows4(gq), _rows4(gk)]
+        outs = [_empty_in_order(x.shape, x.stride(), x.dtype, x.device) for x in (xq, xk)]
+        gws = [torch.empty_like(wq), torch.empty_like(wk)]
+        part = torch.empty(ROPE_PARTS, xq.shape[-1], device=xq.device)
+        b = new("ic_rope_bwd_args", f=_rope_args(ctx.ang, [(xq, None, wq), (xk, None, wk)], eps=ctx.eps), part=part)
+        for r, g, o, gw in zip((b.q, b.k), gs, outs, gws):
+            r.g, r.gx, r.gw = g.data_ptr(), o.data_ptr(), gw.data_ptr()
+            r.g_sb, r.g_sh, r.g_st = g.stride()[:3]
+            r.gx_sb, r.gx_sh, r.gx_st = o.stride()[:3]
+        with _on(xq):
+            _call("ic_rope_bwd", b)
+        return outs[0], outs[1], gws[0], gws[1], None, None
+
+
+ROPE_PARTS = 1024  # workgroups (partial sums of the norm weights' gradients) of ic_rope_bwd: ic_rope_parts()
+
+
+def _check_qk(who, q, k) -> None:
+    _same_device(who, q, k=k)
+    if q.dim() != 4 or q.dtype not in DTYPES or not 1 <= q.shape[3] <= ROPE_MAX_D:
+        raise ValueError(f"{who}: q is {q.dtype} {tuple(q.shape)}, needs fp32, bf16 or fp16 [B,H,T,D] with D <= {ROPE_MAX_D}")
+    if k is not None and (k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], k.shape[2], k.shape[3]) != (q.shape[0], q.shape[2], q.shape[3])):
+        raise ValueError(f"{who}: k is {k.dtype} {tuple(k.shape)}, q is {q.dtype} {tuple(q.shape)}: only the number of heads may differ")
+
+
+def rope(q, k=None, *, cos=None, sin=None, positions=None, freqs=None, layout: str = "interleaved", scale: float = 1.0):
+    """Rotary positions of q [B,H,T,D] and, in the same launch, of k [B,Hk,T,D] (fp32, bf16 or fp16; any strides).
+
+    The first 2m channels of a row are m pairs -- (2j, 2j+1) with layout "interleaved" (iron_rope.py:49-66), (j, m+j) with
+    "half" -- turned by their position's angles; the other D - 2m are copied.  Angles come as fp32 tables cos / sin
+    ([T,m] or [B,T,m]), or from freqs ([m], radians per position, fp32 or fp64) and integer positions ([T] or [B,T]; None:
+    0 .. T-1), whose product is formed in 64 bits.  scale multiplies both cos and sin (the rotated channels).
+    Returns dense [B,H,T,D] rows: the rotated q, or (q, k).  Gradients reach q and k."""
+    _check_qk("rope", q, k)
+    ang = _Angles("rope", q, cos, sin, positions, freqs, layout, scale)
+    if q.numel() == 0 or (k is not None and k.numel() == 0):
+        return (q.clone(), k.clone()) if k is not None else q.clone()
+    yq, yk = RopeFn.apply(q, k, ang)
+    return yq if k is None else (yq, yk)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, *, eps: float = 1e-5, cos=None, sin=None, positions=None, freqs=None,
+                 layout: str = "interleaved", scale: float = 1.0):
+    """rope() of w * x / sqrt(mean_D(x^2) + eps): an RMSNorm of every head's row of q (weight q_weight [D]) and of k
+    (k_weight [D]; weights in fp32 or in the rows' type), then the rotation, in one pass over the rows.
+    Gradients reach q, k and both weights."""
+    _check_qk("qk_norm_rope", q, k)
+    _same_device("qk_norm_rope", q, q_weight=q_weight, k_weight=k_weight)
+    for n, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.dim() != 1 or w.shape[0] != q.shape[3] or w.dtype not in (torch.float32, q.dtype):
+            raise ValueError(f"qk_norm_rope: {n} is {w.dtype} {tuple(w.shape)}, needs fp32 or {q.dtype} [{q.shape[3]}]")
+    if q.shape[1] + k.shape[1] > ROPE_PARTS:
+        raise ValueError(f"qk_norm_rope: {q.shape[1]} + {k.shape[1]} heads (at most {ROPE_PARTS})")
+    ang = _Angles("qk_norm_rope", q, cos, sin, positions, freqs, layout, scale)
+    if q.numel() == 0 or k.numel() == 0:
+        return q * q_weight.to(q.dtype), k * k_weight.to(k.dtype)
+    return QKNormRopeFn.apply(q, k, q_weight, k_weight, ang, float(eps))
 
 
 def hebbian_rank1(W: torch.Tensor, dst_of_edge: torch.Tensor, src: torch.Tensor, widx: torch.Tensor,

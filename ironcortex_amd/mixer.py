@@ -51,6 +51,45 @@ def rope_rotate_pairs(x: torch.Tensor, cos_th: torch.Tensor, sin_th: torch.Tenso
     return torch.cat([rot.flatten(-2), tail], dim=-1)
 
 
+def rotate_qk(q: torch.Tensor, k: torch.Tensor, cos_th: torch.Tensor, sin_th: torch.Tensor):
+    """rope_rotate_pairs of q and k [B,H,T,hd] by angles [B,T,m] in one launch (ops.rope: the same products, differences and
+    sums in the same order, so the same bits); the plain formulation where the kernel has no rows or angles of its kind
+    (CPU or fp64 tensors, angles that carry a gradient)."""
+    if (q.is_cuda and q.dtype in ops.DTYPES and q.shape[-1] <= ops.ROPE_MAX_D and cos_th.dtype == torch.float32
+            and not cos_th.requires_grad):
+        return ops.rope(q, k, cos=cos_th, sin=sin_th)
+    c, s, m = cos_th.unsqueeze(1), sin_th.unsqueeze(1), cos_th.shape[-1]
+    return rope_rotate_pairs(q, c, s, m), rope_rotate_pairs(k, c, s, m)
+
+
+def rope_freqs(m: int, base: float = 10000.0, *, scaling: str = "none", factor: float = 1.0, trained_len: int = 0,
+               turns: Tuple[float, float] = (1.0, 32.0)) -> Tuple[torch.Tensor, float]:
+    """(freqs fp64 [m], scale) for ops.rope / ops.qk_norm_rope: freqs[j] = base^(-j/m) radians per position, adapted to
+    contexts `factor` times as long as the trained one:
+      "none"    as trained;
+      "linear"  every frequency divided by factor (positions squeezed into the trained range);
+      "base"    a larger base: the lowest frequency divided by factor, the highest kept, the others in between;
+      "ramp"    by turns within trained_len positions: pairs that turn at least turns[1] times keep their frequency, pairs
+                that turn at most turns[0] times get it divided by factor, linear in the number of turns in between;
+                scale = 1 + 0.1 ln(factor) on the rotated channels of q and of k."""
+    if m < 1 or base <= 0.0 or factor < 1.0:
+        raise ValueError(f"rope_freqs: m={m}, base={base}, factor={factor} (need m >= 1, base > 0, factor >= 1)")
+    j = torch.arange(m, dtype=torch.float64)
+    if scaling == "base":
+        base = base * factor ** (m / max(1, m - 1))
+    freqs = base ** (-j / m)
+    if scaling in ("none", "base"):
+        return freqs, 1.0
+    if scaling == "linear":
+        return freqs / factor, 1.0
+    if scaling == "ramp":
+        if trained_len < 1 or not 0.0 < turns[0] < turns[1]:
+            raise ValueError(f"rope_freqs: trained_len={trained_len}, turns={turns} (need trained_len >= 1, 0 < turns[0] < turns[1])")
+        keep = ((freqs * trained_len / (2.0 * math.pi) - turns[0]) / (turns[1] - turns[0])).clamp(0.0, 1.0)
+        return freqs * keep + freqs / factor * (1.0 - keep), 1.0 + 0.1 * math.log(factor)
+    raise ValueError(f"rope_freqs: scaling {scaling!r} (one of 'none', 'linear', 'base', 'ramp')")
+
+
 def fourier_features(p: torch.Tensor, W, beta_cos, beta_sin, scale: float = 1.0):
     """(left, right) with left[q] . right[k] = scale * sum_m cos(S)beta_cos + sin(S)beta_sin, S = (p_q - p_k) W^T
     (iron_rope.py:69-97): left [B,T,2m] (headwise betas: [B,H,T,2m]), right [B,T,2m]."""
@@ -135,8 +174,7 @@ class IronRoPESelfAttention(nn.Module):
         q, k, v = (t.view(shp).transpose(1, 2) for t in (q, k, v))
         if self.rope_m > 0:
             theta = coords @ self.W_rope.T
-            c, s = torch.cos(theta).unsqueeze(1), torch.sin(theta).unsqueeze(1)
-            q, k = rope_rotate_pairs(q, c, s, self.rope_m), rope_rotate_pairs(k, c, s, self.rope_m)
+            q, k = rotate_qk(q, k, torch.cos(theta), torch.sin(theta))
         plain = not self.causal and context_mask is None and not (dropout and self.training and self.adrop.p > 0)
         plain = plain and ops.attention_fits(self.head_dim + 2 * self.fb_m, self.head_dim)  # heads wider than 128: [T,T] path
         if plain:  # the library's kernels
