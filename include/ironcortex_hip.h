@@ -711,6 +711,67 @@ typedef struct ic_rope_bwd_args {
 int ic_rope_parts(void);
 int ic_rope_bwd(const ic_rope_bwd_args* b, ic_stream_t stream);
 
+/* ---------------------------------------------------------------- linear attention with a decay for each head
+ * The recurrence of the region cells' decaying state (region.py:128-135,176-190) over a sequence and with a matrix state,
+ * for token mixing next to ic_attn_*:
+ *   S_t = e^{-rate_h} S_{t-1} + k_t v_t^T,   o_t = scale * q_t^T S_t          (S_{-1} = state, zero if NULL)
+ * for the positions t < valid_len[b]; rows behind that are written as zeros and leave the state alone.  Cost linear in T:
+ * chunks of 64 positions on the matrix cores (fp32 accumulation), the state between chunks in fp32.
+ * Rows may be strided (elements; the channels of a row are contiguous); query head h reads key / value head
+ * h / (H / Hk).  Not finite values at a position may spread to the other rows of its chunk and reach the state. */
+typedef struct ic_lattn_args {
+  int32_t B, H, Hk, T;        /* H % Hk == 0 */
+  int32_t Dk, Dv;             /* 1 .. 128 */
+  int32_t dtype;              /* IC_DT_* of q, k, v, out */
+  float scale;
+  const void* q;              /* [B,H,T,Dk]  at b*q_sb + h*q_sh + t*q_st */
+  const void* k;              /* [B,Hk,T,Dk] */
+  const void* v;              /* [B,Hk,T,Dv] */
+  int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st;
+  const float* rate;          /* [H] */
+  const int32_t* valid_len;   /* [B] or NULL: T */
+  const float* state;         /* [B,H,Dk,Dv] or NULL */
+  void* out;                  /* [B,H,T,Dv] */
+  int64_t o_sb, o_sh, o_st;
+  float* state_out;           /* [B,H,Dk,Dv] the state behind the last valid position, or NULL; not the same memory as state */
+  float* ws;                  /* workspace of ic_lattn_ws() floats (may be NULL for 0); calls that share it run in order */
+} ic_lattn_args;
+/* floats of workspace that ic_lattn_fwd (backward = 0) or ic_lattn_bwd (1) of these sizes needs */
+int ic_lattn_ws(const ic_lattn_args* a, int32_t backward, int64_t* floats);
+int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream);
+/* Backward: every gradient is WRITTEN; gradients of shared key / value heads are summed over their query heads in a fixed
+ * order, d rate over sequences and positions in 64 bits: no atomics, run-to-run identical. */
+typedef struct ic_lattn_bwd_args {
+  ic_lattn_args f;            /* the forward's arguments (out, state_out unused; ws for the backward) */
+  const void* dout;           /* [B,H,T,Dv] */
+  int64_t do_sb, do_sh, do_st;
+  const float* dstate_out;    /* [B,H,Dk,Dv] gradient of state_out, or NULL: zero */
+  void* dq;                   /* [B,H,T,Dk] */
+  void* dk;                   /* [B,Hk,T,Dk] */
+  void* dv;                   /* [B,Hk,T,Dv] */
+  int64_t dq_sb, dq_sh, dq_st, dk_sb, dk_sh, dk_st, dv_sb, dv_sh, dv_st;
+  float* drate;               /* [H] or NULL */
+  float* dstate;              /* [B,H,Dk,Dv] gradient of state, or NULL */
+} ic_lattn_bwd_args;
+int ic_lattn_bwd(const ic_lattn_bwd_args* b, ic_stream_t stream);
+/* One position (serving): state <- e^{-rate} state + k v^T in place, out = scale * q^T state.  Sequences with
+ * active[b] == 0 keep their state and get zeros.  q [B,H,Dk], k [B,Hk,Dk], v [B,Hk,Dv], out [B,H,Dv] with strides over b
+ * and h, state dense. */
+typedef struct ic_lattn_step_args {
+  int32_t B, H, Hk, Dk, Dv, dtype;
+  float scale;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh;
+  const float* rate;          /* [H] */
+  const uint8_t* active;      /* [B] or NULL: all */
+  float* state;               /* [B,H,Dk,Dv] */
+  void* out;
+  int64_t o_sb, o_sh;
+} ic_lattn_step_args;
+int ic_lattn_step(const ic_lattn_step_args* a, ic_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

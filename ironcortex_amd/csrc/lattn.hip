@@ -1,0 +1,722 @@
+// Linear attention with a decay for each head, over sequences (chunked) and for single positions (recurrent):
+//   S_t = e^{-r} S_{t-1} + k_t v_t^T,   o_t = scale * q_t^T S_t.
+//
+// Chunks of C = 64 positions.  With S the state at a chunk's border and i, j positions inside the chunk,
+//   o_i = e^{-r(i+1)} q_i^T S + sum_{j <= i} e^{-r(i-j)} (q_i . k_j) v_j,    S' = e^{-rC} S + sum_j e^{-r(C-1-j)} k_j v_j^T:
+// four matrix products on the matrix cores, every exponent of e^{-r} a non-negative count (no quotients of decays).
+//
+// The backward is the same map three more times:
+//   dq = (q, k, v) := (dout, v, k) with the transposed state;
+//   dv = (k, q, scale dout) and dk = (v, dout, scale q), both from the last position to the first, starting from the
+//   gradient of the final state; dstate is where that reversed recurrence ends.
+// So ONE kernel serves the forward (one pass) and the backward (three passes side by side in one launch).  Against a
+// kernel that forms all three gradients of a chunk at once it multiplies 12 tiles instead of 10, and needs neither the
+// state at every chunk's border in memory nor two states in registers.
+// d rate: -d o / d rate weighs every pair by its lag.  The dq pass carries the lag-weighted state L = sum lag e^{-r lag}
+// k v^T next to S, and sums q_i . (lag-weighted dq_i): every term counted once with its own lag, where a difference of
+// position-weighted q . dq and k . dk would cancel to T times the rounding error.
+//
+// Work split: a workgroup owns (sequence, head, segment of chunks); a wave 16 of the value columns, with its [Dk,16] slice
+// of the state in the accumulator registers, in the layout that the next product takes as its operand (16x16 tiles: lane
+// l holds rows 4 (l / 16) + 0..3 of column l % 16, and as an operand k-indices 4 (l / 16) + 0..3 of row / column l % 16).
+// Several segments per sequence only where sequences and heads do not fill the chip: their sums are formed first
+// (k_lattn SUMS), scanned (k_lattn_scan), and each segment starts from its own prefix.
+#include "ic_types.h"
+
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+constexpr int kC = 64;
+
+struct Mat {  // rows [B,heads,T,D] of one of q, k, v, dout, ...
+  void* p;
+  int64_t sb, sh, st;
+  int32_t group;  // query heads that share one of its heads
+  int32_t vec;    // 16-byte accesses are allowed
+};
+
+struct Pass {
+  Mat q, k, v, out, x;      // x: the rows that the lag-weighted output is multiplied with (d rate)
+  int32_t Da, Db;           // channels of q / k rows and of v / out rows
+  int32_t rev;              // positions from the last valid one down
+  int32_t out32;            // out is fp32 whatever the rows' type (partial sums of shared heads)
+  float oscale, vscale;
+  const float* init;        // start state: element (b*H + h) * Dk*Dv + a*ia + b*ib, or NULL: zero
+  int32_t ia, ib;
+  float* fin;               // end state, laid out like init, or NULL
+  int32_t fin_decay;        // the end state takes one more e^{-r} (gradient of the incoming state)
+  const float* seg;         // start states of the segments [B*H][nseg][nst][.] with the strides sga, sgb; NULL: one segment
+  int32_t sga, sgb, nst;
+  const float* gfin;        // gradient of the end state (lag-weighted: d rate), laid out like init, or NULL
+  double* dr;               // [B*H][nseg] partial sums of d rate, or NULL
+};
+
+struct Sums {               // segment sums of one state
+  Mat k, v;
+  int32_t Da, Db, rev, lag;
+  float vscale;
+  float* seg;
+};
+
+struct Geo {
+  int32_t B, H, T, nseg, cps;  // cps: chunks of a segment
+  const float* rate;
+  const int32_t* valid_len;
+};
+
+struct PassArgs {
+  Geo g;
+  Pass p[3];
+};
+struct SumArgs {
+  Geo g;
+  Sums s[2];
+};
+
+__device__ __forceinline__ int valid_of(const Geo& g, int b) {
+  if (!g.valid_len) return g.T;
+  const int n = g.valid_len[b];
+  return n < 0 ? 0 : n < g.T ? n : g.T;
+}
+
+// e^{-rate * n}, n >= 0; n = 0 is 1 for every rate
+__device__ __forceinline__ float decay(float l2, int n) { return n == 0 ? 1.f : exp2f(l2 * (float)n); }
+
+template <typename T>
+__device__ __forceinline__ const T* row_base(const Mat& m, int b, int h) {
+  return (const T*)m.p + (int64_t)b * m.sb + (int64_t)(h / m.group) * m.sh;
+}
+
+// rows [t0, t0 + kC) (virtual positions; rows >= cnt read as zero) of width D -> fp32 tile with padded rows
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void stage(float (*dst)[DP + 4], const T* src, const Mat& m, int D, int base, int cnt, int n, int rev) {
+  constexpr int VE = 16 / (int)sizeof(T), PER = DP / VE;
+  for (int i = threadIdx.x; i < kC * PER; i += NT) {
+    const int r = i / PER, c = (i - r * PER) * VE;
+    T e[VE];
+    *reinterpret_cast<uint4*>(e) = make_uint4(0, 0, 0, 0);
+    if (r < cnt) {
+      const T* row = src + (int64_t)(rev ? n - 1 - (base + r) : base + r) * m.st;
+      if (m.vec) {
+        if (c < D) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(row + c);
+      } else {
+#pragma unroll
+        for (int u = 0; u < VE; ++u)
+          if (c + u < D) e[u] = row[c + u];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < VE; u += 4)
+      *reinterpret_cast<float4*>(&dst[r][c + u]) = make_float4(ic_to_f(e[u]), ic_to_f(e[u + 1]), ic_to_f(e[u + 2]), ic_to_f(e[u + 3]));
+  }
+}
+
+__device__ __forceinline__ v4f mma(float a, float b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+// sum over 16 k-indices: a, b hold k = 4 (lane / 16) + 0..3
+__device__ __forceinline__ v4f mma16(v4f a, v4f b, v4f c) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) c = mma(a[u], b[u], c);
+  return c;
+}
+__device__ __forceinline__ v4f ld4(const float* p) { return *reinterpret_cast<const v4f*>(p); }
+
+template <int DP>
+struct Lds {
+  float Ks[kC][DP + 4];  // (padded rows: 16-byte reads of 16 rows and 4-byte reads of 4 rows spread over the banks)
+  float Qs[kC][DP + 4];
+  float Ps[kC][kC + 4];
+  double red[DP / 16];
+};
+template <int DP>
+struct LdsSums {
+  float Ks[kC][DP + 4];
+};
+
+template <typename T, int DP, bool LAG, bool SUMS, typename LDS>
+__device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Sums* sm, LDS& lds) {
+  constexpr int NT = DP * 4, NW = DP / 16, KS = DP / 16;
+  auto& Ks = lds.Ks;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, q4 = (lane >> 4) * 4;
+  const int seg = blockIdx.x % g.nseg, bh = blockIdx.x / g.nseg, b = bh / g.H, h = bh - b * g.H;
+  const int n = valid_of(g, b);
+  const float l2 = -g.rate[h] * 1.44269504088896340736f;
+  const Mat& mk = SUMS ? sm->k : p->k;
+  const Mat& mv = SUMS ? sm->v : p->v;
+  const int Da = SUMS ? sm->Da : p->Da, Db = SUMS ? sm->Db : p->Db;
+  const int rev = SUMS ? sm->rev : p->rev;
+  const float vscale = SUMS ? sm->vscale : p->vscale;
+  const T* K = row_base<T>(mk, b, h);
+  const T* V = row_base<T>(mv, b, h);
+  const int col = 16 * w + c;  // this lane's value column
+  const int NC = (g.T + kC - 1) / kC;
+  const int ch0 = seg * g.cps, ch1 = ch0 + g.cps < NC ? ch0 + g.cps : NC;
+
+  v4f S[KS], L[LAG ? KS : 1];
+#pragma unroll
+  for (int t = 0; t < KS; ++t) {
+    S[t] = v4f{0.f, 0.f, 0.f, 0.f};
+    if (LAG) L[t] = S[t];
+  }
+  const size_t dd = (size_t)Da * Db;
+  if (!SUMS) {
+    const float* s0 = p->seg ? p->seg + ((size_t)bh * g.nseg + seg) * p->nst * dd : p->init ? p->init + (size_t)bh * dd : nullptr;
+    const int ia = p->seg ? p->sga : p->ia, ib = p->seg ? p->sgb : p->ib;
+    if (s0) {
+#pragma unroll
+      for (int t = 0; t < KS; ++t)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int a = 16 * t + q4 + v;
+          if (a < Da && col < Db) {
+            S[t][v] = s0[(size_t)a * ia + (size_t)col * ib];
+            if (LAG && p->seg) L[t][v] = s0[dd + (size_t)a * ia + (size_t)col * ib];
+          }
+        }
+    }
+  }
+  double dr = 0.0;
+  for (int ch = ch0; ch < ch1; ++ch) {
+    const int base = ch * kC;
+    const int cnt = n - base < 0 ? 0 : n - base < kC ? n - base : kC;
+    if (SUMS && cnt == 0) break;
+    // the gradient of the final state enters the reversed recurrence without a step of decay in front of it
+    const int off = rev && ch == 0 ? 1 : 0;
+    if (cnt > 0) {
+      stage<T, DP, NT>(Ks, K, mk, Da, base, cnt, n, rev);
+      if constexpr (!SUMS) stage<T, DP, NT>(lds.Qs, row_base<T>(p->q, b, h), p->q, Da, base, cnt, n, rev);
+    }
+    v4f vf[4];  // V[16 s + q4 + u][col]
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = 16 * s + q4 + u;
+        vf[s][u] = j < cnt && col < Db ? ic_to_f(V[(int64_t)(rev ? n - 1 - (base + j) : base + j) * mv.st + col]) : 0.f;
+      }
+    __syncthreads();
+    if constexpr (!SUMS) {
+      auto& Ps = lds.Ps;
+      auto& Qs = lds.Qs;
+      v4f O[4], E[LAG ? 4 : 1];
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        O[it] = v4f{0.f, 0.f, 0.f, 0.f};
+        if (LAG) E[it] = O[it];
+      }
+      if (cnt > 0) {
+        // P[i][j] = e^{-r(i-j)} q_i . k_j for the ten 16x16 tiles with a j <= i, formed transposed (rows j)
+        for (int t = w; t < 10; t += NW) {
+          const int it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2;
+          v4f acc = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < KS; ++s) acc = mma16(ld4(&Ks[16 * jt + c][16 * s + q4]), ld4(&Qs[16 * it + c][16 * s + q4]), acc);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int lag = 16 * (it - jt) + c - q4 - v;
+            acc[v] = lag >= 0 ? acc[v] * decay(l2, lag) * vscale : 0.f;
+          }
+          *reinterpret_cast<v4f*>(&Ps[16 * it + c][16 * jt + q4]) = acc;
+        }
+        // what the state at the chunk's border adds
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const v4f bq = ld4(&Qs[16 * it + c][16 * s + q4]);
+            O[it] = mma16(S[s], bq, O[it]);
+            if (LAG) E[it] = mma16(L[s], bq, E[it]);
+          }
+          const int ex = 16 * it + c + 1 - off;
+          const float f = decay(l2, ex);
+          if (LAG) E[it] = f * (E[it] + (float)ex * O[it]);
+          O[it] = f * O[it];
+        }
+      }
+      __syncthreads();
+      float drc = 0.f;
+      if (cnt > 0) {
+#pragma unroll
+        for (int it = 0; it < 4; ++it)
+#pragma unroll
+          for (int s = 0; s <= it; ++s) {
+            v4f bp = ld4(&Ps[16 * it + c][16 * s + q4]);
+            O[it] = mma16(vf[s], bp, O[it]);
+            if (LAG) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u) bp[u] *= (float)(16 * (it - s) + c - q4 - u);  // (0 above the diagonal stays 0)
+              E[it] = mma16(vf[s], bp, E[it]);
+            }
+          }
+      }
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const int i = base + 16 * it + c;
+        if (i >= g.T) continue;
+        const bool live = i < n;
+        const int64_t t = rev && live ? n - 1 - i : i;
+        const int b0 = 16 * w + q4;  // this lane's four columns of row i
+        if (LAG && live) {
+          const T* x = row_base<T>(p->x, b, h) + t * p->x.st;
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (b0 + v < Db) drc = fmaf(E[it][v], ic_to_f(x[b0 + v]), drc);
+        }
+        float o[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) o[v] = live ? O[it][v] * p->oscale : 0.f;
+        if (p->out32) {
+          float* row = (float*)p->out.p + (int64_t)b * p->out.sb + (int64_t)h * p->out.sh + t * p->out.st;
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (b0 + v < Db) row[b0 + v] = o[v];
+        } else {
+          T* row = (T*)p->out.p + (int64_t)b * p->out.sb + (int64_t)h * p->out.sh + t * p->out.st;
+          if (p->out.vec) {
+            if (b0 < Db) {
+              T e[4] = {ic_from_f<T>(o[0]), ic_from_f<T>(o[1]), ic_from_f<T>(o[2]), ic_from_f<T>(o[3])};
+              if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(row + b0) = *reinterpret_cast<uint4*>(e);
+              else *reinterpret_cast<uint2*>(row + b0) = *reinterpret_cast<uint2*>(e);
+            }
+          } else {
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (b0 + v < Db) row[b0 + v] = ic_from_f<T>(o[v]);
+          }
+        }
+      }
+      if (LAG) dr -= (double)drc * (double)p->oscale;
+    }
+    if (cnt > 0) {  // the state behind the chunk
+      const float carry = decay(l2, cnt - off);
+#pragma unroll
+      for (int t = 0; t < KS; ++t) {
+        if (LAG) L[t] = carry * (L[t] + (float)cnt * S[t]);
+        S[t] = carry * S[t];
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        v4f vl;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int left = cnt - 1 - (16 * s + q4 + u);
+          vf[s][u] = left >= 0 ? vf[s][u] * (decay(l2, left) * vscale) : 0.f;
+          vl[u] = vf[s][u] * (float)left;  // (0 where left < 0)
+        }
+#pragma unroll
+        for (int t = 0; t < KS; ++t) {
+          v4f ak;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) ak[u] = Ks[16 * s + q4 + u][16 * t + c];
+          S[t] = mma16(ak, vf[s], S[t]);
+          if (LAG) L[t] = mma16(ak, vl, L[t]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if constexpr (SUMS) {
+    float* dst = sm->seg + ((size_t)bh * g.nseg + seg) * (LAG ? 2 : 1) * dd;
+#pragma unroll
+    for (int t = 0; t < KS; ++t)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int a = 16 * t + q4 + v;
+        if (a < Da && col < Db) {
+          dst[(size_t)a * Db + col] = S[t][v];
+          if (LAG) dst[dd + (size_t)a * Db + col] = L[t][v];
+        }
+      }
+  } else {
+    if (seg == g.nseg - 1) {
+      const float last = p->fin_decay && n > 0 ? decay(l2, 1) : 1.f;
+#pragma unroll
+      for (int t = 0; t < KS; ++t)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int a = 16 * t + q4 + v;
+          if (a < Da && col < Db) {
+            const size_t at = (size_t)bh * dd + (size_t)a * p->ia + (size_t)col * p->ib;
+            if (p->fin) p->fin[at] = S[t][v] * last;
+            if (LAG && p->gfin) dr -= (double)L[t][v] * (double)p->gfin[at];
+          }
+        }
+    }
+    if (LAG) {
+      for (int o = 32; o; o >>= 1) dr += __shfl_xor(dr, o, 64);
+      if (lane == 0) lds.red[w] = dr;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < NW; ++i) t += lds.red[i];
+        p->dr[(size_t)bh * g.nseg + seg] = t;
+      }
+    }
+  }
+}
+
+template <typename T, int DP, bool LAG>
+__global__ __launch_bounds__(DP * 4) void k_lattn(PassArgs a) {
+  __shared__ __align__(16) Lds<DP> lds;
+  if (LAG && blockIdx.y == 0) lattn_body<T, DP, LAG, false>(a.g, &a.p[0], nullptr, lds);
+  else lattn_body<T, DP, false, false>(a.g, &a.p[blockIdx.y], nullptr, lds);
+}
+template <typename T, int DP, bool LAG>
+__global__ __launch_bounds__(DP * 4) void k_lattn_sums(SumArgs a) {
+  __shared__ __align__(16) LdsSums<DP> lds;
+  if (LAG && blockIdx.y == 0) lattn_body<T, DP, LAG, true>(a.g, nullptr, &a.s[0], lds);
+  else lattn_body<T, DP, false, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
+}
+
+// segment sums -> start states: seg[s] <- state in front of segment s
+struct ScanState {
+  float* seg;
+  const float* init;
+  int32_t Da, Db, ia, ib, lag, rev;
+};
+struct ScanArgs {
+  Geo g;
+  ScanState s[2];
+};
+__global__ __launch_bounds__(256) void k_lattn_scan(ScanArgs a) {
+  const ScanState& z = a.s[blockIdx.z];
+  const int dd = z.Da * z.Db, e = blockIdx.x * 256 + threadIdx.x, bh = blockIdx.y;
+  if (e >= dd) return;
+  const int b = bh / a.g.H, h = bh - b * a.g.H, n = valid_of(a.g, b), len = a.g.cps * kC;
+  const float l2 = -a.g.rate[h] * 1.44269504088896340736f;
+  const int nst = z.lag ? 2 : 1;
+  float* at = z.seg + (size_t)bh * a.g.nseg * nst * dd + e;
+  float S = z.init ? z.init[(size_t)bh * dd + (size_t)(e / z.Db) * z.ia + (size_t)(e % z.Db) * z.ib] : 0.f, L = 0.f;
+  for (int s = 0; s < a.g.nseg; ++s, at += (size_t)nst * dd) {
+    int cnt = n - s * len;
+    cnt = cnt < 0 ? 0 : cnt < len ? cnt : len;
+    const bool more = s + 1 < a.g.nseg;  // (the last segment's sum is not formed)
+    const float ls = more ? at[0] : 0.f, ll = more && z.lag ? at[dd] : 0.f;
+    at[0] = S;
+    if (z.lag) at[dd] = L;
+    const float carry = decay(l2, cnt > 0 && z.rev && s == 0 ? cnt - 1 : cnt);
+    L = carry * (L + (float)cnt * S) + ll;
+    S = carry * S + ls;
+  }
+}
+
+// gradients of shared key / value heads: sum over the query heads of a group, fp32 [B,H,T,D] -> rows of the type
+struct JoinArgs {
+  const float* part[2];
+  Mat out[2];
+  int32_t D[2];
+  int32_t B, H, Hk, T;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void k_lattn_join(JoinArgs a) {
+  const int z = blockIdx.y, D = a.D[z], G = a.H / a.Hk;
+  const int64_t n = (int64_t)a.B * a.Hk * a.T * D;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / D;
+    const int j = (int)(i - row * D);
+    const int64_t bk = row / a.T;
+    const int t = (int)(row - bk * a.T), b = (int)(bk / a.Hk), hk = (int)(bk - (int64_t)b * a.Hk);
+    float v = 0.f;
+    for (int gi = 0; gi < G; ++gi) v += a.part[z][(((int64_t)b * a.H + (int64_t)hk * G + gi) * a.T + t) * D + j];
+    ((T*)a.out[z].p)[(int64_t)b * a.out[z].sb + (int64_t)hk * a.out[z].sh + (int64_t)t * a.out[z].st + j] = ic_from_f<T>(v);
+  }
+}
+// d rate of a head: over sequences and segments, in 64 bits
+__global__ __launch_bounds__(64) void k_lattn_drate(const double* part, float* drate, int B, int H, int nseg) {
+  const int h = blockIdx.x;
+  double v = 0.0;
+  for (int i = threadIdx.x; i < B * nseg; i += 64) v += part[((size_t)(i / nseg) * H + h) * nseg + i % nseg];
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
+  if (threadIdx.x == 0) drate[h] = (float)v;
+}
+
+// One position.  Memory-bound: the state is read and written once.  A workgroup owns (sequence, head, 32 value columns):
+// 8 lanes x 4 columns, 32 rows of threads over the key channels; the output's sum over them goes through LDS.
+constexpr int kStepRows = 32;
+template <typename T>
+__global__ __launch_bounds__(256) void k_lattn_step(ic_lattn_step_args a) {
+  __shared__ float red[kStepRows][33];
+  const int bh = blockIdx.x, b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hk);
+  const int r = threadIdx.x >> 3, c0 = blockIdx.y * 32 + (threadIdx.x & 7) * 4;
+  T* out = (T*)a.out + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh;
+  const int oc = blockIdx.y * 32 + threadIdx.x;
+  if (a.active && !a.active[b]) {
+    if (threadIdx.x < 32 && oc < a.Dv) out[oc] = ic_from_f<T>(0.f);
+    return;
+  }
+  const T* Q = (const T*)a.q + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh;
+  const T* K = (const T*)a.k + (int64_t)b * a.k_sb + (int64_t)hk * a.k_sh;
+  const T* V = (const T*)a.v + (int64_t)b * a.v_sb + (int64_t)hk * a.v_sh;
+  float* S = a.state + (size_t)bh * a.Dk * a.Dv;
+  const float dec = expf(-a.rate[h]);
+  float v[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < 4; ++u) v[u] = c0 + u < a.Dv ? ic_to_f(V[c0 + u]) : 0.f;
+  const bool vec = a.Dv % 4 == 0 && ((uintptr_t)a.state & 15) == 0;
+  for (int k = r; k < a.Dk; k += kStepRows) {
+    const float kk = ic_to_f(K[k]), qq = ic_to_f(Q[k]);
+    float* row = S + (size_t)k * a.Dv;
+    if (vec) {
+      if (c0 < a.Dv) {
+        v4f x = ld4(row + c0);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          x[u] = fmaf(kk, v[u], dec * x[u]);
+          o[u] = fmaf(qq, x[u], o[u]);
+        }
+        *reinterpret_cast<v4f*>(row + c0) = x;
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c0 + u < a.Dv) {
+          const float x = fmaf(kk, v[u], dec * row[c0 + u]);
+          row[c0 + u] = x;
+          o[u] = fmaf(qq, x, o[u]);
+        }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) red[r][(threadIdx.x & 7) * 4 + u] = o[u];
+  __syncthreads();
+  if (threadIdx.x < 32 && oc < a.Dv) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kStepRows; ++i) s += red[i][threadIdx.x];
+    out[oc] = ic_from_f<T>(s * a.scale);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------- host
+int check_lattn(const ic_lattn_args* a, const char* who) {
+  IC_REQUIRE(a != nullptr, "%s: NULL args", who);
+  IC_REQUIRE(a->B >= 1 && a->H >= 1 && a->T >= 1, "%s: B=%d H=%d T=%d", who, a->B, a->H, a->T);
+  IC_REQUIRE(a->Hk >= 1 && a->H % a->Hk == 0, "%s: H=%d is no multiple of Hk=%d", who, a->H, a->Hk);
+  IC_REQUIRE((int64_t)a->B * a->H <= 65535, "%s: B*H=%lld (at most 65535)", who, (long long)a->B * a->H);
+  IC_REQUIRE(a->T <= (1 << 30), "%s: T=%d (at most 2^30)", who, a->T);
+  IC_REQUIRE(a->Dk >= 1 && a->Dk <= 128 && a->Dv >= 1 && a->Dv <= 128, "%s: Dk=%d Dv=%d (need 1 .. 128)", who, a->Dk, a->Dv);
+  IC_REQUIRE(ic_dt_ok(a->dtype), "%s: dtype=%d", who, a->dtype);
+  return IC_OK;
+}
+
+int pad_of(const ic_lattn_args* a) {
+  const int d = a->Dk > a->Dv ? a->Dk : a->Dv;
+  return d <= 32 ? 32 : d <= 64 ? 64 : 128;
+}
+
+// Segments: as many as bring `passes` x B x H x segments to the number of workgroups that fill the chip, and no more, since
+// every further one costs its sums.
+Geo geo_of(const ic_lattn_args* a, int passes) {
+  Geo g;
+  g.B = a->B; g.H = a->H; g.T = a->T;
+  g.rate = a->rate;
+  g.valid_len = a->valid_len;
+  const int NC = ic_ceil_div(a->T, kC);
+  const int64_t have = (int64_t)passes * a->B * a->H, want = 512;
+  int64_t ns = (want + have - 1) / have;
+  if (ns > NC) ns = NC;
+  g.cps = (int)((NC + ns - 1) / ns);
+  g.nseg = ic_ceil_div(NC, g.cps);
+  return g;
+}
+
+Mat mat(const void* p, int64_t sb, int64_t sh, int64_t st, int group, int D, int esz) {
+  Mat m;
+  m.p = const_cast<void*>(p);
+  m.sb = sb; m.sh = sh; m.st = st;
+  m.group = group;
+  const int ve = 16 / esz;
+  m.vec = ((uintptr_t)p & 15) == 0 && D % ve == 0 && sb % ve == 0 && sh % ve == 0 && st % ve == 0;
+  return m;
+}
+
+int64_t ws_floats(const ic_lattn_args* a, int backward) {
+  const Geo g = geo_of(a, backward ? 3 : 1);
+  const int64_t bh = (int64_t)a->B * a->H, dd = (int64_t)a->Dk * a->Dv;
+  int64_t n = 0;
+  if (g.nseg > 1) n += bh * g.nseg * dd * (backward ? 3 : 1);
+  if (backward) {
+    n += 2 * bh * g.nseg + 2;  // (doubles, on 8 bytes)
+    if (a->H != a->Hk) n += bh * a->T * (int64_t)(a->Dk + a->Dv);
+  }
+  return n;
+}
+
+}  // namespace
+
+#define IC_LATTN_T(dt, BODY)                     \
+  do {                                           \
+    if ((dt) == IC_DT_F32) { BODY(float) }       \
+    else if ((dt) == IC_DT_BF16) { BODY(ic_bf16) } \
+    else { BODY(ic_f16) }                        \
+  } while (0)
+#define IC_LATTN_DP(dp, T, BODY)                                \
+  if ((dp) == 32) { constexpr int DP = 32; BODY(T, DP); }       \
+  else if ((dp) == 64) { constexpr int DP = 64; BODY(T, DP); }  \
+  else { constexpr int DP = 128; BODY(T, DP); }
+
+extern "C" int ic_lattn_ws(const ic_lattn_args* a, int32_t backward, int64_t* floats) {
+  int rc = check_lattn(a, "ic_lattn_ws");
+  if (rc) return rc;
+  IC_REQUIRE(floats != nullptr, "ic_lattn_ws: NULL pointer");
+  *floats = ws_floats(a, backward);
+  return IC_OK;
+}
+
+extern "C" int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream) {
+  int rc = check_lattn(a, "ic_lattn_fwd");
+  if (rc) return rc;
+  IC_REQUIRE(a->q && a->k && a->v && a->rate && a->out, "ic_lattn_fwd: NULL tensor pointer");
+  IC_REQUIRE(!a->state_out || a->state_out != a->state, "ic_lattn_fwd: state_out is state");
+  IC_REQUIRE(a->ws || ws_floats(a, 0) == 0, "ic_lattn_fwd: NULL workspace");
+  const Geo g = geo_of(a, 1);
+  const int esz = ic_dt_size(a->dtype), G = a->H / a->Hk, dp = pad_of(a), bh = a->B * a->H;
+  hipStream_t st = (hipStream_t)stream;
+  const Mat q = mat(a->q, a->q_sb, a->q_sh, a->q_st, 1, a->Dk, esz), k = mat(a->k, a->k_sb, a->k_sh, a->k_st, G, a->Dk, esz);
+  const Mat v = mat(a->v, a->v_sb, a->v_sh, a->v_st, G, a->Dv, esz), o = mat(a->out, a->o_sb, a->o_sh, a->o_st, 1, a->Dv, esz);
+  if (g.nseg > 1) {
+    SumArgs s{};
+    s.g = g;
+    s.s[0] = Sums{k, v, a->Dk, a->Dv, 0, 0, 1.f, a->ws};
+#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, s))
+#define IC_BODY_T(T) IC_LATTN_DP(dp, T, IC_BODY)
+    IC_LATTN_T(a->dtype, IC_BODY_T);
+#undef IC_BODY
+    IC_LAUNCH_CHECK("ic_lattn_fwd");
+    ScanArgs sc{};
+    sc.g = g;
+    sc.s[0] = ScanState{a->ws, a->state, a->Dk, a->Dv, a->Dv, 1, 0, 0};
+    IC_TIMED(IC_KID_lattn_scan, st, hipLaunchKernelGGL(k_lattn_scan, dim3(ic_ceil_div(a->Dk * a->Dv, 256), bh, 1), dim3(256), 0, st, sc));
+    IC_LAUNCH_CHECK("ic_lattn_fwd");
+  }
+  PassArgs p{};
+  p.g = g;
+  Pass& f = p.p[0];
+  f.q = q; f.k = k; f.v = v; f.out = o;
+  f.Da = a->Dk; f.Db = a->Dv;
+  f.oscale = a->scale; f.vscale = 1.f;
+  f.init = a->state; f.ia = a->Dv; f.ib = 1;
+  f.fin = a->state_out;
+  if (g.nseg > 1) { f.seg = a->ws; f.sga = a->Dv; f.sgb = 1; f.nst = 1; }
+#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_fwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, p))
+  IC_LATTN_T(a->dtype, IC_BODY_T);
+#undef IC_BODY
+  IC_LAUNCH_CHECK("ic_lattn_fwd");
+  return IC_OK;
+}
+
+extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
+  IC_REQUIRE(ba != nullptr, "ic_lattn_bwd: NULL args");
+  const ic_lattn_args* a = &ba->f;
+  int rc = check_lattn(a, "ic_lattn_bwd");
+  if (rc) return rc;
+  IC_REQUIRE(a->q && a->k && a->v && a->rate && ba->dout && ba->dq && ba->dk && ba->dv, "ic_lattn_bwd: NULL tensor pointer");
+  IC_REQUIRE(!ba->dstate || ba->dstate != ba->dstate_out, "ic_lattn_bwd: dstate is dstate_out");
+  IC_REQUIRE(a->ws && ((uintptr_t)a->ws & 7) == 0, "ic_lattn_bwd: the workspace is NULL or not on 8 bytes");
+  const Geo g = geo_of(a, 3);
+  const int esz = ic_dt_size(a->dtype), G = a->H / a->Hk, dp = pad_of(a), bh = a->B * a->H, Dk = a->Dk, Dv = a->Dv;
+  const int64_t dd = (int64_t)Dk * Dv;
+  const bool lag = ba->drate != nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  const Mat q = mat(a->q, a->q_sb, a->q_sh, a->q_st, 1, Dk, esz), k = mat(a->k, a->k_sb, a->k_sh, a->k_st, G, Dk, esz);
+  const Mat v = mat(a->v, a->v_sb, a->v_sh, a->v_st, G, Dv, esz), o = mat(ba->dout, ba->do_sb, ba->do_sh, ba->do_st, 1, Dv, esz);
+  const Mat dk = mat(ba->dk, ba->dk_sb, ba->dk_sh, ba->dk_st, G, Dk, esz), dv = mat(ba->dv, ba->dv_sb, ba->dv_sh, ba->dv_st, G, Dv, esz);
+  double* dr = (double*)a->ws;
+  float* ws = a->ws + 2 * (int64_t)bh * g.nseg;
+  float* seg_s = ws;                                // S (and L): transposed, [Dv][Dk]
+  float* seg_r = ws + (int64_t)bh * g.nseg * dd * 2;  // the reversed state, [Dk][Dv]
+  if (g.nseg > 1) ws += (int64_t)bh * g.nseg * dd * 3;
+  const int nst = lag ? 2 : 1;
+  if (g.nseg > 1) {
+    SumArgs s{};
+    s.g = g;
+    s.s[0] = Sums{v, k, Dv, Dk, 0, lag, 1.f, seg_s};
+    s.s[1] = Sums{q, o, Dk, Dv, 1, 0, a->scale, seg_r};
+#define IC_BODY(T, DP)                                                                                                                        \
+  if (lag) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, true>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, s)); \
+  else IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, s))
+    IC_LATTN_T(a->dtype, IC_BODY_T);
+#undef IC_BODY
+    IC_LAUNCH_CHECK("ic_lattn_bwd");
+    ScanArgs sc{};
+    sc.g = g;
+    sc.s[0] = ScanState{seg_s, a->state, Dv, Dk, 1, Dv, lag, 0};
+    sc.s[1] = ScanState{seg_r, ba->dstate_out, Dk, Dv, Dv, 1, 0, 1};
+    IC_TIMED(IC_KID_lattn_scan, st, hipLaunchKernelGGL(k_lattn_scan, dim3(ic_ceil_div(Dk * Dv, 256), bh, 2), dim3(256), 0, st, sc));
+    IC_LAUNCH_CHECK("ic_lattn_bwd");
+  }
+  float* part_k = ws;
+  float* part_v = ws + (int64_t)bh * a->T * Dk;
+  PassArgs p{};
+  p.g = g;
+  Pass& pq = p.p[0];  // dq
+  pq.q = o; pq.k = v; pq.v = k; pq.x = q;
+  pq.out = mat(ba->dq, ba->dq_sb, ba->dq_sh, ba->dq_st, 1, Dk, esz);
+  pq.Da = Dv; pq.Db = Dk;
+  pq.oscale = a->scale; pq.vscale = 1.f;
+  pq.init = a->state; pq.ia = 1; pq.ib = Dv;
+  pq.gfin = ba->dstate_out;
+  pq.dr = dr;
+  Pass& pv = p.p[1];  // dv
+  pv.q = k; pv.k = q; pv.v = o; pv.out = dv;
+  pv.Da = Dk; pv.Db = Dv;
+  pv.rev = 1;
+  pv.oscale = 1.f; pv.vscale = a->scale;
+  pv.init = ba->dstate_out; pv.ia = Dv; pv.ib = 1;
+  pv.fin = ba->dstate; pv.fin_decay = 1;
+  Pass& pk = p.p[2];  // dk
+  pk.q = v; pk.k = o; pk.v = q; pk.out = dk;
+  pk.Da = Dv; pk.Db = Dk;
+  pk.rev = 1;
+  pk.oscale = 1.f; pk.vscale = a->scale;
+  pk.init = ba->dstate_out; pk.ia = 1; pk.ib = Dv;
+  if (G > 1) {
+    pk.out = Mat{part_k, (int64_t)a->H * a->T * Dk, (int64_t)a->T * Dk, Dk, 1, 0};
+    pv.out = Mat{part_v, (int64_t)a->H * a->T * Dv, (int64_t)a->T * Dv, Dv, 1, 0};
+    pk.out32 = pv.out32 = 1;
+  }
+  if (g.nseg > 1) {
+    pq.seg = seg_s; pq.sga = Dk; pq.sgb = 1; pq.nst = nst;
+    pv.seg = seg_r; pv.sga = Dv; pv.sgb = 1; pv.nst = 1;
+    pk.seg = seg_r; pk.sga = 1; pk.sgb = Dv; pk.nst = 1;
+  }
+#define IC_BODY(T, DP)                                                                                                              \
+  if (lag) IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, true>), dim3(bh * g.nseg, 3), dim3(DP * 4), 0, st, p)); \
+  else IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false>), dim3(bh * g.nseg, 3), dim3(DP * 4), 0, st, p))
+  IC_LATTN_T(a->dtype, IC_BODY_T);
+#undef IC_BODY
+  IC_LAUNCH_CHECK("ic_lattn_bwd");
+  if (G > 1) {
+    JoinArgs j{};
+    j.part[0] = part_k; j.part[1] = part_v;
+    j.out[0] = dk; j.out[1] = dv;
+    j.D[0] = Dk; j.D[1] = Dv;
+    j.B = a->B; j.H = a->H; j.Hk = a->Hk; j.T = a->T;
+    const int64_t most = (int64_t)a->B * a->Hk * a->T * (Dk > Dv ? Dk : Dv);
+    const int blocks = (int)(most / 256 + 1 < 4096 ? most / 256 + 1 : 4096);
+#define IC_BODY(T) IC_TIMED(IC_KID_lattn_join, st, hipLaunchKernelGGL(k_lattn_join<T>, dim3(blocks, 2), dim3(256), 0, st, j));
+    IC_LATTN_T(a->dtype, IC_BODY);
+#undef IC_BODY
+    IC_LAUNCH_CHECK("ic_lattn_bwd");
+  }
+  if (lag) {
+    IC_TIMED(IC_KID_lattn_join, st, hipLaunchKernelGGL(k_lattn_drate, dim3(a->H), dim3(64), 0, st, dr, ba->drate, a->B, a->H, g.nseg));
+    IC_LAUNCH_CHECK("ic_lattn_bwd");
+  }
+  return IC_OK;
+}
+
+extern "C" int ic_lattn_step(const ic_lattn_step_args* a, ic_stream_t stream) {
+  IC_REQUIRE(a != nullptr, "ic_lattn_step: NULL args");
+  IC_REQUIRE(a->B >= 1 && a->H >= 1 && (int64_t)a->B * a->H < (1ll << 31), "ic_lattn_step: B=%d H=%d", a->B, a->H);
+  IC_REQUIRE(a->Hk >= 1 && a->H % a->Hk == 0, "ic_lattn_step: H=%d is no multiple of Hk=%d", a->H, a->Hk);
+  IC_REQUIRE(a->Dk >= 1 && a->Dk <= 1024 && a->Dv >= 1 && a->Dv <= 1024, "ic_lattn_step: Dk=%d Dv=%d (need 1 .. 1024)", a->Dk, a->Dv);
+  IC_REQUIRE(ic_dt_ok(a->dtype), "ic_lattn_step: dtype=%d", a->dtype);
+  IC_REQUIRE(a->q && a->k && a->v && a->rate && a->state && a->out, "ic_lattn_step: NULL tensor pointer");
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid(a->B * a->H, ic_ceil_div(a->Dv, 32));
+#define IC_BODY(T) IC_TIMED(IC_KID_lattn_step, st, hipLaunchKernelGGL(k_lattn_step<T>, grid, dim3(256), 0, st, *a));
+  IC_LATTN_T(a->dtype, IC_BODY);
+#undef IC_BODY
+  IC_LAUNCH_CHECK("ic_lattn_step");
+  return IC_OK;
+}

@@ -121,8 +121,10 @@ def lib():
         _lib.ic_hebbian_rank1.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp]
         for fn_ in ("ic_region_phase_fwd", "ic_region_phase_bwd", "ic_region_wgrad", "ic_router_fwd", "ic_router_bwd", "ic_router_wgrad",
                     "ic_gate_scores", "ic_gate_select", "ic_gate_fwd", "ic_heads_fwd", "ic_heads_fwd_static", "ic_steer_select",
-                    "ic_loop_steer", "ic_linear_bwd", "ic_attn_fwd", "ic_attn_bwd", "ic_rope_fwd", "ic_rope_bwd"):
+                    "ic_loop_steer", "ic_linear_bwd", "ic_attn_fwd", "ic_attn_bwd", "ic_rope_fwd", "ic_rope_bwd",
+                    "ic_lattn_fwd", "ic_lattn_bwd", "ic_lattn_step"):
             getattr(_lib, fn_).argtypes = [vp, vp]  # (struct pointer, stream)
+        _lib.ic_lattn_ws.argtypes = [vp, i32, vp]
         _lib.ic_graph_begin.argtypes = [vp]
         _lib.ic_graph_end.argtypes = [vp, vp, vp]
         _lib.ic_graph_launch.argtypes = [vp, vp]

@@ -1114,6 +1114,156 @@ def qk_norm_rope(q, k, q_weight, k_weight, *, eps: float = 1e-5, cos=None, sin=N
     return QKNormRopeFn.apply(q, k, q_weight, k_weight, ang, float(eps))
 
 
+# ---------------------------------------------------------------- linear attention with a decay for each head
+LATTN_MAX_D = 128        # channels of a head's keys and values
+LATTN_STEP_MAX_D = 1024  # the same for single positions
+
+
+def _strides(obj, name: str, t: torch.Tensor, n: int) -> None:
+    for f, s in zip(("sb", "sh", "st")[:n], t.stride()):
+        setattr(obj, f"{name}_{f}", s)
+
+
+def _lattn_args(q, k, v, rate, valid_len, state, scale, out=None, state_out=None):
+    B, H, T, Dk = q.shape
+    a = new("ic_lattn_args", B=B, H=H, Hk=k.shape[1], T=T, Dk=Dk, Dv=v.shape[3], dtype=DTYPES[q.dtype], scale=scale, rate=rate,
+            valid_len=valid_len, state=state, state_out=state_out)
+    for n, t in (("q", q), ("k", k), ("v", v), ("o", out)):
+        if t is not None:
+            setattr(a, "out" if n == "o" else n, t.data_ptr())
+            _strides(a, n, t, 3)
+    return a
+
+
+def _lattn_ws(a, backward: int, device) -> Optional[torch.Tensor]:
+    n = ctypes.c_int64(0)
+    check(lib().ic_lattn_ws(ctypes.byref(a), backward, ctypes.byref(n)), "ic_lattn_ws")
+    if n.value == 0:
+        return None
+    ws = torch.empty(n.value, dtype=torch.float32, device=device)
+    a.ws = ws.data_ptr()
+    return ws  # (held by the caller until the launches are queued; the allocator orders reuse on this stream)
+
+
+class LinearAttnFn(torch.autograd.Function):
+    """ic_lattn_fwd / ic_lattn_bwd: the rows are saved, nothing else; the backward forms the states again."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, rate, state, valid_len, scale):
+        q, k, v = _rows4(q), _rows4(k), _rows4(v)
+        B, H, T, Dk = q.shape
+        Dv = v.shape[3]
+        out = torch.empty(B, T, H, Dv, dtype=q.dtype, device=q.device).transpose(1, 2)
+        state_out = torch.empty(B, H, Dk, Dv, device=q.device)
+        a = _lattn_args(q, k, v, rate, valid_len, state, scale, out, state_out)
+        with _on(q):
+            ws = _lattn_ws(a, 0, q.device)  # noqa: F841
+            _call("ic_lattn_fwd", a)
+        ctx.save_for_backward(q, k, v, rate, state, valid_len)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return out, state_out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout, gstate):
+        q, k, v, rate, state, valid_len = ctx.saved_tensors
+        if gout is None and gstate is None:
+            return (None,) * 7
+        B, H, T, Dk = q.shape
+        gout = torch.zeros(B, H, T, v.shape[3], dtype=q.dtype, device=q.device) if gout is None else _rows4(gout)
+        dq, dk, dv = (_empty_in_order(t.shape, t.stride(), t.dtype, t.device) for t in (q, k, v))
+        drate = torch.empty_like(rate) if ctx.needs_input_grad[3] else None
+        dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
+        f = _lattn_args(q, k, v, rate, valid_len, state, ctx.scale)
+        with _on(q):
+            ws = _lattn_ws(f, 1, q.device)  # noqa: F841
+            b = new("ic_lattn_bwd_args", f=f, dout=gout.data_ptr(), dstate_out=None if gstate is None else gstate.contiguous(),
+                    dq=dq.data_ptr(), dk=dk.data_ptr(), dv=dv.data_ptr(), drate=drate, dstate=dstate)
+            for n, t in (("do", gout), ("dq", dq), ("dk", dk), ("dv", dv)):
+                _strides(b, n, t, 3)
+            _call("ic_lattn_bwd", b)
+        return dq, dk, dv, drate, dstate, None, None
+
+
+def _check_linear(who, q, k, v, rate, state, dims: int, most: int):
+    _same_device(who, q, k=k, v=v, rate=rate, state=state)
+    want = "[B,H,T,Dk], [B,Hk,T,Dk], [B,Hk,T,Dv]" if dims == 4 else "[B,H,Dk], [B,Hk,Dk], [B,Hk,Dv]"
+    say = lambda: f"{who}: q, k, v are {q.dtype} {tuple(q.shape)}, {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}"  # noqa: E731
+    if q.dtype not in DTYPES or k.dtype != q.dtype or v.dtype != q.dtype or not (q.dim() == k.dim() == v.dim() == dims):
+        raise ValueError(f"{say()}: needs one type of fp32, bf16, fp16 and {want}")
+    if k.shape[:-1] != v.shape[:-1] or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:] or (k.shape[1] == 0) != (q.shape[1] == 0) or (k.shape[1] and q.shape[1] % k.shape[1]):
+        raise ValueError(f"{say()}: needs {want} with H a multiple of Hk")
+    B, H, Dk, Dv = q.shape[0], q.shape[1], q.shape[-1], v.shape[-1]
+    if not (1 <= Dk <= most and 1 <= Dv <= most):
+        raise ValueError(f"{say()}: Dk and Dv must be 1 .. {most}")
+    if rate.dtype != torch.float32 or rate.shape != (H,):
+        raise ValueError(f"{who}: rate is {rate.dtype} {tuple(rate.shape)}, needs fp32 [{H}]")
+    if state is not None and (state.dtype != torch.float32 or state.shape != (B, H, Dk, Dv)):
+        raise ValueError(f"{who}: state is {state.dtype} {tuple(state.shape)}, needs fp32 [{B},{H},{Dk},{Dv}]")
+
+
+def linear_attention(q, k, v, rate, *, scale: float = 1.0, state=None, valid_len=None):
+    """Causal linear attention with a decay for each head, in time linear in T: with S_t = exp(-rate_h) S_{t-1} + k_t v_t^T,
+    out_t = scale * q_t^T S_t.
+
+    q [B,H,T,Dk], k [B,Hk,T,Dk], v [B,Hk,T,Dv] in fp32, bf16 or fp16 (any strides; Dk, Dv <= 128); query head h reads key /
+    value head h // (H // Hk).  rate [H] fp32 >= 0.  state [B,H,Dk,Dv] fp32: S before the first position (None: zero).
+    valid_len [B]: positions >= valid_len[b] are padding (zeros out, the state passes them by, whatever they hold).
+    Returns (out [B,H,T,Dv] in q's type, its memory in [B,T,H,Dv] order; the state behind the last valid position, fp32:
+    the next call's `state`, or linear_attention_step's).  Gradients reach q, k, v, rate and state."""
+    if q.dim() != 4:
+        raise ValueError(f"linear_attention: q is {tuple(q.shape)}, needs [B,H,T,Dk]")
+    _check_linear("linear_attention", q, k, v, rate, state, 4, LATTN_MAX_D)
+    B, H, T, Dk = q.shape
+    if valid_len is not None:
+        _same_device("linear_attention", q, valid_len=valid_len)
+        if valid_len.shape != (B,) or valid_len.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"linear_attention: valid_len is {valid_len.dtype} {tuple(valid_len.shape)}, needs int32 or int64 [{B}]")
+        valid_len = valid_len.to(torch.int32).contiguous()
+    if B * H > 65535:
+        raise ValueError(f"linear_attention: B * H = {B * H} (at most 65535)")
+    if B * H * T == 0:
+        st = torch.zeros(B, H, Dk, v.shape[3], device=q.device) if state is None else state.clone()
+        return q.new_empty(B, H, T, v.shape[3]) + 0 * (q.sum() + k.sum() + v.sum()), st
+    st = None if state is None else state.contiguous()
+    return LinearAttnFn.apply(q, k, v, rate.contiguous(), st, valid_len, float(scale))
+
+
+def linear_attention_step(q, k, v, rate, state, *, scale: float = 1.0, active=None):
+    """One position of linear_attention for every sequence (serving): state [B,H,Dk,Dv] fp32, dense, is updated IN PLACE to
+    exp(-rate_h) state + k v^T; returns scale * q^T state, [B,H,Dv].
+
+    q [B,H,Dk], k [B,Hk,Dk], v [B,Hk,Dv] in fp32, bf16 or fp16; Dk, Dv <= 1024.  active [B] (bool or uint8): sequences with
+    0 keep their state and get zeros.  No gradients: raises where one would be expected."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, rate, state)):
+        raise RuntimeError("linear_attention_step: no gradients (linear_attention has them): call it under torch.no_grad()")
+    if q.dim() != 3:
+        raise ValueError(f"linear_attention_step: q is {tuple(q.shape)}, needs [B,H,Dk]")
+    _check_linear("linear_attention_step", q, k, v, rate, state, 3, LATTN_STEP_MAX_D)
+    if not state.is_contiguous():
+        raise ValueError("linear_attention_step: the state is updated in place and has to be dense")
+    B, H, Dk = q.shape
+    Dv = v.shape[2]
+    if active is not None:
+        _same_device("linear_attention_step", q, active=active)
+        if active.shape != (B,) or active.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"linear_attention_step: active is {active.dtype} {tuple(active.shape)}, needs bool or uint8 [{B}]")
+        active = active.contiguous()
+    out = torch.empty(B, H, Dv, dtype=q.dtype, device=q.device)
+    if B * H == 0:
+        return out
+    q, k, v = _rows4(q), _rows4(k), _rows4(v)
+    a = new("ic_lattn_step_args", B=B, H=H, Hk=k.shape[1], Dk=Dk, Dv=Dv, dtype=DTYPES[q.dtype], scale=float(scale), rate=rate.contiguous(),
+            active=None if active is None else active.view(torch.uint8), state=state, q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out)
+    for n, t in (("q", q), ("k", k), ("v", v), ("o", out)):
+        _strides(a, n, t, 2)
+    with _on(q):
+        _call("ic_lattn_step", a)
+    torch.autograd.graph.increment_version(state)
+    return out
+
+
 def hebbian_rank1(W: torch.Tensor, dst_of_edge: torch.Tensor, src: torch.Tensor, widx: torch.Tensor,
                   coef: torch.Tensor, H: torch.Tensor) -> None:
     """In-place W[widx[e]] += sum_b coef[b,e] * outer(H[b,dst_e], H[b,src_e])."""
