@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 from typing import Dict, List, Tuple
 
 _PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -144,6 +145,38 @@ def new(struct_name: str, **kw):
     for k, v in kw.items():
         set_field(obj, k, v)
     return obj
+
+
+_FORMATS = {ctypes.c_void_p: "P", ctypes.c_int32: "i", ctypes.c_int: "i", ctypes.c_int64: "q", ctypes.c_float: "f",
+            ctypes.c_double: "d", ctypes.c_uint8: "B"}
+
+
+def packer(struct_name: str):
+    """A function from keyword arguments to the bytes of a C struct, for entry points called per token or per layer: one
+    struct.pack (2 us for 45 fields) instead of an attribute assignment per field (0.3 us each).  Members of a member
+    struct are named <member>_<field>; pointers are device addresses; what is left out is 0 / NULL."""
+    names: List[str] = []
+    fmt = "="
+
+    def walk(cls, prefix: str, base: int) -> None:
+        nonlocal fmt
+        for name, ct in cls._fields_:
+            at = base + getattr(cls, name).offset
+            if isinstance(ct, type) and issubclass(ct, ctypes.Structure):
+                walk(ct, f"{prefix}{name}_", at)
+            else:
+                fmt += "x" * (at - struct.calcsize(fmt)) + _FORMATS[ct].replace("P", "Q")
+                names.append(prefix + name)
+
+    cls = CLASSES[struct_name]
+    walk(cls, "", 0)
+    pack = struct.Struct(fmt + "x" * (ctypes.sizeof(cls) - struct.calcsize(fmt))).pack
+    assert len(set(names)) == len(names), struct_name
+    scope = {"pack": pack}
+    exec(f"def fill({', '.join('*' * (i == 0) + (', ' if i == 0 else '') + n + '=0' for i, n in enumerate(names))}): return pack({', '.join(names)})", scope)
+    fill = scope["fill"]
+    fill.__name__ = fill.__qualname__ = f"pack_{struct_name}"
+    return fill
 
 
 def ptr(t) -> int:

@@ -6,7 +6,6 @@ gradients are deferred to one ic_*_wgrad launch per backward pass through a tape
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 from typing import Callable, Dict, List, Optional
@@ -14,7 +13,7 @@ from typing import Callable, Dict, List, Optional
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import ENUMS, check, lib, new, ptr, stream_handle
+from . import ENUMS, check, lib, new, packer, ptr, stream_handle
 
 IC_F_AFD = ENUMS["IC_F_AFD"]
 IC_F_RT = ENUMS["IC_F_RT"]
@@ -920,12 +919,21 @@ def attention(q, k, v, valid_len=None, alpha=None, lag_dt: float = 1.0, eps_log:
 DTYPES = {torch.float32: ENUMS["IC_DT_F32"], torch.bfloat16: ENUMS["IC_DT_BF16"], torch.float16: ENUMS["IC_DT_F16"]}
 ROPE_LAYOUTS = {"interleaved": ENUMS["IC_ROPE_INTERLEAVED"], "half": ENUMS["IC_ROPE_HALF"]}
 ROPE_MAX_D = 512
-_NO_GUARD = contextlib.nullcontext()
+ROPE_PARTS = 1024  # workgroups (partial sums of the norm weights' gradients) of ic_rope_bwd: ic_rope_parts()
+_pack_rope, _pack_rope_bwd = packer("ic_rope_args"), packer("ic_rope_bwd_args")
 
 
-def _on(t: torch.Tensor):
-    """The launches below go to the tensors' own device (its current stream), whatever the current device is."""
-    return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _launch(name: str, blob: bytes, device: torch.device) -> None:
+    """One C call with a packed argument struct, on the tensors' own device (its current stream), whatever the current
+    device is."""
+    fn = getattr(lib(), name)
+    if device.index == torch._C._cuda_getDevice():
+        rc = fn(blob, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(blob, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc:
+        check(rc, name)
 
 
 def _same_device(who: str, first: torch.Tensor, **others) -> None:
@@ -936,104 +944,116 @@ def _same_device(who: str, first: torch.Tensor, **others) -> None:
             raise RuntimeError(f"{who}: {n} is on {t.device}, the rows are on {first.device}")
 
 
+def _addr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def _rows4(t: torch.Tensor) -> torch.Tensor:
     """Rows whose channels lie side by side (any strides of the other dimensions)."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _empty_in_order(shape, strides, dtype, device) -> torch.Tensor:
-    """A dense [B,H,T,D] tensor whose dimensions lie in memory in the order of the given strides (D innermost): the
+def _dense_order(t: torch.Tensor) -> list:
+    """Strides of a dense [B,H,T,D] tensor whose dimensions lie in memory in the order of t's, channels side by side: the
     gradient of a [B,T,H,D]-ordered view comes back in that order."""
-    o = sorted((0, 1, 2), key=lambda i: -strides[i])
-    return torch.empty([shape[i] for i in o] + [shape[3]], dtype=dtype, device=device).permute([o.index(i) for i in (0, 1, 2)] + [3])
+    shape, stride = t.shape, t.stride()
+    out, n = [0, 0, 0, 1], shape[3]
+    for i in sorted((0, 1, 2), key=stride.__getitem__):
+        out[i] = n
+        n *= shape[i]
+    return out
 
 
-class _Angles:
-    """Checked angles of a rotation: tables cos / sin, or positions and frequencies."""
-
-    def __init__(self, who, q, cos, sin, positions, freqs, layout, scale):
-        B, _, T, D = q.shape
-        if layout not in ROPE_LAYOUTS:
-            raise ValueError(f"{who}: layout {layout!r} (one of {sorted(ROPE_LAYOUTS)})")
-        if (cos is None) != (sin is None) or (cos is None) == (freqs is None):
-            raise ValueError(f"{who}: angles are given either as cos and sin or as freqs (with positions)")
-        if cos is not None and positions is not None:
-            raise ValueError(f"{who}: positions go with freqs, not with cos / sin")
-        _same_device(who, q, cos=cos, sin=sin, positions=positions, freqs=freqs)
-        if any(t is not None and t.requires_grad for t in (cos, sin, freqs)):
-            raise RuntimeError(f"{who}: no gradient reaches the angles (cos, sin, freqs): detach them")
-        self.scale, self.layout = float(scale), ROPE_LAYOUTS[layout]
-        if cos is not None:
-            for n, t in (("cos", cos), ("sin", sin)):
-                if t.dtype != torch.float32 or t.shape != cos.shape or t.dim() not in (2, 3) or t.shape[-2] != T or (t.dim() == 3 and t.shape[0] not in (1, B)):
-                    raise ValueError(f"{who}: {n} is {t.dtype} {tuple(t.shape)}, needs fp32 [T,m], [1,T,m] or [B,T,m] with B={B}, T={T}")
-            self.m = cos.shape[-1]
-            self.cos, self.sin, self.pos, self.freqs = cos.contiguous(), sin.contiguous(), None, None
-            self.sb = T * self.m if cos.dim() == 3 and cos.shape[0] == B and B > 1 else 0
-        else:
-            if freqs.dim() != 1 or freqs.dtype not in (torch.float32, torch.float64):
-                raise ValueError(f"{who}: freqs is {freqs.dtype} {tuple(freqs.shape)}, needs fp32 or fp64 [m]")
-            self.m = freqs.shape[0]
-            self.sb = 0
-            if positions is not None:
-                if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((T,), (1, T), (B, T)):
-                    raise ValueError(f"{who}: positions is {positions.dtype} {tuple(positions.shape)}, needs int32 or int64 [T], [1,T] or [B,T] with B={B}, T={T}")
-                positions = positions.contiguous()
-                self.sb = T if positions.dim() == 2 and positions.shape[0] == B and B > 1 else 0
-            self.cos = self.sin = None
-            self.pos, self.freqs = positions, freqs.contiguous()
-        if 2 * self.m > D:
-            raise ValueError(f"{who}: {self.m} rotated pairs do not fit rows of {D} channels")
-
-    def fill(self, a) -> None:
-        a.m, a.layout, a.scale = self.m, self.layout, self.scale
-        if self.cos is not None:
-            a.cos, a.sin, a.cs_sb = self.cos.data_ptr(), self.sin.data_ptr(), self.sb
-        else:
-            a.freqs, a.freq64 = self.freqs.data_ptr(), int(self.freqs.dtype == torch.float64)
-            if self.pos is not None:
-                a.positions, a.pos64, a.pos_sb = self.pos.data_ptr(), int(self.pos.dtype == torch.int64), self.sb
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
-def _rope_args(ang: _Angles, rows, inverse: int = 0, eps: float = 0.0):
-    """ic_rope_args for [(x, y, weight), ...] (q, and k if there is one)."""
-    B, _, T, D = rows[0][0].shape
-    a = new("ic_rope_args", B=B, T=T, D=D, dtype=DTYPES[rows[0][0].dtype], inverse=inverse, eps=eps)
-    ang.fill(a)
-    for r, (x, y, w) in zip((a.q, a.k), rows):
-        r.H, r.x = x.shape[1], x.data_ptr()
-        r.x_sb, r.x_sh, r.x_st = x.stride()[:3]
+def _angles(who, q, cos, sin, positions, freqs, layout, scale):
+    """Checked angles of a rotation -- tables cos / sin, or positions and frequencies -- as the fields of ic_rope_args, and
+    the tensors that hold them."""
+    B, _, T, D = q.shape
+    if layout not in ROPE_LAYOUTS:
+        raise ValueError(f"{who}: layout {layout!r} (one of {sorted(ROPE_LAYOUTS)})")
+    if (cos is None) != (sin is None) or (cos is None) == (freqs is None):
+        raise ValueError(f"{who}: angles are given either as cos and sin or as freqs (with positions)")
+    if cos is not None and positions is not None:
+        raise ValueError(f"{who}: positions go with freqs, not with cos / sin")
+    _same_device(who, q, cos=cos, sin=sin, positions=positions, freqs=freqs)
+    f = dict(layout=ROPE_LAYOUTS[layout], scale=float(scale))
+    if cos is not None:
+        for n, t in (("cos", cos), ("sin", sin)):
+            if t.dtype != torch.float32 or t.shape != cos.shape or t.dim() not in (2, 3) or t.shape[-2] != T or (t.dim() == 3 and t.shape[0] not in (1, B)):
+                raise ValueError(f"{who}: {n} is {t.dtype} {tuple(t.shape)}, needs fp32 [T,m], [1,T,m] or [B,T,m] with B={B}, T={T}")
+        if cos.requires_grad or sin.requires_grad:
+            raise RuntimeError(f"{who}: no gradient reaches the angles (cos, sin): detach them")
+        m = cos.shape[-1]
+        cos, sin = cos.contiguous(), sin.contiguous()
+        f.update(m=m, cos=cos.data_ptr(), sin=sin.data_ptr(), cs_sb=T * m if cos.dim() == 3 and cos.shape[0] == B and B > 1 else 0)
+        hold = (cos, sin)
+    else:
+        if freqs.dim() != 1 or freqs.dtype not in (torch.float32, torch.float64):
+            raise ValueError(f"{who}: freqs is {freqs.dtype} {tuple(freqs.shape)}, needs fp32 or fp64 [m]")
+        if freqs.requires_grad:
+            raise RuntimeError(f"{who}: no gradient reaches the angles (freqs): detach them")
+        m = freqs.shape[0]
+        freqs = freqs.contiguous()
+        f.update(m=m, freqs=freqs.data_ptr(), freq64=int(freqs.dtype == torch.float64))
+        hold = (freqs,)
+        if positions is not None:
+            if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((T,), (1, T), (B, T)):
+                raise ValueError(f"{who}: positions is {positions.dtype} {tuple(positions.shape)}, needs int32 or int64 [T], [1,T] or [B,T] with B={B}, T={T}")
+            positions = positions.contiguous()
+            f.update(positions=positions.data_ptr(), pos64=int(positions.dtype == torch.int64),
+                     pos_sb=T if positions.dim() == 2 and positions.shape[0] == B and B > 1 else 0)
+            hold = (freqs, positions)
+    if 2 * m > D:
+        raise ValueError(f"{who}: {m} rotated pairs do not fit rows of {D} channels")
+    return f, hold
+
+
+def _rope_fields(ang, q, k, yq=None, yk=None, wq=None, wk=None, eps: float = 0.0, inverse: int = 0, pre: str = "") -> dict:
+    """Fields of ic_rope_args (`pre`: as a member of another struct)."""
+    B, H, T, D = q.shape
+    f = dict(ang, B=B, T=T, D=D, dtype=DTYPES[q.dtype], inverse=inverse, eps=eps)
+    for n, x, y, w in (("q", q, yq, wq), ("k", k, yk, wk)):
+        if x is None:
+            continue
+        f[n + "_H"], f[n + "_x"] = x.shape[1], x.data_ptr()
+        f[n + "_x_sb"], f[n + "_x_sh"], f[n + "_x_st"], _ = x.stride()
         if y is not None:
-            r.y = y.data_ptr()
-            r.y_sb, r.y_sh, r.y_st = y.stride()[:3]
+            f[n + "_y"] = y.data_ptr()
+            f[n + "_y_sb"], f[n + "_y_sh"], f[n + "_y_st"], _ = y.stride()
         if w is not None:
-            r.w, r.w_dtype = w.data_ptr(), DTYPES[w.dtype]
-    return a
+            f[n + "_w"], f[n + "_w_dtype"] = w.data_ptr(), DTYPES[w.dtype]
+    return {pre + n: v for n, v in f.items()} if pre else f
+
+
+def _rope_run(ang, q, k, wq=None, wk=None, eps: float = 0.0):
+    yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    yk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    _launch("ic_rope_fwd", _pack_rope(**_rope_fields(ang, q, k, yq, yk, wq, wk, eps)), q.device)
+    return yq, yk
 
 
 class RopeFn(torch.autograd.Function):
     """Rotated queries (and keys) in one launch (ic_rope_fwd); the backward is the rotation by the negative angles."""
 
     @staticmethod
-    def forward(ctx, q, k, ang):
-        xs = [_rows4(t) for t in (q, k) if t is not None]
-        ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
-        with _on(q):
-            _call("ic_rope_fwd", _rope_args(ang, [(x, y, None) for x, y in zip(xs, ys)]))
-        ctx.like = [x.stride() for x in xs]
+    def forward(ctx, q, k, ang, *hold):
+        ctx.save_for_backward(*hold)  # (so that angles changed in place raise)
         ctx.ang = ang
-        ctx.save_for_backward(ang.cos, ang.sin, ang.pos, ang.freqs)  # (so that angles changed in place raise)
-        return ys[0], (ys[1] if len(ys) > 1 else None)
+        ctx.order = [_dense_order(t) for t in (q, k) if t is not None]
+        return _rope_run(ang, q, k)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
-        ctx.saved_tensors
-        gs = [_rows4(g) for g in (gq, gk)[:len(ctx.like)]]
-        outs = [_empty_in_order(g.shape, st, g.dtype, g.device) for g, st in zip(gs, ctx.like)]
-        with _on(gs[0]):
-            _call("ic_rope_fwd", _rope_args(ctx.ang, [(g, o, None) for g, o in zip(gs, outs)], inverse=1))
-        return outs[0], (outs[1] if len(outs) > 1 else None), None
+        hold = ctx.saved_tensors
+        gq, gk = _rows4(gq), _rows4(gk) if len(ctx.order) > 1 else None
+        oq = torch.empty_strided(gq.shape, ctx.order[0], dtype=gq.dtype, device=gq.device)
+        ok = None if gk is None else torch.empty_strided(gk.shape, ctx.order[1], dtype=gk.dtype, device=gk.device)
+        _launch("ic_rope_fwd", _pack_rope(**_rope_fields(ctx.ang, gq, gk, oq, ok, inverse=1)), gq.device)
+        return (oq, ok, None) + (None,) * len(hold)
 
 
 class QKNormRopeFn(torch.autograd.Function):
@@ -1041,35 +1061,32 @@ class QKNormRopeFn(torch.autograd.Function):
     (ic_rope_bwd) reads the rows again instead of keeping their norms."""
 
     @staticmethod
-    def forward(ctx, q, k, wq, wk, ang, eps):
-        xs = [_rows4(q), _rows4(k)]
-        ws = [wq.contiguous(), wk.contiguous()]
-        ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
-        with _on(q):
-            _call("ic_rope_fwd", _rope_args(ang, list(zip(xs, ys, ws)), eps=eps))
+    def forward(ctx, q, k, wq, wk, ang, eps, *hold):
+        ctx.save_for_backward(q, k, wq, wk, *hold)
         ctx.ang, ctx.eps = ang, eps
-        ctx.save_for_backward(*xs, *ws, ang.cos, ang.sin, ang.pos, ang.freqs)
-        return ys[0], ys[1]
+        return _rope_run(ang, q, k, wq, wk, eps)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
-        xq, xk, wq, wk = ctx.saved_tensors[:4]
-        gs = [_rows4(gq), _rows4(gk)]
-        outs = [_empty_in_order(x.shape, x.stride(), x.dtype, x.device) for x in (xq, xk)]
-        gws = [torch.empty_like(wq), torch.empty_like(wk)]
-        part = torch.empty(ROPE_PARTS, xq.shape[-1], device=xq.device)
-        b = new("ic_rope_bwd_args", f=_rope_args(ctx.ang, [(xq, None, wq), (xk, None, wk)], eps=ctx.eps), part=part)
-        for r, g, o, gw in zip((b.q, b.k), gs, outs, gws):
-            r.g, r.gx, r.gw = g.data_ptr(), o.data_ptr(), gw.data_ptr()
-            r.g_sb, r.g_sh, r.g_st = g.stride()[:3]
-            r.gx_sb, r.gx_sh, r.gx_st = o.stride()[:3]
-        with _on(xq):
-            _call("ic_rope_bwd", b)
-        return outs[0], outs[1], gws[0], gws[1], None, None
-
-
-ROPE_PARTS = 1024  # workgroups (partial sums of the norm weights' gradients) of ic_rope_bwd: ic_rope_parts()
+        q, k, wq, wk, *hold = ctx.saved_tensors
+        dev = q.device
+        f = _rope_fields(ctx.ang, q, k, None, None, wq, wk, ctx.eps, pre="f_")
+        part = torch.empty(ROPE_PARTS * q.shape[3], device=dev)
+        f["part"] = part.data_ptr()
+        gws, outs, keep = [], [], []
+        for n, x, w, g in (("q", q, wq, gq), ("k", k, wk, gk)):
+            g = _rows4(g)
+            gx = torch.empty_strided(x.shape, _dense_order(x), dtype=x.dtype, device=dev)
+            gw = torch.empty_like(w)
+            f[n + "_g"], f[n + "_gx"], f[n + "_gw"] = g.data_ptr(), gx.data_ptr(), gw.data_ptr()
+            f[n + "_g_sb"], f[n + "_g_sh"], f[n + "_g_st"], _ = g.stride()
+            f[n + "_gx_sb"], f[n + "_gx_sh"], f[n + "_gx_st"], _ = gx.stride()
+            keep.append(g)
+            outs.append(gx)
+            gws.append(gw)
+        _launch("ic_rope_bwd", _pack_rope_bwd(**f), dev)
+        return (*outs, *gws, None, None) + (None,) * len(hold)
 
 
 def _check_qk(who, q, k) -> None:
@@ -1089,10 +1106,11 @@ def rope(q, k=None, *, cos=None, sin=None, positions=None, freqs=None, layout: s
     0 .. T-1), whose product is formed in 64 bits.  scale multiplies both cos and sin (the rotated channels).
     Returns dense [B,H,T,D] rows: the rotated q, or (q, k).  Gradients reach q and k."""
     _check_qk("rope", q, k)
-    ang = _Angles("rope", q, cos, sin, positions, freqs, layout, scale)
+    ang, hold = _angles("rope", q, cos, sin, positions, freqs, layout, scale)
     if q.numel() == 0 or (k is not None and k.numel() == 0):
         return (q.clone(), k.clone()) if k is not None else q.clone()
-    yq, yk = RopeFn.apply(q, k, ang)
+    q, k = _rows4(q), None if k is None else _rows4(k)
+    yq, yk = RopeFn.apply(q, k, ang, *hold) if _wants_grad(q, k) else _rope_run(ang, q, k)
     return yq if k is None else (yq, yk)
 
 
@@ -1108,41 +1126,61 @@ def qk_norm_rope(q, k, q_weight, k_weight, *, eps: float = 1e-5, cos=None, sin=N
             raise ValueError(f"qk_norm_rope: {n} is {w.dtype} {tuple(w.shape)}, needs fp32 or {q.dtype} [{q.shape[3]}]")
     if q.shape[1] + k.shape[1] > ROPE_PARTS:
         raise ValueError(f"qk_norm_rope: {q.shape[1]} + {k.shape[1]} heads (at most {ROPE_PARTS})")
-    ang = _Angles("qk_norm_rope", q, cos, sin, positions, freqs, layout, scale)
+    ang, hold = _angles("qk_norm_rope", q, cos, sin, positions, freqs, layout, scale)
     if q.numel() == 0 or k.numel() == 0:
         return q * q_weight.to(q.dtype), k * k_weight.to(k.dtype)
-    return QKNormRopeFn.apply(q, k, q_weight, k_weight, ang, float(eps))
+    q, k, q_weight, k_weight = _rows4(q), _rows4(k), q_weight.contiguous(), k_weight.contiguous()
+    if _wants_grad(q, k, q_weight, k_weight):
+        return QKNormRopeFn.apply(q, k, q_weight, k_weight, ang, float(eps), *hold)
+    return _rope_run(ang, q, k, q_weight, k_weight, float(eps))
 
 
 # ---------------------------------------------------------------- linear attention with a decay for each head
 LATTN_MAX_D = 128        # channels of a head's keys and values
 LATTN_STEP_MAX_D = 1024  # the same for single positions
+_pack_lattn, _pack_lattn_bwd, _pack_lattn_step = packer("ic_lattn_args"), packer("ic_lattn_bwd_args"), packer("ic_lattn_step_args")
 
 
-def _strides(obj, name: str, t: torch.Tensor, n: int) -> None:
-    for f, s in zip(("sb", "sh", "st")[:n], t.stride()):
-        setattr(obj, f"{name}_{f}", s)
-
-
-def _lattn_args(q, k, v, rate, valid_len, state, scale, out=None, state_out=None):
+def _lattn_fields(q, k, v, rate, valid_len, state, scale) -> dict:
     B, H, T, Dk = q.shape
-    a = new("ic_lattn_args", B=B, H=H, Hk=k.shape[1], T=T, Dk=Dk, Dv=v.shape[3], dtype=DTYPES[q.dtype], scale=scale, rate=rate,
-            valid_len=valid_len, state=state, state_out=state_out)
-    for n, t in (("q", q), ("k", k), ("v", v), ("o", out)):
-        if t is not None:
-            setattr(a, "out" if n == "o" else n, t.data_ptr())
-            _strides(a, n, t, 3)
-    return a
+    f = dict(B=B, H=H, Hk=k.shape[1], T=T, Dk=Dk, Dv=v.shape[3], dtype=DTYPES[q.dtype], scale=scale, q=q.data_ptr(), k=k.data_ptr(),
+             v=v.data_ptr(), rate=rate.data_ptr(), valid_len=_addr(valid_len), state=_addr(state))
+    f["q_sb"], f["q_sh"], f["q_st"], _ = q.stride()
+    f["k_sb"], f["k_sh"], f["k_st"], _ = k.stride()
+    f["v_sb"], f["v_sh"], f["v_st"], _ = v.stride()
+    return f
 
 
-def _lattn_ws(a, backward: int, device) -> Optional[torch.Tensor]:
-    n = ctypes.c_int64(0)
-    check(lib().ic_lattn_ws(ctypes.byref(a), backward, ctypes.byref(n)), "ic_lattn_ws")
-    if n.value == 0:
+_LATTN_WS: Dict[tuple, int] = {}  # workspace floats by sizes (a pure function of them)
+
+
+def _lattn_ws(f: dict, backward: int, device) -> Optional[torch.Tensor]:
+    """Workspace of a call (held by the caller until its launches are queued; the allocator orders reuse on the stream)."""
+    key = (f["B"], f["H"], f["Hk"], f["T"], f["Dk"], f["Dv"], f["dtype"], backward)
+    n = _LATTN_WS.get(key)
+    if n is None:
+        got = ctypes.c_int64(0)
+        check(lib().ic_lattn_ws(_pack_lattn(**f), backward, ctypes.byref(got)), "ic_lattn_ws")
+        if len(_LATTN_WS) > 4096:
+            _LATTN_WS.clear()
+        n = _LATTN_WS[key] = got.value
+    if n == 0:
         return None
-    ws = torch.empty(n.value, dtype=torch.float32, device=device)
-    a.ws = ws.data_ptr()
-    return ws  # (held by the caller until the launches are queued; the allocator orders reuse on this stream)
+    ws = torch.empty(n, dtype=torch.float32, device=device)
+    f["ws"] = ws.data_ptr()
+    return ws
+
+
+def _lattn_run(q, k, v, rate, state, valid_len, scale):
+    B, H, T, Dk = q.shape
+    Dv, dev = v.shape[3], q.device
+    out = torch.empty((B, T, H, Dv), dtype=q.dtype, device=dev).transpose(1, 2)
+    state_out = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=dev)
+    f = _lattn_fields(q, k, v, rate, valid_len, state, scale)
+    ws = _lattn_ws(f, 0, dev)  # noqa: F841
+    sb, sh, st, _ = out.stride()
+    _launch("ic_lattn_fwd", _pack_lattn(**f, out=out.data_ptr(), o_sb=sb, o_sh=sh, o_st=st, state_out=state_out.data_ptr()), dev)
+    return out, state_out
 
 
 class LinearAttnFn(torch.autograd.Function):
@@ -1150,19 +1188,10 @@ class LinearAttnFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, rate, state, valid_len, scale):
-        q, k, v = _rows4(q), _rows4(k), _rows4(v)
-        B, H, T, Dk = q.shape
-        Dv = v.shape[3]
-        out = torch.empty(B, T, H, Dv, dtype=q.dtype, device=q.device).transpose(1, 2)
-        state_out = torch.empty(B, H, Dk, Dv, device=q.device)
-        a = _lattn_args(q, k, v, rate, valid_len, state, scale, out, state_out)
-        with _on(q):
-            ws = _lattn_ws(a, 0, q.device)  # noqa: F841
-            _call("ic_lattn_fwd", a)
         ctx.save_for_backward(q, k, v, rate, state, valid_len)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
-        return out, state_out
+        return _lattn_run(q, k, v, rate, state, valid_len, scale)
 
     @staticmethod
     @once_differentiable
@@ -1171,19 +1200,24 @@ class LinearAttnFn(torch.autograd.Function):
         if gout is None and gstate is None:
             return (None,) * 7
         B, H, T, Dk = q.shape
-        gout = torch.zeros(B, H, T, v.shape[3], dtype=q.dtype, device=q.device) if gout is None else _rows4(gout)
-        dq, dk, dv = (_empty_in_order(t.shape, t.stride(), t.dtype, t.device) for t in (q, k, v))
+        dev = q.device
+        gout = torch.zeros((B, H, T, v.shape[3]), dtype=q.dtype, device=dev) if gout is None else _rows4(gout)
+        gstate = None if gstate is None else gstate.contiguous()
         drate = torch.empty_like(rate) if ctx.needs_input_grad[3] else None
         dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
-        f = _lattn_args(q, k, v, rate, valid_len, state, ctx.scale)
-        with _on(q):
-            ws = _lattn_ws(f, 1, q.device)  # noqa: F841
-            b = new("ic_lattn_bwd_args", f=f, dout=gout.data_ptr(), dstate_out=None if gstate is None else gstate.contiguous(),
-                    dq=dq.data_ptr(), dk=dk.data_ptr(), dv=dv.data_ptr(), drate=drate, dstate=dstate)
-            for n, t in (("do", gout), ("dq", dq), ("dk", dk), ("dv", dv)):
-                _strides(b, n, t, 3)
-            _call("ic_lattn_bwd", b)
-        return dq, dk, dv, drate, dstate, None, None
+        f = _lattn_fields(q, k, v, rate, valid_len, state, ctx.scale)
+        ws = _lattn_ws(f, 1, dev)  # noqa: F841
+        f = {"f_" + n: x for n, x in f.items()}
+        f.update(dout=gout.data_ptr(), dstate_out=_addr(gstate), drate=_addr(drate), dstate=_addr(dstate))
+        f["do_sb"], f["do_sh"], f["do_st"], _ = gout.stride()
+        outs = []
+        for n, t in (("dq", q), ("dk", k), ("dv", v)):
+            g = torch.empty_strided(t.shape, _dense_order(t), dtype=t.dtype, device=dev)
+            f[n] = g.data_ptr()
+            f[n + "_sb"], f[n + "_sh"], f[n + "_st"], _ = g.stride()
+            outs.append(g)
+        _launch("ic_lattn_bwd", _pack_lattn_bwd(**f), dev)
+        return (*outs, drate, dstate, None, None)
 
 
 def _check_linear(who, q, k, v, rate, state, dims: int, most: int):
@@ -1192,9 +1226,10 @@ def _check_linear(who, q, k, v, rate, state, dims: int, most: int):
     say = lambda: f"{who}: q, k, v are {q.dtype} {tuple(q.shape)}, {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}"  # noqa: E731
     if q.dtype not in DTYPES or k.dtype != q.dtype or v.dtype != q.dtype or not (q.dim() == k.dim() == v.dim() == dims):
         raise ValueError(f"{say()}: needs one type of fp32, bf16, fp16 and {want}")
-    if k.shape[:-1] != v.shape[:-1] or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:] or (k.shape[1] == 0) != (q.shape[1] == 0) or (k.shape[1] and q.shape[1] % k.shape[1]):
+    sq, sk, sv = q.shape, k.shape, v.shape
+    B, H, Hk, Dk, Dv = sq[0], sq[1], sk[1], sq[-1], sv[-1]
+    if sk[:-1] != sv[:-1] or sk[0] != B or sk[2:] != sq[2:] or (Hk == 0) != (H == 0) or (Hk and H % Hk):
         raise ValueError(f"{say()}: needs {want} with H a multiple of Hk")
-    B, H, Dk, Dv = q.shape[0], q.shape[1], q.shape[-1], v.shape[-1]
     if not (1 <= Dk <= most and 1 <= Dv <= most):
         raise ValueError(f"{say()}: Dk and Dv must be 1 .. {most}")
     if rate.dtype != torch.float32 or rate.shape != (H,):
@@ -1220,14 +1255,16 @@ def linear_attention(q, k, v, rate, *, scale: float = 1.0, state=None, valid_len
         _same_device("linear_attention", q, valid_len=valid_len)
         if valid_len.shape != (B,) or valid_len.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"linear_attention: valid_len is {valid_len.dtype} {tuple(valid_len.shape)}, needs int32 or int64 [{B}]")
-        valid_len = valid_len.to(torch.int32).contiguous()
+        valid_len = valid_len.clamp(0, T).to(torch.int32).contiguous() if valid_len.dtype == torch.int64 else valid_len.contiguous()
     if B * H > 65535:
         raise ValueError(f"linear_attention: B * H = {B * H} (at most 65535)")
     if B * H * T == 0:
         st = torch.zeros(B, H, Dk, v.shape[3], device=q.device) if state is None else state.clone()
         return q.new_empty(B, H, T, v.shape[3]) + 0 * (q.sum() + k.sum() + v.sum()), st
-    st = None if state is None else state.contiguous()
-    return LinearAttnFn.apply(q, k, v, rate.contiguous(), st, valid_len, float(scale))
+    q, k, v, rate, state = _rows4(q), _rows4(k), _rows4(v), rate.contiguous(), None if state is None else state.contiguous()
+    if _wants_grad(q, k, v, rate, state):
+        return LinearAttnFn.apply(q, k, v, rate, state, valid_len, float(scale))
+    return _lattn_run(q, k, v, rate, state, valid_len, float(scale))
 
 
 def linear_attention_step(q, k, v, rate, state, *, scale: float = 1.0, active=None):
@@ -1236,7 +1273,7 @@ def linear_attention_step(q, k, v, rate, state, *, scale: float = 1.0, active=No
 
     q [B,H,Dk], k [B,Hk,Dk], v [B,Hk,Dv] in fp32, bf16 or fp16; Dk, Dv <= 1024.  active [B] (bool or uint8): sequences with
     0 keep their state and get zeros.  No gradients: raises where one would be expected."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, rate, state)):
+    if _wants_grad(q, k, v, rate, state):
         raise RuntimeError("linear_attention_step: no gradients (linear_attention has them): call it under torch.no_grad()")
     if q.dim() != 3:
         raise ValueError(f"linear_attention_step: q is {tuple(q.shape)}, needs [B,H,Dk]")
@@ -1244,22 +1281,21 @@ def linear_attention_step(q, k, v, rate, state, *, scale: float = 1.0, active=No
     if not state.is_contiguous():
         raise ValueError("linear_attention_step: the state is updated in place and has to be dense")
     B, H, Dk = q.shape
-    Dv = v.shape[2]
+    Dv, dev = v.shape[2], q.device
     if active is not None:
         _same_device("linear_attention_step", q, active=active)
         if active.shape != (B,) or active.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"linear_attention_step: active is {active.dtype} {tuple(active.shape)}, needs bool or uint8 [{B}]")
         active = active.contiguous()
-    out = torch.empty(B, H, Dv, dtype=q.dtype, device=q.device)
+    out = torch.empty((B, H, Dv), dtype=q.dtype, device=dev)
     if B * H == 0:
         return out
-    q, k, v = _rows4(q), _rows4(k), _rows4(v)
-    a = new("ic_lattn_step_args", B=B, H=H, Hk=k.shape[1], Dk=Dk, Dv=Dv, dtype=DTYPES[q.dtype], scale=float(scale), rate=rate.contiguous(),
-            active=None if active is None else active.view(torch.uint8), state=state, q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out)
-    for n, t in (("q", q), ("k", k), ("v", v), ("o", out)):
-        _strides(a, n, t, 2)
-    with _on(q):
-        _call("ic_lattn_step", a)
+    q, k, v, rate = _rows4(q), _rows4(k), _rows4(v), rate.contiguous()
+    (q_sb, q_sh, _), (k_sb, k_sh, _), (v_sb, v_sh, _) = q.stride(), k.stride(), v.stride()
+    _launch("ic_lattn_step", _pack_lattn_step(
+        B=B, H=H, Hk=k.shape[1], Dk=Dk, Dv=Dv, dtype=DTYPES[q.dtype], scale=scale, q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(),
+        q_sb=q_sb, q_sh=q_sh, k_sb=k_sb, k_sh=k_sh, v_sb=v_sb, v_sh=v_sh, rate=rate.data_ptr(), active=_addr(active),
+        state=state.data_ptr(), out=out.data_ptr(), o_sb=H * Dv, o_sh=Dv), dev)
     torch.autograd.graph.increment_version(state)
     return out
 

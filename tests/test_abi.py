@@ -47,3 +47,22 @@ def test_ops_refuse_cpu_tensors():
     from ironcortex_amd.utils import KWTA
     with pytest.raises(RuntimeError):
         KWTA(torch.randn(2, 8), 2)
+
+
+def test_packed_structs_equal_the_assigned_ones():
+    """hip.packer: the same bytes as setting every field of the ctypes structure."""
+    def fill(obj, prefix, kw, n):
+        for name, ct in obj._fields_:
+            if isinstance(ct, type) and issubclass(ct, ctypes.Structure):
+                n = fill(getattr(obj, name), prefix + name + "_", kw, n)
+            else:
+                n += 1
+                setattr(obj, name, n)
+                kw[prefix + name] = n
+        return n
+
+    for s in ("ic_rope_args", "ic_rope_bwd_args", "ic_lattn_args", "ic_lattn_bwd_args", "ic_lattn_step_args"):
+        obj, kw = hip.CLASSES[s](), {}
+        fill(obj, "", kw, 0)
+        assert hip.packer(s)(**kw) == bytes(obj), s
+        assert hip.packer(s)() == bytes(hip.CLASSES[s]()), s
