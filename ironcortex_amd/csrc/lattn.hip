@@ -21,6 +21,8 @@
 // l holds rows 4 (l / 16) + 0..3 of column l % 16, and as an operand k-indices 4 (l / 16) + 0..3 of row / column l % 16).
 // Several segments per sequence only where sequences and heads do not fill the chip: their sums are formed first
 // (k_lattn SUMS), scanned (k_lattn_scan), and each segment starts from its own prefix.
+#include <type_traits>
+
 #include "ic_types.h"
 
 namespace {
@@ -131,6 +133,52 @@ template <int DP>
 struct LdsSums {
   float Ks[kC][DP + 4];
 };
+
+// the end of a segment: its sums, or (last segment) the end state; d rate's partial sum
+template <bool LAG, bool SUMS, int NT, typename LDS, int NL>
+__device__ __forceinline__ void finish(const Geo& g, const Pass* p, const Sums* sm, LDS& lds, const v4f (&S)[NT], const v4f (&L)[NL],
+                                       double dr, size_t dd, int Da, int Db, int col, int q4, int bh, int seg, int n, float l2) {
+  if constexpr (SUMS) {
+    float* dst = sm->seg + ((size_t)bh * g.nseg + seg) * (LAG ? 2 : 1) * dd;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int a = 16 * t + q4 + v;
+        if (a < Da && col < Db) {
+          dst[(size_t)a * Db + col] = S[t][v];
+          if constexpr (LAG) dst[dd + (size_t)a * Db + col] = L[t][v];
+        }
+      }
+  } else {
+    if (seg == g.nseg - 1) {
+      const float last = p->fin_decay && n > 0 ? decay(l2, 1) : 1.f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int a = 16 * t + q4 + v;
+          if (a < Da && col < Db) {
+            const size_t at = (size_t)bh * dd + (size_t)a * p->ia + (size_t)col * p->ib;
+            if (p->fin) p->fin[at] = S[t][v] * last;
+            if constexpr (LAG) {
+              if (p->gfin) dr -= (double)L[t][v] * (double)p->gfin[at];
+            }
+          }
+        }
+    }
+    if constexpr (LAG) {
+      for (int o = 32; o; o >>= 1) dr += __shfl_xor(dr, o, 64);
+      if ((threadIdx.x & 63) == 0) lds.red[threadIdx.x >> 6] = dr;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < NT; ++i) t += lds.red[i];  // (as many waves as 16-row tiles)
+        p->dr[(size_t)bh * g.nseg + seg] = t;
+      }
+    }
+  }
+}
 
 template <typename T, int DP, bool LAG, bool SUMS, typename LDS>
 __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Sums* sm, LDS& lds) {
@@ -314,57 +362,344 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
     }
     __syncthreads();
   }
-  if constexpr (SUMS) {
-    float* dst = sm->seg + ((size_t)bh * g.nseg + seg) * (LAG ? 2 : 1) * dd;
+  finish<LAG, SUMS, KS>(g, p, sm, lds, S, L, dr, dd, Da, Db, col, q4, bh, seg, n, l2);
+}
+
+// ------------------------------------------------------------------------------------------------ bf16 rows
+// The same map on bf16 matrix instructions (16x16x32: sixteen times the fp32 rate).  Products of rows (q . k) are exact
+// there.  Operands that are computed in fp32 -- the decayed products P, the state, the decay-weighted values -- are split
+// into bf16 parts (x = x1 + x2 [+ x3], each the rounded rest of the one before: 8 bits of the value apiece): two parts where
+// the sum ends in a bf16 output (2^-17 of a term against the output's own 2^-9), three where it ends in an fp32 one (the
+// state, d rate).  Rows lie in LDS as they come; column operands (k^T, v^T) are read with the transposing LDS load
+// (16 lanes x 8 bytes of four rows -> four rows of one column per lane).  A 32-deep operand of a lane is therefore k-indices
+// 4 q .. 4 q + 3 of either 16-row half, on both sides of a product; products of rows use contiguous eights instead.
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+constexpr int kPad16 = 16, kPw = kC + 8;
+
+template <int DP>
+struct RowTile {
+  uint16_t r[kC][DP + kPad16];  // 32 bytes of padding: the transposing reads of 8 rows and the 16-byte reads of 8 rows spread over the banks
+};
+template <int DP, bool LAG>
+struct Lds16 {
+  RowTile<DP> K, V, Q;
+  RowTile<LAG ? DP : 16> X;
+  uint16_t P1[kC][kPw], P2[kC][kPw];
+  double red[DP / 16];
+};
+template <int DP>
+struct LdsSums16 {
+  RowTile<DP> K, V;
+};
+
+__device__ __forceinline__ v4f mma32(b8 a, b8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ b8 lds16(const uint16_t* p) { return *reinterpret_cast<const b8*>(p); }
+__device__ __forceinline__ b8 lds8x2(const uint16_t* p) {  // k-indices p[0..3] and p[16..19]
+  union { uint64_t u[2]; b8 b; } x;
+  x.u[0] = *reinterpret_cast<const uint64_t*>(p);
+  x.u[1] = *reinterpret_cast<const uint64_t*>(p + 16);
+  return x.b;
+}
+// rows [r0, r0 + 32) of column c0 + lane % 16: k-indices 4 (lane / 16) + 0..3 of either half
+template <int W>
+__device__ __forceinline__ b8 lds_col(const uint16_t (*t)[W], int r0, int c0, int lane) {
+  const int c = lane & 15, q = lane >> 4;
+  const uint16_t* p = &t[r0 + 4 * q + (c >> 2)][c0 + 4 * (c & 3)];
+  union { s4v s[2]; b8 b; } x;
+  x.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)p);
+  x.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)(p + 16 * W));
+  return x.b;
+}
+// bf16 parts of eight fp32 values; x keeps the rest
+__device__ __forceinline__ b8 take_part(float (&x)[8]) {
+  b8 p;
 #pragma unroll
-    for (int t = 0; t < KS; ++t)
+  for (int u = 0; u < 8; ++u) {
+    p[u] = (__bf16)x[u];
+    x[u] -= (float)p[u];
+  }
+  return p;
+}
+template <int N>
+__device__ __forceinline__ void split(const v4f& a, const v4f& b, b8 (&out)[N]) {
+  float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int a = 16 * t + q4 + v;
-        if (a < Da && col < Db) {
-          dst[(size_t)a * Db + col] = S[t][v];
-          if (LAG) dst[dd + (size_t)a * Db + col] = L[t][v];
-        }
-      }
-  } else {
-    if (seg == g.nseg - 1) {
-      const float last = p->fin_decay && n > 0 ? decay(l2, 1) : 1.f;
+  for (int i = 0; i < N; ++i) out[i] = take_part(x);
+}
+
+// 16-byte pieces of a tile's rows in flight: fetch (global -> registers), put (registers -> LDS)
+template <int DP>
+struct Piece {
+  uint4 x[2];  // kC rows x DP / 8 pieces over 4 DP threads
+};
+template <int DP>
+__device__ __forceinline__ void fetch16(Piece<DP>& t, const uint16_t* src, const Mat& m, int D, int base, int cnt, int n, int rev) {
+  constexpr int PER = DP / 8, RT = 32;  // (4 DP threads: 32 rows at a time)
 #pragma unroll
-      for (int t = 0; t < KS; ++t)
+  for (int j = 0; j < 2; ++j) {
+    const int r = threadIdx.x / PER + RT * j, c = (threadIdx.x % PER) * 8;
+    t.x[j] = make_uint4(0, 0, 0, 0);
+    if (r < cnt) {
+      const uint16_t* row = src + (int64_t)(rev ? n - 1 - (base + r) : base + r) * m.st;
+      if (m.vec) {
+        if (c < D) t.x[j] = *reinterpret_cast<const uint4*>(row + c);
+      } else {
+        uint32_t e[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int a = 16 * t + q4 + v;
-          if (a < Da && col < Db) {
-            const size_t at = (size_t)bh * dd + (size_t)a * p->ia + (size_t)col * p->ib;
-            if (p->fin) p->fin[at] = S[t][v] * last;
-            if (LAG && p->gfin) dr -= (double)L[t][v] * (double)p->gfin[at];
-          }
-        }
-    }
-    if (LAG) {
-      for (int o = 32; o; o >>= 1) dr += __shfl_xor(dr, o, 64);
-      if (lane == 0) lds.red[w] = dr;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        double t = 0.0;
-        for (int i = 0; i < NW; ++i) t += lds.red[i];
-        p->dr[(size_t)bh * g.nseg + seg] = t;
+        for (int u = 0; u < 8; ++u)
+          if (c + u < D) e[u >> 1] |= (uint32_t)row[c + u] << (16 * (u & 1));
+        t.x[j] = make_uint4(e[0], e[1], e[2], e[3]);
       }
     }
   }
 }
+template <int DP>
+__device__ __forceinline__ void put16(RowTile<DP>& dst, const Piece<DP>& t) {
+  constexpr int PER = DP / 8, RT = 32;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) *reinterpret_cast<uint4*>(&dst.r[threadIdx.x / PER + RT * j][(threadIdx.x % PER) * 8]) = t.x[j];
+}
+
+template <int DP, bool LAG, bool SUMS, typename LDS>
+__device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const Sums* sm, LDS& lds) {
+  constexpr int NW = DP / 16, NT = DP / 16, KS = DP / 32;
+  constexpr int RP = LAG ? 3 : 2;  // parts of the state where it is read
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, q4 = (lane >> 4) * 4;
+  const int seg = blockIdx.x % g.nseg, bh = blockIdx.x / g.nseg, b = bh / g.H, h = bh - b * g.H;
+  const int n = valid_of(g, b);
+  const float l2 = -g.rate[h] * 1.44269504088896340736f;
+  const Mat& mk = SUMS ? sm->k : p->k;
+  const Mat& mv = SUMS ? sm->v : p->v;
+  const int Da = SUMS ? sm->Da : p->Da, Db = SUMS ? sm->Db : p->Db;
+  const int rev = SUMS ? sm->rev : p->rev;
+  const float vscale = SUMS ? sm->vscale : p->vscale;
+  const uint16_t* K = row_base<uint16_t>(mk, b, h);
+  const uint16_t* V = row_base<uint16_t>(mv, b, h);
+  const uint16_t* Q = SUMS ? nullptr : row_base<uint16_t>(p->q, b, h);
+  const uint16_t* X = LAG && !SUMS ? row_base<uint16_t>(p->x, b, h) : nullptr;
+  const int col = 16 * w + c;
+  const int NC = (g.T + kC - 1) / kC;
+  const int ch0 = seg * g.cps, ch1 = ch0 + g.cps < NC ? ch0 + g.cps : NC;
+  const size_t dd = (size_t)Da * Db;
+
+  v4f S[NT], L[LAG ? NT : 1];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    S[t] = v4f{0.f, 0.f, 0.f, 0.f};
+    if (LAG) L[t] = S[t];
+  }
+  if constexpr (!SUMS) {
+    const float* s0 = p->seg ? p->seg + ((size_t)bh * g.nseg + seg) * p->nst * dd : p->init ? p->init + (size_t)bh * dd : nullptr;
+    const int ia = p->seg ? p->sga : p->ia, ib = p->seg ? p->sgb : p->ib;
+    if (s0) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int a = 16 * t + q4 + v;
+          if (a < Da && col < Db) {
+            S[t][v] = s0[(size_t)a * ia + (size_t)col * ib];
+            if (LAG && p->seg) L[t][v] = s0[dd + (size_t)a * ia + (size_t)col * ib];
+          }
+        }
+    }
+    // the two 16x16 tiles of P above the diagonal that a 32-deep product reads stay zero
+    for (int i = threadIdx.x; i < 128; i += 4 * DP) {
+      const int it = i >> 6 << 1, r = i & 15, k = 8 * ((i >> 4) & 3);  // rows 16 it + r, second halves of the eights
+      const int at = 32 * (it >> 1) + k + 4;
+      *reinterpret_cast<uint64_t*>(&lds.P1[16 * it + r][at]) = 0;
+      *reinterpret_cast<uint64_t*>(&lds.P2[16 * it + r][at]) = 0;
+    }
+  }
+  double dr = 0.0;
+  Piece<DP> fk, fv, fq, fx;
+  auto fetch = [&](int ch) {
+    const int base = ch * kC, left = n - base, cnt = left < kC ? left : kC;
+    fetch16<DP>(fk, K, mk, Da, base, cnt, n, rev);
+    fetch16<DP>(fv, V, mv, Db, base, cnt, n, rev);
+    if constexpr (!SUMS) fetch16<DP>(fq, Q, p->q, Da, base, cnt, n, rev);
+    if constexpr (!SUMS && LAG) fetch16<DP>(fx, X, p->x, Db, base, cnt, n, rev);
+  };
+  if (ch0 * kC < n) fetch(ch0);
+  for (int ch = ch0; ch < ch1; ++ch) {
+    const int base = ch * kC;
+    const int cnt = n - base < 0 ? 0 : n - base < kC ? n - base : kC;
+    if (SUMS && cnt == 0) break;
+    const int off = rev && ch == 0 ? 1 : 0;  // (the gradient of the final state enters without a step of decay)
+    v4f O[4];
+    float drc = 0.f;
+    b8 vf[2];
+    if (cnt > 0) {
+      put16<DP>(lds.K, fk);
+      put16<DP>(lds.V, fv);
+      if constexpr (!SUMS) put16<DP>(lds.Q, fq);
+      if constexpr (!SUMS && LAG) put16<DP>(lds.X, fx);
+      __syncthreads();
+      if (ch + 1 < ch1 && base + kC < n) fetch(ch + 1);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) vf[s] = lds_col(lds.V.r, 32 * s, 16 * w, lane);
+      if constexpr (!SUMS) {
+        for (int t = w; t < 10; t += NW) {
+          const int it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2;
+          v4f acc = v4f{0.f, 0.f, 0.f, 0.f}, ax = acc;
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            acc = mma32(lds16(&lds.K.r[16 * jt + c][32 * s + 2 * q4]), lds16(&lds.Q.r[16 * it + c][32 * s + 2 * q4]), acc);
+            if constexpr (LAG) ax = mma32(lds16(&lds.V.r[16 * jt + c][32 * s + 2 * q4]), lds16(&lds.X.r[16 * it + c][32 * s + 2 * q4]), ax);
+          }
+          union { __bf16 e[4]; uint64_t u; } p1, p2;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int lag = 16 * (it - jt) + c - q4 - v;
+            const float x = lag >= 0 ? acc[v] * decay(l2, lag) * vscale : 0.f;
+            if (LAG && lag > 0) drc = fmaf((float)lag * x, ax[v], drc);
+            p1.e[v] = (__bf16)x;
+            p2.e[v] = (__bf16)(x - (float)p1.e[v]);
+          }
+          const int at = 32 * (jt >> 1) + 2 * q4 + 4 * (jt & 1);  // the order in which a 32-deep operand of P is read
+          *reinterpret_cast<uint64_t*>(&lds.P1[16 * it + c][at]) = p1.u;
+          *reinterpret_cast<uint64_t*>(&lds.P2[16 * it + c][at]) = p2.u;
+        }
+        v4f E[LAG ? 4 : 1];
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          O[it] = v4f{0.f, 0.f, 0.f, 0.f};
+          if (LAG) E[it] = O[it];
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          b8 sp[RP], lp[RP];
+          split<RP>(S[2 * s], S[2 * s + 1], sp);
+          if (LAG) split<RP>(L[2 * s], L[2 * s + 1], lp);
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            const b8 bq = lds8x2(&lds.Q.r[16 * it + c][32 * s + q4]);
+#pragma unroll
+            for (int i = 0; i < RP; ++i) {
+              O[it] = mma32(sp[i], bq, O[it]);
+              if (LAG) E[it] = mma32(lp[i], bq, E[it]);
+            }
+          }
+        }
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const int ex = 16 * it + c + 1 - off;
+          const float f = decay(l2, ex);
+          O[it] = f * O[it];
+          if constexpr (LAG) {  // what the lag-weighted state adds to d rate
+            E[it] = f * E[it] + (float)ex * O[it];
+            const uint16_t* x = &lds.X.r[16 * it + c][16 * w + q4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) drc = fmaf(E[it][v], __uint_as_float((uint32_t)x[v] << 16), drc);
+          }
+        }
+        if (LAG) dr -= (double)drc * (double)p->oscale;
+        __syncthreads();
+#pragma unroll
+        for (int it = 0; it < 4; ++it)
+#pragma unroll
+          for (int s = 0; s <= it / 2; ++s) {
+            O[it] = mma32(vf[s], lds16(&lds.P1[16 * it + c][32 * s + 2 * q4]), O[it]);
+            O[it] = mma32(vf[s], lds16(&lds.P2[16 * it + c][32 * s + 2 * q4]), O[it]);
+          }
+      }
+    }
+    if constexpr (!SUMS) {
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const int i = base + 16 * it + c;
+        if (i >= g.T) continue;
+        const bool live = i < n;
+        const int64_t t = rev && live ? n - 1 - i : i;
+        const int b0 = 16 * w + q4;
+        float o[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) o[v] = live ? O[it][v] * p->oscale : 0.f;
+        const int64_t at = (int64_t)b * p->out.sb + (int64_t)h * p->out.sh + t * p->out.st;
+        if (p->out32) {
+          float* row = (float*)p->out.p + at;
+          if (p->out.vec) {
+            if (b0 < Db) *reinterpret_cast<float4*>(row + b0) = make_float4(o[0], o[1], o[2], o[3]);
+          } else {
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (b0 + v < Db) row[b0 + v] = o[v];
+          }
+        } else {
+          ic_bf16* row = (ic_bf16*)p->out.p + at;
+          if (p->out.vec) {
+            union { ic_bf16 e[4]; uint64_t u; } x;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) x.e[v] = ic_from_f<ic_bf16>(o[v]);
+            if (b0 < Db) *reinterpret_cast<uint64_t*>(row + b0) = x.u;
+          } else {
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (b0 + v < Db) row[b0 + v] = ic_from_f<ic_bf16>(o[v]);
+          }
+        }
+      }
+    }
+    if (cnt > 0) {  // the state behind the chunk
+      const float carry = decay(l2, cnt - off);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (LAG) L[t] = carry * (L[t] + (float)cnt * S[t]);
+        S[t] = carry * S[t];
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        b8 vp[3], lp[LAG ? 3 : 1];
+        {
+          float x[8], y[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int left = cnt - 1 - (32 * s + 16 * (u >> 2) + q4 + (u & 3));
+            x[u] = left >= 0 ? (float)vf[s][u] * (decay(l2, left) * vscale) : 0.f;
+            y[u] = x[u] * (float)left;
+          }
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            vp[i] = take_part(x);
+            if constexpr (LAG) lp[i] = take_part(y);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const b8 ak = lds_col(lds.K.r, 32 * s, 16 * t, lane);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            S[t] = mma32(ak, vp[i], S[t]);
+            if constexpr (LAG) L[t] = mma32(ak, lp[i], L[t]);
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+  finish<LAG, SUMS, NT>(g, p, sm, lds, S, L, dr, dd, Da, Db, col, q4, bh, seg, n, l2);
+}
 
 template <typename T, int DP, bool LAG>
 __global__ __launch_bounds__(DP * 4) void k_lattn(PassArgs a) {
-  __shared__ __align__(16) Lds<DP> lds;
-  if (LAG && blockIdx.y == 0) lattn_body<T, DP, LAG, false>(a.g, &a.p[0], nullptr, lds);
-  else lattn_body<T, DP, false, false>(a.g, &a.p[blockIdx.y], nullptr, lds);
+  if constexpr (std::is_same<T, ic_bf16>::value) {
+    __shared__ __align__(16) Lds16<DP, LAG> lds;
+    lattn_body16<DP, LAG, false>(a.g, &a.p[blockIdx.y], nullptr, lds);
+  } else {
+    __shared__ __align__(16) Lds<DP> lds;
+    lattn_body<T, DP, LAG, false>(a.g, &a.p[blockIdx.y], nullptr, lds);
+  }
 }
 template <typename T, int DP, bool LAG>
 __global__ __launch_bounds__(DP * 4) void k_lattn_sums(SumArgs a) {
-  __shared__ __align__(16) LdsSums<DP> lds;
-  if (LAG && blockIdx.y == 0) lattn_body<T, DP, LAG, true>(a.g, nullptr, &a.s[0], lds);
-  else lattn_body<T, DP, false, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
+  if constexpr (std::is_same<T, ic_bf16>::value) {
+    __shared__ __align__(16) LdsSums16<DP> lds;
+    lattn_body16<DP, LAG, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
+  } else {
+    __shared__ __align__(16) LdsSums<DP> lds;
+    lattn_body<T, DP, LAG, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
+  }
 }
 
 // segment sums -> start states: seg[s] <- state in front of segment s
@@ -632,8 +967,14 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
     s.s[0] = Sums{v, k, Dv, Dk, 0, lag, 1.f, seg_s};
     s.s[1] = Sums{q, o, Dk, Dv, 1, 0, a->scale, seg_r};
 #define IC_BODY(T, DP)                                                                                                                        \
-  if (lag) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, true>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, s)); \
-  else IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, s))
+  if (lag) {                                                                                                                                   \
+    IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, true>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, s));         \
+    SumArgs s1 = s;                                                                                                                            \
+    s1.s[0] = s.s[1];                                                                                                                          \
+    IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, s1));       \
+  } else {                                                                                                                                     \
+    IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, s));        \
+  }
     IC_LATTN_T(a->dtype, IC_BODY_T);
 #undef IC_BODY
     IC_LAUNCH_CHECK("ic_lattn_bwd");
@@ -670,8 +1011,8 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
   pk.oscale = 1.f; pk.vscale = a->scale;
   pk.init = ba->dstate_out; pk.ia = 1; pk.ib = Dv;
   if (G > 1) {
-    pk.out = Mat{part_k, (int64_t)a->H * a->T * Dk, (int64_t)a->T * Dk, Dk, 1, 0};
-    pv.out = Mat{part_v, (int64_t)a->H * a->T * Dv, (int64_t)a->T * Dv, Dv, 1, 0};
+    pk.out = mat(part_k, (int64_t)a->H * a->T * Dk, (int64_t)a->T * Dk, Dk, 1, Dk, 4);
+    pv.out = mat(part_v, (int64_t)a->H * a->T * Dv, (int64_t)a->T * Dv, Dv, 1, Dv, 4);
     pk.out32 = pv.out32 = 1;
   }
   if (g.nseg > 1) {
@@ -680,8 +1021,15 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
     pk.seg = seg_r; pk.sga = 1; pk.sgb = Dv; pk.nst = 1;
   }
 #define IC_BODY(T, DP)                                                                                                              \
-  if (lag) IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, true>), dim3(bh * g.nseg, 3), dim3(DP * 4), 0, st, p)); \
-  else IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false>), dim3(bh * g.nseg, 3), dim3(DP * 4), 0, st, p))
+  if (lag) {                                                                                                                       \
+    IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, true>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, p));   \
+    PassArgs p1 = p;                                                                                                               \
+    p1.p[0] = p.p[1];                                                                                                              \
+    p1.p[1] = p.p[2];                                                                                                              \
+    IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, p1)); \
+  } else {                                                                                                                         \
+    IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false>), dim3(bh * g.nseg, 3), dim3(DP * 4), 0, st, p));  \
+  }
   IC_LATTN_T(a->dtype, IC_BODY_T);
 #undef IC_BODY
   IC_LAUNCH_CHECK("ic_lattn_bwd");
