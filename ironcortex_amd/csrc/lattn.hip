@@ -21,14 +21,13 @@
 // l holds rows 4 (l / 16) + 0..3 of column l % 16, and as an operand k-indices 4 (l / 16) + 0..3 of row / column l % 16).
 // Several segments per sequence only where sequences and heads do not fill the chip: their sums are formed first
 // (k_lattn SUMS), scanned (k_lattn_scan), and each segment starts from its own prefix.
-#include <type_traits>
-
 #include "ic_types.h"
 
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 constexpr int kC = 64;
+constexpr int64_t kMaxStride = 1 << 22;  // elements from position to position
 
 struct Mat {  // rows [B,heads,T,D] of one of q, k, v, dout, ...
   void* p;
@@ -134,49 +133,51 @@ struct LdsSums {
   float Ks[kC][DP + 4];
 };
 
-// the end of a segment: its sums, or (last segment) the end state; d rate's partial sum
-template <bool LAG, bool SUMS, int NT, typename LDS, int NL>
-__device__ __forceinline__ void finish(const Geo& g, const Pass* p, const Sums* sm, LDS& lds, const v4f (&S)[NT], const v4f (&L)[NL],
-                                       double dr, size_t dd, int Da, int Db, int col, int q4, int bh, int seg, int n, float l2) {
-  if constexpr (SUMS) {
-    float* dst = sm->seg + ((size_t)bh * g.nseg + seg) * (LAG ? 2 : 1) * dd;
+// the end of a segment: its sums, or (last segment) the end state and its share of d rate; d rate's partial sum.
+// S[t][v]: element (16 t + q4 + v, col)
+template <bool LAG, int NT, int NL>
+__device__ __forceinline__ void write_sums(const Geo& g, const Sums* sm, const v4f (&S)[NT], const v4f (&L)[NL], size_t dd, int Da, int Db, int col, int q4, int bh, int seg) {
+  float* dst = sm->seg + ((size_t)bh * g.nseg + seg) * (LAG ? 2 : 1) * dd;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int a = 16 * t + q4 + v;
-        if (a < Da && col < Db) {
-          dst[(size_t)a * Db + col] = S[t][v];
-          if constexpr (LAG) dst[dd + (size_t)a * Db + col] = L[t][v];
-        }
-      }
-  } else {
-    if (seg == g.nseg - 1) {
-      const float last = p->fin_decay && n > 0 ? decay(l2, 1) : 1.f;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int a = 16 * t + q4 + v;
-          if (a < Da && col < Db) {
-            const size_t at = (size_t)bh * dd + (size_t)a * p->ia + (size_t)col * p->ib;
-            if (p->fin) p->fin[at] = S[t][v] * last;
-            if constexpr (LAG) {
-              if (p->gfin) dr -= (double)L[t][v] * (double)p->gfin[at];
-            }
-          }
-        }
-    }
-    if constexpr (LAG) {
-      for (int o = 32; o; o >>= 1) dr += __shfl_xor(dr, o, 64);
-      if ((threadIdx.x & 63) == 0) lds.red[threadIdx.x >> 6] = dr;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        double t = 0.0;
-        for (int i = 0; i < NT; ++i) t += lds.red[i];  // (as many waves as 16-row tiles)
-        p->dr[(size_t)bh * g.nseg + seg] = t;
+    for (int v = 0; v < 4; ++v) {
+      const int a = 16 * t + q4 + v;
+      if (a < Da && col < Db) {
+        dst[(size_t)a * Db + col] = S[t][v];
+        if constexpr (LAG) dst[dd + (size_t)a * Db + col] = L[t][v];
       }
     }
+}
+template <bool LAG, int NT, int NL>
+__device__ __forceinline__ double write_end(const Geo& g, const Pass* p, const v4f (&S)[NT], const v4f (&L)[NL], size_t dd, int Da, int Db, int col, int q4, int bh, int seg, int n, float l2) {
+  double dr = 0.0;
+  if (seg != g.nseg - 1) return dr;
+  const float last = p->fin_decay && n > 0 ? decay(l2, 1) : 1.f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int a = 16 * t + q4 + v;
+      if (a < Da && col < Db) {
+        const size_t at = (size_t)bh * dd + (size_t)a * p->ia + (size_t)col * p->ib;
+        if (p->fin) p->fin[at] = S[t][v] * last;
+        if constexpr (LAG) {
+          if (p->gfin) dr -= (double)L[t][v] * (double)p->gfin[at];
+        }
+      }
+    }
+  return dr;
+}
+template <int NW>
+__device__ __forceinline__ void write_drate(const Geo& g, const Pass* p, double* red, double dr, int bh, int seg) {
+  for (int o = 32; o; o >>= 1) dr += __shfl_xor(dr, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = dr;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int i = 0; i < NW; ++i) t += red[i];
+    p->dr[(size_t)bh * g.nseg + seg] = t;
   }
 }
 
@@ -362,10 +363,16 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
     }
     __syncthreads();
   }
-  finish<LAG, SUMS, KS>(g, p, sm, lds, S, L, dr, dd, Da, Db, col, q4, bh, seg, n, l2);
+  if constexpr (SUMS) {
+    write_sums<LAG>(g, sm, S, L, dd, Da, Db, col, q4, bh, seg);
+  } else {
+    dr += write_end<LAG>(g, p, S, L, dd, Da, Db, col, q4, bh, seg, n, l2);
+    if constexpr (LAG) write_drate<NW>(g, p, lds.red, dr, bh, seg);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ bf16 rows
+// Rows that allow 16-byte accesses (others take the body above).
 // The same map on bf16 matrix instructions (16x16x32: sixteen times the fp32 rate).  Products of rows (q . k) are exact
 // there.  Operands that are computed in fp32 -- the decayed products P, the state, the decay-weighted values -- are split
 // into bf16 parts (x = x1 + x2 [+ x3], each the rounded rest of the one before: 8 bits of the value apiece): two parts where
@@ -375,22 +382,26 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
 // 4 q .. 4 q + 3 of either 16-row half, on both sides of a product; products of rows use contiguous eights instead.
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef short s4v __attribute__((ext_vector_type(4)));
-constexpr int kPad16 = 16, kPw = kC + 8;
+constexpr int kPw = kC + 8;
 
-template <int DP>
+// padding: 32 bytes a row spread the 8 rows of a transposing read over the 64 banks, 16 bytes the 16 rows of a 16-byte read
+template <int W>
 struct RowTile {
-  uint16_t r[kC][DP + kPad16];  // 32 bytes of padding: the transposing reads of 8 rows and the 16-byte reads of 8 rows spread over the banks
+  uint16_t r[kC][W];
 };
 template <int DP, bool LAG>
 struct Lds16 {
-  RowTile<DP> K, V, Q;
-  RowTile<LAG ? DP : 16> X;
+  RowTile<DP + 16> K, V;
+  RowTile<DP + 8> Q;
+  RowTile<LAG ? DP + 8 : 8> X;
   uint16_t P1[kC][kPw], P2[kC][kPw];
+  float dec[2 * kC + 1];  // dec[kC + lag] = e^{-r lag}, 0 for lag < 0
   double red[DP / 16];
 };
 template <int DP>
 struct LdsSums16 {
-  RowTile<DP> K, V;
+  RowTile<DP + 16> K, V;
+  float dec[2 * kC + 1];
 };
 
 __device__ __forceinline__ v4f mma32(b8 a, b8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -411,136 +422,178 @@ __device__ __forceinline__ b8 lds_col(const uint16_t (*t)[W], int r0, int c0, in
   x.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)(p + 16 * W));
   return x.b;
 }
-// bf16 parts of eight fp32 values; x keeps the rest
-__device__ __forceinline__ b8 take_part(float (&x)[8]) {
-  b8 p;
+// bf16 parts of fp32 values, two at a time: the next part of x, x keeps the rest
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack2(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2)); }
+__device__ __forceinline__ uint32_t take2(float& a, float& b) {
+  const uint32_t u = pack2(a, b);
+  a -= __uint_as_float(u << 16);
+  b -= __uint_as_float(u & 0xffff0000u);
+  return u;
+}
+template <int N>
+__device__ __forceinline__ void split(float (&x)[8], b8 (&out)[N]) {
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    p[u] = (__bf16)x[u];
-    x[u] -= (float)p[u];
+  for (int i = 0; i < N; ++i) {
+    union { uint32_t u[4]; b8 b; } y;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) y.u[u] = i + 1 < N ? take2(x[2 * u], x[2 * u + 1]) : pack2(x[2 * u], x[2 * u + 1]);
+    out[i] = y.b;
   }
-  return p;
 }
 template <int N>
 __device__ __forceinline__ void split(const v4f& a, const v4f& b, b8 (&out)[N]) {
   float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-#pragma unroll
-  for (int i = 0; i < N; ++i) out[i] = take_part(x);
+  split<N>(x, out);
 }
 
-// 16-byte pieces of a tile's rows in flight: fetch (global -> registers), put (registers -> LDS)
-template <int DP>
-struct Piece {
-  uint4 x[2];  // kC rows x DP / 8 pieces over 4 DP threads
-};
-template <int DP>
-__device__ __forceinline__ void fetch16(Piece<DP>& t, const uint16_t* src, const Mat& m, int D, int base, int cnt, int n, int rev) {
-  constexpr int PER = DP / 8, RT = 32;  // (4 DP threads: 32 rows at a time)
+// four consecutive columns of an output row
+__device__ __forceinline__ void store4(char* row, const v4f& o, bool f32) {
+  if (f32) *reinterpret_cast<v4f*>(row) = o;
+  else *reinterpret_cast<uint2*>(row) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
+}
+
+// Rows of one matrix as a workgroup of 4 DP threads reads them: 16-byte pieces, 32 rows at a time.  A chunk's address is
+// uniform, base positions times `step` behind `src`; a lane's place in the chunk is fixed (a 32-bit byte offset: 64 rows span
+// less than 2^31 bytes, checked on the host).  In a reversed pass step < 0 and src is 63 rows below the first position's, so
+// that the lanes' offsets count down and stay positive.
+__device__ __forceinline__ const char* chunk_src(const char* rows, int64_t st, int n, int rev) { return rows + (rev ? (int64_t)(n - kC) * st : 0); }
+template <int DP, int CW>
+struct Rows {
+  static constexpr int RT = 32 / CW, NP = 2 * CW;  // rows at a time, times
+  const char* src;
+  int64_t step;
+  uint32_t off;  // this lane's piece of row threadIdx / (DP / 8)
+  bool live;     // inside the row
+  __device__ __forceinline__ void open(const Mat& m, int b, int h, int D, int n, int rev) {
+    constexpr int PER = DP / 8;
+    const int64_t st = m.st * 2;
+    src = chunk_src((const char*)row_base<uint16_t>(m, b, h), st, n, rev);
+    step = rev ? -st : st;
+    const int r = threadIdx.x / PER, c = (threadIdx.x % PER) * 8;
+    live = c < D;
+    off = (uint32_t)((rev ? kC - 1 - r : r) * (int32_t)st + c * 2);
+  }
+  // rows [base, base + cnt) (virtual positions); others read as zero
+  __device__ __forceinline__ void fetch(uint4 (&x)[NP], int base, int cnt) const {
+    const int r = threadIdx.x / (DP / 8);
+    const char* at = src + base * step;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int r = threadIdx.x / PER + RT * j, c = (threadIdx.x % PER) * 8;
-    t.x[j] = make_uint4(0, 0, 0, 0);
-    if (r < cnt) {
-      const uint16_t* row = src + (int64_t)(rev ? n - 1 - (base + r) : base + r) * m.st;
-      if (m.vec) {
-        if (c < D) t.x[j] = *reinterpret_cast<const uint4*>(row + c);
-      } else {
-        uint32_t e[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (c + u < D) e[u >> 1] |= (uint32_t)row[c + u] << (16 * (u & 1));
-        t.x[j] = make_uint4(e[0], e[1], e[2], e[3]);
-      }
+    for (int j = 0; j < NP; ++j, at += RT * step) {
+      x[j] = make_uint4(0, 0, 0, 0);
+      if (live && r + RT * j < cnt) x[j] = *reinterpret_cast<const uint4*>(at + off);
     }
   }
-}
-template <int DP>
-__device__ __forceinline__ void put16(RowTile<DP>& dst, const Piece<DP>& t) {
-  constexpr int PER = DP / 8, RT = 32;
+  template <int W>
+  static __device__ __forceinline__ void put(RowTile<W>& dst, const uint4 (&x)[NP]) {
+    constexpr int PER = DP / 8;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) *reinterpret_cast<uint4*>(&dst.r[threadIdx.x / PER + RT * j][(threadIdx.x % PER) * 8]) = t.x[j];
-}
+    for (int j = 0; j < NP; ++j) *reinterpret_cast<uint4*>(&dst.r[threadIdx.x / PER + RT * j][(threadIdx.x % PER) * 8]) = x[j];
+  }
+};
 
-template <int DP, bool LAG, bool SUMS, typename LDS>
+// A wave owns CW tiles of 16 value columns; a workgroup has DP / (16 CW) waves.
+template <int DP, int CW, bool LAG, bool SUMS, typename LDS>
 __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const Sums* sm, LDS& lds) {
-  constexpr int NW = DP / 16, NT = DP / 16, KS = DP / 32;
+  constexpr int NW = DP / (16 * CW), NT = DP / 16, KS = DP / 32, MT = (10 + NW - 1) / NW;
   constexpr int RP = LAG ? 3 : 2;  // parts of the state where it is read
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, q4 = (lane >> 4) * 4;
+  using R = Rows<DP, CW>;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, q4 = (lane >> 4) * 4;
   const int seg = blockIdx.x % g.nseg, bh = blockIdx.x / g.nseg, b = bh / g.H, h = bh - b * g.H;
-  const int n = valid_of(g, b);
+  const int n = valid_of(g, b), T = g.T;
   const float l2 = -g.rate[h] * 1.44269504088896340736f;
-  const Mat& mk = SUMS ? sm->k : p->k;
-  const Mat& mv = SUMS ? sm->v : p->v;
   const int Da = SUMS ? sm->Da : p->Da, Db = SUMS ? sm->Db : p->Db;
   const int rev = SUMS ? sm->rev : p->rev;
-  const float vscale = SUMS ? sm->vscale : p->vscale;
-  const uint16_t* K = row_base<uint16_t>(mk, b, h);
-  const uint16_t* V = row_base<uint16_t>(mv, b, h);
-  const uint16_t* Q = SUMS ? nullptr : row_base<uint16_t>(p->q, b, h);
-  const uint16_t* X = LAG && !SUMS ? row_base<uint16_t>(p->x, b, h) : nullptr;
-  const int col = 16 * w + c;
-  const int NC = (g.T + kC - 1) / kC;
+  const float vscale = SUMS ? sm->vscale : p->vscale, oscale = SUMS ? 1.f : p->oscale;
+  R rk, rv, rq, rx;
+  rk.open(SUMS ? sm->k : p->k, b, h, Da, n, rev);
+  rv.open(SUMS ? sm->v : p->v, b, h, Db, n, rev);
+  if constexpr (!SUMS) rq.open(p->q, b, h, Da, n, rev);
+  if constexpr (!SUMS && LAG) rx.open(p->x, b, h, Db, n, rev);
+  for (int i = threadIdx.x; i < 2 * kC + 1; i += 64 * NW) lds.dec[i] = i < kC ? 0.f : decay(l2, i - kC);
+  const int col0 = 16 * CW * w;  // this wave's columns
+  const int NC = (T + kC - 1) / kC;
   const int ch0 = seg * g.cps, ch1 = ch0 + g.cps < NC ? ch0 + g.cps : NC;
   const size_t dd = (size_t)Da * Db;
 
-  v4f S[NT], L[LAG ? NT : 1];
+  v4f S[CW][NT], L[LAG ? CW : 1][LAG ? NT : 1];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    S[t] = v4f{0.f, 0.f, 0.f, 0.f};
-    if (LAG) L[t] = S[t];
-  }
+  for (int k = 0; k < CW; ++k)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      S[k][t] = v4f{0.f, 0.f, 0.f, 0.f};
+      if (LAG) L[k][t] = S[k][t];
+    }
+  char* out = nullptr;
+  int64_t ost = 0;
+  uint32_t ooff = 0;
+  bool o32 = false;
   if constexpr (!SUMS) {
+    o32 = p->out32;
+    const int esz = o32 ? 4 : 2;
+    ost = p->out.st * esz;
+    out = (char*)p->out.p + ((int64_t)b * p->out.sb + (int64_t)h * p->out.sh) * esz;
+    ooff = (uint32_t)((rev ? kC - 1 - c : c) * (int32_t)ost + (col0 + q4) * esz);
     const float* s0 = p->seg ? p->seg + ((size_t)bh * g.nseg + seg) * p->nst * dd : p->init ? p->init + (size_t)bh * dd : nullptr;
     const int ia = p->seg ? p->sga : p->ia, ib = p->seg ? p->sgb : p->ib;
     if (s0) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int k = 0; k < CW; ++k)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int a = 16 * t + q4 + v;
-          if (a < Da && col < Db) {
-            S[t][v] = s0[(size_t)a * ia + (size_t)col * ib];
-            if (LAG && p->seg) L[t][v] = s0[dd + (size_t)a * ia + (size_t)col * ib];
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int a = 16 * t + q4 + v, col = col0 + 16 * k + c;
+            if (a < Da && col < Db) {
+              S[k][t][v] = s0[(size_t)a * ia + (size_t)col * ib];
+              if constexpr (LAG) {
+                if (p->seg) L[k][t][v] = s0[dd + (size_t)a * ia + (size_t)col * ib];
+              }
+            }
           }
-        }
     }
     // the two 16x16 tiles of P above the diagonal that a 32-deep product reads stay zero
-    for (int i = threadIdx.x; i < 128; i += 4 * DP) {
-      const int it = i >> 6 << 1, r = i & 15, k = 8 * ((i >> 4) & 3);  // rows 16 it + r, second halves of the eights
-      const int at = 32 * (it >> 1) + k + 4;
+    for (int i = threadIdx.x; i < 128; i += 64 * NW) {
+      const int it = (i >> 6) << 1, r = i & 15, at = 32 * (it >> 1) + 8 * ((i >> 4) & 3) + 4;
       *reinterpret_cast<uint64_t*>(&lds.P1[16 * it + r][at]) = 0;
       *reinterpret_cast<uint64_t*>(&lds.P2[16 * it + r][at]) = 0;
     }
   }
   double dr = 0.0;
-  Piece<DP> fk, fv, fq, fx;
-  auto fetch = [&](int ch) {
-    const int base = ch * kC, left = n - base, cnt = left < kC ? left : kC;
-    fetch16<DP>(fk, K, mk, Da, base, cnt, n, rev);
-    fetch16<DP>(fv, V, mv, Db, base, cnt, n, rev);
-    if constexpr (!SUMS) fetch16<DP>(fq, Q, p->q, Da, base, cnt, n, rev);
-    if constexpr (!SUMS && LAG) fetch16<DP>(fx, X, p->x, Db, base, cnt, n, rev);
+  uint4 fk[R::NP], fv[R::NP], fq[SUMS ? 1 : R::NP], fx[!SUMS && LAG ? R::NP : 1];
+  auto fetch = [&](int base) {
+    const int cnt = n - base < kC ? n - base : kC;
+    rk.fetch(fk, base, cnt);
+    rv.fetch(fv, base, cnt);
+    if constexpr (!SUMS) rq.fetch(fq, base, cnt);
+    if constexpr (!SUMS && LAG) rx.fetch(fx, base, cnt);
   };
-  if (ch0 * kC < n) fetch(ch0);
+  if (ch0 * kC < n) fetch(ch0 * kC);
   for (int ch = ch0; ch < ch1; ++ch) {
     const int base = ch * kC;
     const int cnt = n - base < 0 ? 0 : n - base < kC ? n - base : kC;
     if (SUMS && cnt == 0) break;
     const int off = rev && ch == 0 ? 1 : 0;  // (the gradient of the final state enters without a step of decay)
-    v4f O[4];
-    float drc = 0.f;
-    b8 vf[2];
+    v4f O[CW][4];
+    b8 vf[CW][2];
     if (cnt > 0) {
-      put16<DP>(lds.K, fk);
-      put16<DP>(lds.V, fv);
-      if constexpr (!SUMS) put16<DP>(lds.Q, fq);
-      if constexpr (!SUMS && LAG) put16<DP>(lds.X, fx);
+      R::put(lds.K, fk);
+      R::put(lds.V, fv);
+      if constexpr (!SUMS) R::put(lds.Q, fq);
+      if constexpr (!SUMS && LAG) R::put(lds.X, fx);
       __syncthreads();
-      if (ch + 1 < ch1 && base + kC < n) fetch(ch + 1);
+      if (ch + 1 < ch1 && base + kC < n) fetch(base + kC);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) vf[s] = lds_col(lds.V.r, 32 * s, 16 * w, lane);
+      for (int k = 0; k < CW; ++k)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) vf[k][s] = lds_col(lds.V.r, 32 * s, col0 + 16 * k, lane);
       if constexpr (!SUMS) {
-        for (int t = w; t < 10; t += NW) {
+        float drc = 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int t = w + i * NW;
+          if (t >= 10) break;
           const int it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2;
           v4f acc = v4f{0.f, 0.f, 0.f, 0.f}, ax = acc;
 #pragma unroll
@@ -548,154 +601,174 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
             acc = mma32(lds16(&lds.K.r[16 * jt + c][32 * s + 2 * q4]), lds16(&lds.Q.r[16 * it + c][32 * s + 2 * q4]), acc);
             if constexpr (LAG) ax = mma32(lds16(&lds.V.r[16 * jt + c][32 * s + 2 * q4]), lds16(&lds.X.r[16 * it + c][32 * s + 2 * q4]), ax);
           }
-          union { __bf16 e[4]; uint64_t u; } p1, p2;
+          float x[4];
+          const int lag0 = 16 * (it - jt) + c - q4;
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            const int lag = 16 * (it - jt) + c - q4 - v;
-            const float x = lag >= 0 ? acc[v] * decay(l2, lag) * vscale : 0.f;
-            if (LAG && lag > 0) drc = fmaf((float)lag * x, ax[v], drc);
-            p1.e[v] = (__bf16)x;
-            p2.e[v] = (__bf16)(x - (float)p1.e[v]);
+            const float d = lds.dec[kC + lag0 - v] * (vscale * oscale);
+            x[v] = lag0 >= v ? acc[v] * d : 0.f;  // (a select: what lies above the diagonal may be infinite)
+            if constexpr (LAG) drc = lag0 > v ? fmaf((float)(lag0 - v) * x[v], ax[v], drc) : drc;
           }
+          uint2 p1, p2;
+          p1.x = take2(x[0], x[1]);
+          p1.y = take2(x[2], x[3]);
+          p2 = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
           const int at = 32 * (jt >> 1) + 2 * q4 + 4 * (jt & 1);  // the order in which a 32-deep operand of P is read
-          *reinterpret_cast<uint64_t*>(&lds.P1[16 * it + c][at]) = p1.u;
-          *reinterpret_cast<uint64_t*>(&lds.P2[16 * it + c][at]) = p2.u;
+          *reinterpret_cast<uint2*>(&lds.P1[16 * it + c][at]) = p1;
+          *reinterpret_cast<uint2*>(&lds.P2[16 * it + c][at]) = p2;
         }
-        v4f E[LAG ? 4 : 1];
+        v4f E[LAG ? CW : 1][4];
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
-          O[it] = v4f{0.f, 0.f, 0.f, 0.f};
-          if (LAG) E[it] = O[it];
-        }
+        for (int k = 0; k < CW; ++k)
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            O[k][it] = v4f{0.f, 0.f, 0.f, 0.f};
+            if constexpr (LAG) E[k][it] = O[k][it];
+          }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          b8 sp[RP], lp[RP];
-          split<RP>(S[2 * s], S[2 * s + 1], sp);
-          if (LAG) split<RP>(L[2 * s], L[2 * s + 1], lp);
+          b8 sp[CW][RP], lp[LAG ? CW : 1][RP];
+#pragma unroll
+          for (int k = 0; k < CW; ++k) {
+            split<RP>(S[k][2 * s], S[k][2 * s + 1], sp[k]);
+            if constexpr (LAG) split<RP>(L[k][2 * s], L[k][2 * s + 1], lp[k]);
+          }
 #pragma unroll
           for (int it = 0; it < 4; ++it) {
             const b8 bq = lds8x2(&lds.Q.r[16 * it + c][32 * s + q4]);
 #pragma unroll
-            for (int i = 0; i < RP; ++i) {
-              O[it] = mma32(sp[i], bq, O[it]);
-              if (LAG) E[it] = mma32(lp[i], bq, E[it]);
-            }
+            for (int i = 0; i < RP; ++i)
+#pragma unroll
+              for (int k = 0; k < CW; ++k) {
+                O[k][it] = mma32(sp[k][i], bq, O[k][it]);
+                if constexpr (LAG) E[k][it] = mma32(lp[k][i], bq, E[k][it]);
+              }
           }
         }
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
-          const int ex = 16 * it + c + 1 - off;
-          const float f = decay(l2, ex);
-          O[it] = f * O[it];
-          if constexpr (LAG) {  // what the lag-weighted state adds to d rate
-            E[it] = f * E[it] + (float)ex * O[it];
-            const uint16_t* x = &lds.X.r[16 * it + c][16 * w + q4];
+          const float f = lds.dec[kC + 16 * it + c + 1 - off] * oscale;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) drc = fmaf(E[it][v], __uint_as_float((uint32_t)x[v] << 16), drc);
+          for (int k = 0; k < CW; ++k) {
+            O[k][it] = f * O[k][it];
+            if constexpr (LAG) {  // what the lag-weighted state adds to d rate
+              E[k][it] = f * E[k][it] + (float)(16 * it + c + 1) * O[k][it];
+              const uint16_t* x = &lds.X.r[16 * it + c][col0 + 16 * k + q4];
+#pragma unroll
+              for (int v = 0; v < 4; ++v) drc = fmaf(E[k][it][v], __uint_as_float((uint32_t)x[v] << 16), drc);
+            }
           }
         }
-        if (LAG) dr -= (double)drc * (double)p->oscale;
+        if (LAG) dr -= (double)drc;
         __syncthreads();
 #pragma unroll
         for (int it = 0; it < 4; ++it)
 #pragma unroll
           for (int s = 0; s <= it / 2; ++s) {
-            O[it] = mma32(vf[s], lds16(&lds.P1[16 * it + c][32 * s + 2 * q4]), O[it]);
-            O[it] = mma32(vf[s], lds16(&lds.P2[16 * it + c][32 * s + 2 * q4]), O[it]);
+            const b8 x1 = lds16(&lds.P1[16 * it + c][32 * s + 2 * q4]), x2 = lds16(&lds.P2[16 * it + c][32 * s + 2 * q4]);
+#pragma unroll
+            for (int k = 0; k < CW; ++k) {
+              O[k][it] = mma32(vf[k][s], x1, O[k][it]);
+              O[k][it] = mma32(vf[k][s], x2, O[k][it]);
+            }
           }
       }
     }
     if constexpr (!SUMS) {
+      const int esz = o32 ? 4 : 2;
+      if (cnt == kC) {  // a whole chunk
+        const int64_t step = rev ? -ost : ost;
+        char* at = const_cast<char*>(chunk_src(out, ost, n, rev)) + base * step;
 #pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const int i = base + 16 * it + c;
-        if (i >= g.T) continue;
-        const bool live = i < n;
-        const int64_t t = rev && live ? n - 1 - i : i;
-        const int b0 = 16 * w + q4;
-        float o[4];
+        for (int it = 0; it < 4; ++it, at += 16 * step)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) o[v] = live ? O[it][v] * p->oscale : 0.f;
-        const int64_t at = (int64_t)b * p->out.sb + (int64_t)h * p->out.sh + t * p->out.st;
-        if (p->out32) {
-          float* row = (float*)p->out.p + at;
-          if (p->out.vec) {
-            if (b0 < Db) *reinterpret_cast<float4*>(row + b0) = make_float4(o[0], o[1], o[2], o[3]);
-          } else {
+          for (int k = 0; k < CW; ++k)
+            if (col0 + 16 * k + q4 < Db) store4(at + ooff + 16 * k * esz, O[k][it], o32);
+      } else {
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (b0 + v < Db) row[b0 + v] = o[v];
-          }
-        } else {
-          ic_bf16* row = (ic_bf16*)p->out.p + at;
-          if (p->out.vec) {
-            union { ic_bf16 e[4]; uint64_t u; } x;
+        for (int it = 0; it < 4; ++it) {
+          const int i = base + 16 * it + c;
+          const bool live = i < n;
+          char* at = out + (rev && live ? n - 1 - i : i) * ost + (col0 + q4) * esz;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) x.e[v] = ic_from_f<ic_bf16>(o[v]);
-            if (b0 < Db) *reinterpret_cast<uint64_t*>(row + b0) = x.u;
-          } else {
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (b0 + v < Db) row[b0 + v] = ic_from_f<ic_bf16>(o[v]);
+          for (int k = 0; k < CW; ++k) {
+            if (!live) O[k][it] = v4f{0.f, 0.f, 0.f, 0.f};
+            if (i < T && col0 + 16 * k + q4 < Db) store4(at + 16 * k * esz, O[k][it], o32);
           }
         }
       }
     }
     if (cnt > 0) {  // the state behind the chunk
-      const float carry = decay(l2, cnt - off);
+      const float carry = lds.dec[kC + cnt - off];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if (LAG) L[t] = carry * (L[t] + (float)cnt * S[t]);
-        S[t] = carry * S[t];
-      }
+      for (int k = 0; k < CW; ++k)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (LAG) L[k][t] = carry * (L[k][t] + (float)cnt * S[k][t]);
+          S[k][t] = carry * S[k][t];
+        }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        b8 vp[3], lp[LAG ? 3 : 1];
-        {
+        b8 vp[CW][3], lp[LAG ? CW : 1][3];
+        const float* dl = &lds.dec[kC + cnt - 1 - q4 - 51];  // (51: the largest position of this lane's values)
+#pragma unroll
+        for (int k = 0; k < CW; ++k) {
           float x[8], y[8];
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            const int left = cnt - 1 - (32 * s + 16 * (u >> 2) + q4 + (u & 3));
-            x[u] = left >= 0 ? (float)vf[s][u] * (decay(l2, left) * vscale) : 0.f;
-            y[u] = x[u] * (float)left;
+            const int j = 32 * s + 16 * (u >> 2) + (u & 3);
+            x[u] = (float)vf[k][s][u] * (dl[51 - j] * vscale);
+            if constexpr (LAG) y[u] = x[u] * (float)(cnt - 1 - q4 - j);  // (0 behind the last valid position)
           }
-#pragma unroll
-          for (int i = 0; i < 3; ++i) {
-            vp[i] = take_part(x);
-            if constexpr (LAG) lp[i] = take_part(y);
-          }
+          split<3>(x, vp[k]);
+          if constexpr (LAG) split<3>(y, lp[k]);
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const b8 ak = lds_col(lds.K.r, 32 * s, 16 * t, lane);
 #pragma unroll
-          for (int i = 0; i < 3; ++i) {
-            S[t] = mma32(ak, vp[i], S[t]);
-            if constexpr (LAG) L[t] = mma32(ak, lp[i], L[t]);
-          }
+          for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int k = 0; k < CW; ++k) {
+              S[k][t] = mma32(ak, vp[k][i], S[k][t]);
+              if constexpr (LAG) L[k][t] = mma32(ak, lp[k][i], L[k][t]);
+            }
         }
       }
       __syncthreads();
     }
   }
-  finish<LAG, SUMS, NT>(g, p, sm, lds, S, L, dr, dd, Da, Db, col, q4, bh, seg, n, l2);
+  if constexpr (SUMS) {
+#pragma unroll
+    for (int k = 0; k < CW; ++k) write_sums<LAG>(g, sm, S[k], L[LAG ? k : 0], dd, Da, Db, col0 + 16 * k + c, q4, bh, seg);
+  } else {
+#pragma unroll
+    for (int k = 0; k < CW; ++k) dr += write_end<LAG>(g, p, S[k], L[LAG ? k : 0], dd, Da, Db, col0 + 16 * k + c, q4, bh, seg, n, l2);
+    if constexpr (LAG) write_drate<NW>(g, p, lds.red, dr, bh, seg);
+  }
 }
 
-template <typename T, int DP, bool LAG>
-__global__ __launch_bounds__(DP * 4) void k_lattn(PassArgs a) {
-  if constexpr (std::is_same<T, ic_bf16>::value) {
+// bf16 rows, 128 channels: two column tiles a wave, so that 4 waves own the columns and two workgroups fit a compute unit
+// (74 KB of LDS, <= 256 registers): the one's barriers under the other's products.  One tile a wave where the lag-weighted
+// state doubles the registers.
+template <int DP, bool LAG, bool W16>
+constexpr int cw_of() { return W16 && DP == 128 && !LAG ? 2 : 1; }
+
+template <typename T, int DP, bool LAG, bool W16>
+__global__ __launch_bounds__((DP * 4 / cw_of<DP, LAG, W16>()), 2) void k_lattn(PassArgs a) {
+  if constexpr (W16) {
     __shared__ __align__(16) Lds16<DP, LAG> lds;
-    lattn_body16<DP, LAG, false>(a.g, &a.p[blockIdx.y], nullptr, lds);
+    lattn_body16<DP, cw_of<DP, LAG, W16>(), LAG, false>(a.g, &a.p[blockIdx.y], nullptr, lds);
   } else {
     __shared__ __align__(16) Lds<DP> lds;
     lattn_body<T, DP, LAG, false>(a.g, &a.p[blockIdx.y], nullptr, lds);
   }
 }
-template <typename T, int DP, bool LAG>
+template <typename T, int DP, bool LAG, bool W16>
 __global__ __launch_bounds__(DP * 4) void k_lattn_sums(SumArgs a) {
-  if constexpr (std::is_same<T, ic_bf16>::value) {
+  if constexpr (W16) {
     __shared__ __align__(16) LdsSums16<DP> lds;
-    lattn_body16<DP, LAG, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
+    lattn_body16<DP, 1, LAG, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
   } else {
     __shared__ __align__(16) LdsSums<DP> lds;
     lattn_body<T, DP, LAG, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
@@ -833,6 +906,12 @@ int check_lattn(const ic_lattn_args* a, const char* who) {
   return IC_OK;
 }
 
+// 64 rows of a matrix lie within 2^31 bytes (the kernels' offsets inside a chunk)
+int check_stride(int64_t st, const char* who, const char* n) {
+  IC_REQUIRE(st > -kMaxStride && st < kMaxStride, "%s: %s has %lld elements from position to position (below %lld)", who, n, (long long)st, (long long)kMaxStride);
+  return IC_OK;
+}
+
 int pad_of(const ic_lattn_args* a) {
   const int d = a->Dk > a->Dv ? a->Dk : a->Dv;
   return d <= 32 ? 32 : d <= 64 ? 64 : 128;
@@ -878,11 +957,12 @@ int64_t ws_floats(const ic_lattn_args* a, int backward) {
 
 }  // namespace
 
-#define IC_LATTN_T(dt, BODY)                     \
-  do {                                           \
-    if ((dt) == IC_DT_F32) { BODY(float) }       \
-    else if ((dt) == IC_DT_BF16) { BODY(ic_bf16) } \
-    else { BODY(ic_f16) }                        \
+#define IC_LATTN_T(dt, wide, BODY)                                                   \
+  do {                                                                               \
+    if ((dt) == IC_DT_F32) { [[maybe_unused]] constexpr bool W16 = false; BODY(float) }               \
+    else if ((dt) == IC_DT_BF16 && (wide)) { [[maybe_unused]] constexpr bool W16 = true; BODY(ic_bf16) } \
+    else if ((dt) == IC_DT_BF16) { [[maybe_unused]] constexpr bool W16 = false; BODY(ic_bf16) }       \
+    else { [[maybe_unused]] constexpr bool W16 = false; BODY(ic_f16) }                                \
   } while (0)
 #define IC_LATTN_DP(dp, T, BODY)                                \
   if ((dp) == 32) { constexpr int DP = 32; BODY(T, DP); }       \
@@ -903,18 +983,21 @@ extern "C" int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream) {
   IC_REQUIRE(a->q && a->k && a->v && a->rate && a->out, "ic_lattn_fwd: NULL tensor pointer");
   IC_REQUIRE(!a->state_out || a->state_out != a->state, "ic_lattn_fwd: state_out is state");
   IC_REQUIRE(a->ws || ws_floats(a, 0) == 0, "ic_lattn_fwd: NULL workspace");
+  if ((rc = check_stride(a->q_st, "ic_lattn_fwd", "q")) || (rc = check_stride(a->k_st, "ic_lattn_fwd", "k")) ||
+      (rc = check_stride(a->v_st, "ic_lattn_fwd", "v")) || (rc = check_stride(a->o_st, "ic_lattn_fwd", "out"))) return rc;
   const Geo g = geo_of(a, 1);
   const int esz = ic_dt_size(a->dtype), G = a->H / a->Hk, dp = pad_of(a), bh = a->B * a->H;
   hipStream_t st = (hipStream_t)stream;
   const Mat q = mat(a->q, a->q_sb, a->q_sh, a->q_st, 1, a->Dk, esz), k = mat(a->k, a->k_sb, a->k_sh, a->k_st, G, a->Dk, esz);
   const Mat v = mat(a->v, a->v_sb, a->v_sh, a->v_st, G, a->Dv, esz), o = mat(a->out, a->o_sb, a->o_sh, a->o_st, 1, a->Dv, esz);
+  const bool wide = a->dtype == IC_DT_BF16 && q.vec && k.vec && v.vec && o.vec;
   if (g.nseg > 1) {
     SumArgs s{};
     s.g = g;
     s.s[0] = Sums{k, v, a->Dk, a->Dv, 0, 0, 1.f, a->ws};
-#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, s))
+#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, s))
 #define IC_BODY_T(T) IC_LATTN_DP(dp, T, IC_BODY)
-    IC_LATTN_T(a->dtype, IC_BODY_T);
+    IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
     IC_LAUNCH_CHECK("ic_lattn_fwd");
     ScanArgs sc{};
@@ -932,8 +1015,8 @@ extern "C" int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream) {
   f.init = a->state; f.ia = a->Dv; f.ib = 1;
   f.fin = a->state_out;
   if (g.nseg > 1) { f.seg = a->ws; f.sga = a->Dv; f.sgb = 1; f.nst = 1; }
-#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_fwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, p))
-  IC_LATTN_T(a->dtype, IC_BODY_T);
+#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_fwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false, W16>), dim3(bh * g.nseg, 1), dim3(DP * 4 / cw_of<DP, false, W16>()), 0, st, p))
+  IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
   IC_LAUNCH_CHECK("ic_lattn_fwd");
   return IC_OK;
@@ -947,6 +1030,10 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
   IC_REQUIRE(a->q && a->k && a->v && a->rate && ba->dout && ba->dq && ba->dk && ba->dv, "ic_lattn_bwd: NULL tensor pointer");
   IC_REQUIRE(!ba->dstate || ba->dstate != ba->dstate_out, "ic_lattn_bwd: dstate is dstate_out");
   IC_REQUIRE(a->ws && ((uintptr_t)a->ws & 7) == 0, "ic_lattn_bwd: the workspace is NULL or not on 8 bytes");
+  if ((rc = check_stride(a->q_st, "ic_lattn_bwd", "q")) || (rc = check_stride(a->k_st, "ic_lattn_bwd", "k")) ||
+      (rc = check_stride(a->v_st, "ic_lattn_bwd", "v")) || (rc = check_stride(ba->do_st, "ic_lattn_bwd", "dout")) ||
+      (rc = check_stride(ba->dq_st, "ic_lattn_bwd", "dq")) || (rc = check_stride(ba->dk_st, "ic_lattn_bwd", "dk")) ||
+      (rc = check_stride(ba->dv_st, "ic_lattn_bwd", "dv"))) return rc;
   const Geo g = geo_of(a, 3);
   const int esz = ic_dt_size(a->dtype), G = a->H / a->Hk, dp = pad_of(a), bh = a->B * a->H, Dk = a->Dk, Dv = a->Dv;
   const int64_t dd = (int64_t)Dk * Dv;
@@ -955,6 +1042,8 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
   const Mat q = mat(a->q, a->q_sb, a->q_sh, a->q_st, 1, Dk, esz), k = mat(a->k, a->k_sb, a->k_sh, a->k_st, G, Dk, esz);
   const Mat v = mat(a->v, a->v_sb, a->v_sh, a->v_st, G, Dv, esz), o = mat(ba->dout, ba->do_sb, ba->do_sh, ba->do_st, 1, Dv, esz);
   const Mat dk = mat(ba->dk, ba->dk_sb, ba->dk_sh, ba->dk_st, G, Dk, esz), dv = mat(ba->dv, ba->dv_sb, ba->dv_sh, ba->dv_st, G, Dv, esz);
+  const Mat dq = mat(ba->dq, ba->dq_sb, ba->dq_sh, ba->dq_st, 1, Dk, esz);
+  const bool wide = a->dtype == IC_DT_BF16 && q.vec && k.vec && v.vec && o.vec && dq.vec && dk.vec && dv.vec;
   double* dr = (double*)a->ws;
   float* ws = a->ws + 2 * (int64_t)bh * g.nseg;
   float* seg_s = ws;                                // S (and L): transposed, [Dv][Dk]
@@ -968,14 +1057,14 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
     s.s[1] = Sums{q, o, Dk, Dv, 1, 0, a->scale, seg_r};
 #define IC_BODY(T, DP)                                                                                                                        \
   if (lag) {                                                                                                                                   \
-    IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, true>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, s));         \
+    IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, true, W16>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, s));         \
     SumArgs s1 = s;                                                                                                                            \
     s1.s[0] = s.s[1];                                                                                                                          \
-    IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, s1));       \
+    IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, s1));       \
   } else {                                                                                                                                     \
-    IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, s));        \
+    IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, s));        \
   }
-    IC_LATTN_T(a->dtype, IC_BODY_T);
+    IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
     IC_LAUNCH_CHECK("ic_lattn_bwd");
     ScanArgs sc{};
@@ -991,7 +1080,7 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
   p.g = g;
   Pass& pq = p.p[0];  // dq
   pq.q = o; pq.k = v; pq.v = k; pq.x = q;
-  pq.out = mat(ba->dq, ba->dq_sb, ba->dq_sh, ba->dq_st, 1, Dk, esz);
+  pq.out = dq;
   pq.Da = Dv; pq.Db = Dk;
   pq.oscale = a->scale; pq.vscale = 1.f;
   pq.init = a->state; pq.ia = 1; pq.ib = Dv;
@@ -1022,15 +1111,15 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
   }
 #define IC_BODY(T, DP)                                                                                                              \
   if (lag) {                                                                                                                       \
-    IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, true>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, p));   \
+    IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, true, W16>), dim3(bh * g.nseg, 1), dim3(DP * 4 / cw_of<DP, true, W16>()), 0, st, p));   \
     PassArgs p1 = p;                                                                                                               \
     p1.p[0] = p.p[1];                                                                                                              \
     p1.p[1] = p.p[2];                                                                                                              \
-    IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, p1)); \
+    IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false, W16>), dim3(bh * g.nseg, 2), dim3(DP * 4 / cw_of<DP, false, W16>()), 0, st, p1)); \
   } else {                                                                                                                         \
-    IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false>), dim3(bh * g.nseg, 3), dim3(DP * 4), 0, st, p));  \
+    IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false, W16>), dim3(bh * g.nseg, 3), dim3(DP * 4 / cw_of<DP, false, W16>()), 0, st, p));  \
   }
-  IC_LATTN_T(a->dtype, IC_BODY_T);
+  IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
   IC_LAUNCH_CHECK("ic_lattn_bwd");
   if (G > 1) {
@@ -1042,7 +1131,7 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
     const int64_t most = (int64_t)a->B * a->Hk * a->T * (Dk > Dv ? Dk : Dv);
     const int blocks = (int)(most / 256 + 1 < 4096 ? most / 256 + 1 : 4096);
 #define IC_BODY(T) IC_TIMED(IC_KID_lattn_join, st, hipLaunchKernelGGL(k_lattn_join<T>, dim3(blocks, 2), dim3(256), 0, st, j));
-    IC_LATTN_T(a->dtype, IC_BODY);
+    IC_LATTN_T(a->dtype, false, IC_BODY);
 #undef IC_BODY
     IC_LAUNCH_CHECK("ic_lattn_bwd");
   }
@@ -1063,7 +1152,7 @@ extern "C" int ic_lattn_step(const ic_lattn_step_args* a, ic_stream_t stream) {
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid(a->B * a->H, ic_ceil_div(a->Dv, 32));
 #define IC_BODY(T) IC_TIMED(IC_KID_lattn_step, st, hipLaunchKernelGGL(k_lattn_step<T>, grid, dim3(256), 0, st, *a));
-  IC_LATTN_T(a->dtype, IC_BODY);
+  IC_LATTN_T(a->dtype, false, IC_BODY);
 #undef IC_BODY
   IC_LAUNCH_CHECK("ic_lattn_step");
   return IC_OK;
