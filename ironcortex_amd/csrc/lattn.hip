@@ -794,16 +794,28 @@ __global__ __launch_bounds__(256) void k_lattn_scan(ScanArgs a) {
   const int nst = z.lag ? 2 : 1;
   float* at = z.seg + (size_t)bh * a.g.nseg * nst * dd + e;
   float S = z.init ? z.init[(size_t)bh * dd + (size_t)(e / z.Db) * z.ia + (size_t)(e % z.Db) * z.ib] : 0.f, L = 0.f;
-  for (int s = 0; s < a.g.nseg; ++s, at += (size_t)nst * dd) {
-    int cnt = n - s * len;
-    cnt = cnt < 0 ? 0 : cnt < len ? cnt : len;
-    const bool more = s + 1 < a.g.nseg;  // (the last segment's sum is not formed)
-    const float ls = more ? at[0] : 0.f, ll = more && z.lag ? at[dd] : 0.f;
-    at[0] = S;
-    if (z.lag) at[dd] = L;
-    const float carry = decay(l2, cnt > 0 && z.rev && s == 0 ? cnt - 1 : cnt);
-    L = carry * (L + (float)cnt * S) + ll;
-    S = carry * S + ls;
+  const size_t next = (size_t)nst * dd;
+  constexpr int U = 8;  // sums in flight: the chain of states would wait for each of them in turn otherwise
+  for (int s0 = 0; s0 < a.g.nseg; s0 += U, at += U * next) {
+    float ls[U], ll[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool more = s0 + u + 1 < a.g.nseg;  // (the last segment's sum is not formed)
+      ls[u] = more ? at[u * next] : 0.f;
+      ll[u] = more && z.lag ? at[u * next + dd] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u;
+      if (s >= a.g.nseg) break;
+      int cnt = n - s * len;
+      cnt = cnt < 0 ? 0 : cnt < len ? cnt : len;
+      at[u * next] = S;
+      if (z.lag) at[u * next + dd] = L;
+      const float carry = decay(l2, cnt > 0 && z.rev && s == 0 ? cnt - 1 : cnt);
+      L = carry * (L + (float)cnt * S) + ll[u];
+      S = carry * S + ls[u];
+    }
   }
 }
 
@@ -814,18 +826,32 @@ struct JoinArgs {
   int32_t D[2];
   int32_t B, H, Hk, T;
 };
+// memory-bound; four channels a thread where the rows allow it
 template <typename T>
 __global__ __launch_bounds__(256) void k_lattn_join(JoinArgs a) {
   const int z = blockIdx.y, D = a.D[z], G = a.H / a.Hk;
-  const int64_t n = (int64_t)a.B * a.Hk * a.T * D;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / D;
-    const int j = (int)(i - row * D);
-    const int64_t bk = row / a.T;
-    const int t = (int)(row - bk * a.T), b = (int)(bk / a.Hk), hk = (int)(bk - (int64_t)b * a.Hk);
-    float v = 0.f;
-    for (int gi = 0; gi < G; ++gi) v += a.part[z][(((int64_t)b * a.H + (int64_t)hk * G + gi) * a.T + t) * D + j];
-    ((T*)a.out[z].p)[(int64_t)b * a.out[z].sb + (int64_t)hk * a.out[z].sh + (int64_t)t * a.out[z].st + j] = ic_from_f<T>(v);
+  const Mat& o = a.out[z];
+  const int V = o.vec ? 4 : 1;
+  const uint32_t per = D / V;
+  const uint32_t rows = (uint32_t)a.T;
+  const int hk = blockIdx.z % a.Hk, b = blockIdx.z / a.Hk;
+  const float* part = a.part[z] + ((int64_t)b * a.H + (int64_t)hk * G) * a.T * D;
+  const int64_t hs = (int64_t)a.T * D;
+  T* out = (T*)o.p + (int64_t)b * o.sb + (int64_t)hk * o.sh;
+  for (uint32_t r = blockIdx.x * 256 + threadIdx.x; r < rows * per; r += gridDim.x * 256) {
+    const uint32_t t = r / per, j = (r - t * per) * V;
+    const float* x = part + (int64_t)t * D + j;
+    T* y = out + (int64_t)t * o.st + j;
+    if (V == 4) {
+      v4f v = ld4(x);
+      for (int gi = 1; gi < G; ++gi) v += ld4(x + gi * hs);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) y[u] = ic_from_f<T>(v[u]);
+    } else {
+      float v = *x;
+      for (int gi = 1; gi < G; ++gi) v += x[gi * hs];
+      *y = ic_from_f<T>(v);
+    }
   }
 }
 // d rate of a head: over sequences and segments, in 64 bits
@@ -917,21 +943,41 @@ int pad_of(const ic_lattn_args* a) {
   return d <= 32 ? 32 : d <= 64 ? 64 : 128;
 }
 
-// Segments: as many as bring `passes` x B x H x segments to the number of workgroups that fill the chip, and no more, since
-// every further one costs its sums.
-Geo geo_of(const ic_lattn_args* a, int passes) {
+// Segments of a sequence: the number for which the last of the launch's workgroups ends first, counted in chunks.  A chip of
+// 256 compute units holds `slots` workgroups at a time (LDS and registers: see the kernels); every round of them takes the
+// chunks of a segment and about one more (start state, first loads), and with more than one segment their sums come first,
+// at 0.4 of a chunk's time each.  (passes x B x H = 64, 64 chunks, 512 slots: 8 segments, 9.0 + 3.2 chunks against 65.)
+Geo geo_of(const ic_lattn_args* a, int passes, int slots) {
   Geo g;
   g.B = a->B; g.H = a->H; g.T = a->T;
   g.rate = a->rate;
   g.valid_len = a->valid_len;
   const int NC = ic_ceil_div(a->T, kC);
-  const int64_t have = (int64_t)passes * a->B * a->H, want = 512;
-  int64_t ns = (want + have - 1) / have;
-  if (ns > NC) ns = NC;
-  g.cps = (int)((NC + ns - 1) / ns);
-  g.nseg = ic_ceil_div(NC, g.cps);
+  const int64_t bh = (int64_t)a->B * a->H, have = bh * passes;
+  double best = 0.0;
+  g.nseg = 1;
+  g.cps = NC;
+  const int64_t most = (2 * slots + have - 1) / have;
+  for (int ns = 1; ns <= most && ns <= NC; ++ns) {
+    const int cps = ic_ceil_div(NC, ns);
+    if (ic_ceil_div(NC, cps) != ns) continue;
+    const double rounds = (double)((have * ns + slots - 1) / slots);
+    const double cost = rounds * (cps + 1.0) + (ns > 1 ? 0.4 * rounds * cps + 2.0 : 0.0);
+    if (ns == 1 || cost < best) {
+      best = cost;
+      g.nseg = ns;
+      g.cps = cps;
+    }
+  }
   return g;
 }
+int slots_of(const ic_lattn_args* a, bool lag) {
+  const int dp = pad_of(a);
+  return 256 * (dp == 32 ? 4 : dp == 64 ? 2 : a->dtype == IC_DT_BF16 && !lag ? 2 : 1);
+}
+Geo geo_fwd(const ic_lattn_args* a) { return geo_of(a, 1, slots_of(a, false)); }
+// (with d rate the dq pass is a launch of its own, and the smaller of the two)
+Geo geo_bwd(const ic_lattn_args* a, bool lag) { return geo_of(a, lag ? 1 : 3, slots_of(a, lag)); }
 
 Mat mat(const void* p, int64_t sb, int64_t sh, int64_t st, int group, int D, int esz) {
   Mat m;
@@ -943,15 +989,22 @@ Mat mat(const void* p, int64_t sb, int64_t sh, int64_t st, int group, int D, int
   return m;
 }
 
+// floats of workspace: the segments' states (backward: the forward state and, for d rate, its lag-weighted companion, and the
+// reversed state), partial sums of d rate (doubles), partial gradients of shared heads
 int64_t ws_floats(const ic_lattn_args* a, int backward) {
-  const Geo g = geo_of(a, backward ? 3 : 1);
   const int64_t bh = (int64_t)a->B * a->H, dd = (int64_t)a->Dk * a->Dv;
-  int64_t n = 0;
-  if (g.nseg > 1) n += bh * g.nseg * dd * (backward ? 3 : 1);
-  if (backward) {
-    n += 2 * bh * g.nseg + 2;  // (doubles, on 8 bytes)
-    if (a->H != a->Hk) n += bh * a->T * (int64_t)(a->Dk + a->Dv);
+  if (!backward) {
+    const Geo g = geo_fwd(a);
+    return g.nseg > 1 ? bh * g.nseg * dd : 0;
   }
+  int64_t n = 0;
+  for (int lag = 0; lag < 2; ++lag) {  // (whether d rate is wanted is the call's matter, not the sizes')
+    const Geo g = geo_bwd(a, lag);
+    const int64_t m = (lag ? 2 * bh * g.nseg : 0) + (g.nseg > 1 ? bh * g.nseg * dd * (lag ? 3 : 2) : 0);
+    n = n > m ? n : m;
+  }
+  n += 2;
+  if (a->H != a->Hk) n += bh * a->T * (int64_t)(a->Dk + a->Dv) + 8;
   return n;
 }
 
@@ -985,7 +1038,7 @@ extern "C" int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream) {
   IC_REQUIRE(a->ws || ws_floats(a, 0) == 0, "ic_lattn_fwd: NULL workspace");
   if ((rc = check_stride(a->q_st, "ic_lattn_fwd", "q")) || (rc = check_stride(a->k_st, "ic_lattn_fwd", "k")) ||
       (rc = check_stride(a->v_st, "ic_lattn_fwd", "v")) || (rc = check_stride(a->o_st, "ic_lattn_fwd", "out"))) return rc;
-  const Geo g = geo_of(a, 1);
+  const Geo g = geo_fwd(a);
   const int esz = ic_dt_size(a->dtype), G = a->H / a->Hk, dp = pad_of(a), bh = a->B * a->H;
   hipStream_t st = (hipStream_t)stream;
   const Mat q = mat(a->q, a->q_sb, a->q_sh, a->q_st, 1, a->Dk, esz), k = mat(a->k, a->k_sb, a->k_sh, a->k_st, G, a->Dk, esz);
@@ -1034,22 +1087,22 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
       (rc = check_stride(a->v_st, "ic_lattn_bwd", "v")) || (rc = check_stride(ba->do_st, "ic_lattn_bwd", "dout")) ||
       (rc = check_stride(ba->dq_st, "ic_lattn_bwd", "dq")) || (rc = check_stride(ba->dk_st, "ic_lattn_bwd", "dk")) ||
       (rc = check_stride(ba->dv_st, "ic_lattn_bwd", "dv"))) return rc;
-  const Geo g = geo_of(a, 3);
+  const bool lag = ba->drate != nullptr;
+  const Geo g = geo_bwd(a, lag);
   const int esz = ic_dt_size(a->dtype), G = a->H / a->Hk, dp = pad_of(a), bh = a->B * a->H, Dk = a->Dk, Dv = a->Dv;
   const int64_t dd = (int64_t)Dk * Dv;
-  const bool lag = ba->drate != nullptr;
   hipStream_t st = (hipStream_t)stream;
   const Mat q = mat(a->q, a->q_sb, a->q_sh, a->q_st, 1, Dk, esz), k = mat(a->k, a->k_sb, a->k_sh, a->k_st, G, Dk, esz);
   const Mat v = mat(a->v, a->v_sb, a->v_sh, a->v_st, G, Dv, esz), o = mat(ba->dout, ba->do_sb, ba->do_sh, ba->do_st, 1, Dv, esz);
   const Mat dk = mat(ba->dk, ba->dk_sb, ba->dk_sh, ba->dk_st, G, Dk, esz), dv = mat(ba->dv, ba->dv_sb, ba->dv_sh, ba->dv_st, G, Dv, esz);
   const Mat dq = mat(ba->dq, ba->dq_sb, ba->dq_sh, ba->dq_st, 1, Dk, esz);
   const bool wide = a->dtype == IC_DT_BF16 && q.vec && k.vec && v.vec && o.vec && dq.vec && dk.vec && dv.vec;
-  double* dr = (double*)a->ws;
-  float* ws = a->ws + 2 * (int64_t)bh * g.nseg;
-  float* seg_s = ws;                                // S (and L): transposed, [Dv][Dk]
-  float* seg_r = ws + (int64_t)bh * g.nseg * dd * 2;  // the reversed state, [Dk][Dv]
-  if (g.nseg > 1) ws += (int64_t)bh * g.nseg * dd * 3;
   const int nst = lag ? 2 : 1;
+  double* dr = (double*)a->ws;
+  float* seg_s = a->ws + (lag ? 2 * (int64_t)bh * g.nseg : 0);  // S (and L): transposed, [Dv][Dk]
+  float* seg_r = seg_s + (int64_t)bh * g.nseg * dd * nst;       // the reversed state, [Dk][Dv]
+  float* ws = g.nseg > 1 ? seg_r + (int64_t)bh * g.nseg * dd : seg_s;
+  ws += -(((uintptr_t)ws / 4)) & 3;  // (the partial gradients' rows on 16 bytes)
   if (g.nseg > 1) {
     SumArgs s{};
     s.g = g;
@@ -1128,9 +1181,9 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
     j.out[0] = dk; j.out[1] = dv;
     j.D[0] = Dk; j.D[1] = Dv;
     j.B = a->B; j.H = a->H; j.Hk = a->Hk; j.T = a->T;
-    const int64_t most = (int64_t)a->B * a->Hk * a->T * (Dk > Dv ? Dk : Dv);
-    const int blocks = (int)(most / 256 + 1 < 4096 ? most / 256 + 1 : 4096);
-#define IC_BODY(T) IC_TIMED(IC_KID_lattn_join, st, hipLaunchKernelGGL(k_lattn_join<T>, dim3(blocks, 2), dim3(256), 0, st, j));
+    const int64_t most = ((int64_t)a->T * (Dk > Dv ? Dk : Dv) + 2047) / 2048;  // (eight elements a thread)
+    const int blocks = (int)(most < 4096 ? most : 4096);
+#define IC_BODY(T) IC_TIMED(IC_KID_lattn_join, st, hipLaunchKernelGGL(k_lattn_join<T>, dim3(blocks, 2, a->B * a->Hk), dim3(256), 0, st, j));
     IC_LATTN_T(a->dtype, false, IC_BODY);
 #undef IC_BODY
     IC_LAUNCH_CHECK("ic_lattn_bwd");
