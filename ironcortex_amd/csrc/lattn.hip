@@ -133,40 +133,60 @@ struct LdsSums {
   float Ks[kC][DP + 4];
 };
 
-// the end of a segment: its sums, or (last segment) the end state and its share of d rate; d rate's partial sum.
-// S[t][v]: element (16 t + q4 + v, col)
-template <bool LAG, int NT, int NL>
-__device__ __forceinline__ void write_sums(const Geo& g, const Sums* sm, const v4f (&S)[NT], const v4f (&L)[NL], size_t dd, int Da, int Db, int col, int q4, int bh, int seg) {
-  float* dst = sm->seg + ((size_t)bh * g.nseg + seg) * (LAG ? 2 : 1) * dd;
+// A wave's slice of a state: elements (16 t + q4 + v, col) at a * ia + b * ib of src.  Out of range: zero, read at a clamped
+// address and without a branch, so that all loads are in flight together.
+template <int NT>
+__device__ __forceinline__ void load_state(v4f (&S)[NT], const float* src, int ia, int ib, int Da, int Db, int col, int q4) {
+  const bool in = col < Db;
+  const float* at = src + (size_t)(in ? col : 0) * ib;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const int a = 16 * t + q4 + v;
-      if (a < Da && col < Db) {
-        dst[(size_t)a * Db + col] = S[t][v];
-        if constexpr (LAG) dst[dd + (size_t)a * Db + col] = L[t][v];
-      }
+      const bool ok = in && a < Da;
+      const float x = at[(size_t)(ok ? a : 0) * ia];
+      S[t][v] = ok ? x : 0.f;
     }
+}
+template <int NT>
+__device__ __forceinline__ void store_state(const v4f (&S)[NT], float* dst, int ia, int ib, int Da, int Db, int col, int q4, float f) {
+  if (col >= Db) return;
+  float* at = dst + (size_t)col * ib;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int a = 16 * t + q4 + v;
+      if (a < Da) at[(size_t)a * ia] = S[t][v] * f;
+    }
+}
+template <int NT>
+__device__ __forceinline__ double dot_state(const v4f (&S)[NT], const float* src, int ia, int ib, int Da, int Db, int col, int q4) {
+  v4f G[NT];
+  load_state(G, src, ia, ib, Da, Db, col, q4);
+  double d = 0.0;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) d += (double)S[t][v] * (double)G[t][v];
+  return d;
+}
+// the end of a segment: its sums, or (last segment) the end state and its share of d rate; d rate's partial sum.
+template <bool LAG, int NT, int NL>
+__device__ __forceinline__ void write_sums(const Geo& g, const Sums* sm, const v4f (&S)[NT], const v4f (&L)[NL], size_t dd, int Da, int Db, int col, int q4, int bh, int seg) {
+  float* dst = sm->seg + ((size_t)bh * g.nseg + seg) * (LAG ? 2 : 1) * dd;
+  store_state(S, dst, Db, 1, Da, Db, col, q4, 1.f);
+  if constexpr (LAG) store_state(L, dst + dd, Db, 1, Da, Db, col, q4, 1.f);
 }
 template <bool LAG, int NT, int NL>
 __device__ __forceinline__ double write_end(const Geo& g, const Pass* p, const v4f (&S)[NT], const v4f (&L)[NL], size_t dd, int Da, int Db, int col, int q4, int bh, int seg, int n, float l2) {
   double dr = 0.0;
   if (seg != g.nseg - 1) return dr;
-  const float last = p->fin_decay && n > 0 ? decay(l2, 1) : 1.f;
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int a = 16 * t + q4 + v;
-      if (a < Da && col < Db) {
-        const size_t at = (size_t)bh * dd + (size_t)a * p->ia + (size_t)col * p->ib;
-        if (p->fin) p->fin[at] = S[t][v] * last;
-        if constexpr (LAG) {
-          if (p->gfin) dr -= (double)L[t][v] * (double)p->gfin[at];
-        }
-      }
-    }
+  if (p->fin) store_state(S, p->fin + (size_t)bh * dd, p->ia, p->ib, Da, Db, col, q4, p->fin_decay && n > 0 ? decay(l2, 1) : 1.f);
+  if constexpr (LAG) {
+    if (p->gfin) dr -= dot_state(L, p->gfin + (size_t)bh * dd, p->ia, p->ib, Da, Db, col, q4);
+  }
   return dr;
 }
 template <int NW>
@@ -211,16 +231,10 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
     const float* s0 = p->seg ? p->seg + ((size_t)bh * g.nseg + seg) * p->nst * dd : p->init ? p->init + (size_t)bh * dd : nullptr;
     const int ia = p->seg ? p->sga : p->ia, ib = p->seg ? p->sgb : p->ib;
     if (s0) {
-#pragma unroll
-      for (int t = 0; t < KS; ++t)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int a = 16 * t + q4 + v;
-          if (a < Da && col < Db) {
-            S[t][v] = s0[(size_t)a * ia + (size_t)col * ib];
-            if (LAG && p->seg) L[t][v] = s0[dd + (size_t)a * ia + (size_t)col * ib];
-          }
-        }
+      load_state(S, s0, ia, ib, Da, Db, col, q4);
+      if constexpr (LAG) {
+        if (p->seg) load_state(L, s0 + dd, ia, ib, Da, Db, col, q4);
+      }
     }
   }
   double dr = 0.0;
@@ -375,9 +389,9 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
 // Rows that allow 16-byte accesses (others take the body above).
 // The same map on bf16 matrix instructions (16x16x32: sixteen times the fp32 rate).  Products of rows (q . k) are exact
 // there.  Operands that are computed in fp32 -- the decayed products P, the state, the decay-weighted values -- are split
-// into bf16 parts (x = x1 + x2 [+ x3], each the rounded rest of the one before: 8 bits of the value apiece): two parts where
-// the sum ends in a bf16 output (2^-17 of a term against the output's own 2^-9), three where it ends in an fp32 one (the
-// state, d rate).  Rows lie in LDS as they come; column operands (k^T, v^T) are read with the transposing LDS load
+// into two bf16 parts (x = x1 + x2, x2 the rounded rest: 16 bits of the value; an error of at most 2^-18 of a term, 2^-20.5
+// in the mean square, where the outputs' own rounding is 2^-9 and the fp32 state keeps 20 bits of a sum of such terms).
+// Rows lie in LDS as they come; column operands (k^T, v^T) are read with the transposing LDS load
 // (16 lanes x 8 bytes of four rows -> four rows of one column per lane).  A 32-deep operand of a lane is therefore k-indices
 // 4 q .. 4 q + 3 of either 16-row half, on both sides of a product; products of rows use contiguous eights instead.
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
@@ -395,13 +409,13 @@ struct Lds16 {
   RowTile<DP + 8> Q;
   RowTile<LAG ? DP + 8 : 8> X;
   uint16_t P1[kC][kPw], P2[kC][kPw];
-  float dec[2 * kC + 1];  // dec[kC + lag] = e^{-r lag}, 0 for lag < 0
+  float dec[2 * kC + 1], dev[2 * kC + 1];  // dec[kC + lag] = e^{-r lag}, 0 for lag < 0; dev = dec * vscale
   double red[DP / 16];
 };
 template <int DP>
 struct LdsSums16 {
   RowTile<DP + 16> K, V;
-  float dec[2 * kC + 1];
+  float dec[2 * kC + 1], dev[2 * kC + 1];
 };
 
 __device__ __forceinline__ v4f mma32(b8 a, b8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -422,7 +436,7 @@ __device__ __forceinline__ b8 lds_col(const uint16_t (*t)[W], int r0, int c0, in
   x.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)(p + 16 * W));
   return x.b;
 }
-// bf16 parts of fp32 values, two at a time: the next part of x, x keeps the rest
+// two values' bf16 parts; take2: x keeps the rest
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack2(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2)); }
@@ -432,20 +446,19 @@ __device__ __forceinline__ uint32_t take2(float& a, float& b) {
   b -= __uint_as_float(u & 0xffff0000u);
   return u;
 }
-template <int N>
-__device__ __forceinline__ void split(float (&x)[8], b8 (&out)[N]) {
+__device__ __forceinline__ void split(float (&x)[8], b8 (&out)[2]) {
+  union { uint32_t u[4]; b8 b; } y, z;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    union { uint32_t u[4]; b8 b; } y;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) y.u[u] = i + 1 < N ? take2(x[2 * u], x[2 * u + 1]) : pack2(x[2 * u], x[2 * u + 1]);
-    out[i] = y.b;
+  for (int u = 0; u < 4; ++u) {
+    y.u[u] = take2(x[2 * u], x[2 * u + 1]);
+    z.u[u] = pack2(x[2 * u], x[2 * u + 1]);
   }
+  out[0] = y.b;
+  out[1] = z.b;
 }
-template <int N>
-__device__ __forceinline__ void split(const v4f& a, const v4f& b, b8 (&out)[N]) {
+__device__ __forceinline__ void split(const v4f& a, const v4f& b, b8 (&out)[2]) {
   float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-  split<N>(x, out);
+  split(x, out);
 }
 
 // four consecutive columns of an output row
@@ -466,6 +479,7 @@ struct Rows {
   int64_t step;
   uint32_t off;  // this lane's piece of row threadIdx / (DP / 8)
   bool live;     // inside the row
+  bool whole;    // (uniform) every lane is
   __device__ __forceinline__ void open(const Mat& m, int b, int h, int D, int n, int rev) {
     constexpr int PER = DP / 8;
     const int64_t st = m.st * 2;
@@ -473,12 +487,18 @@ struct Rows {
     step = rev ? -st : st;
     const int r = threadIdx.x / PER, c = (threadIdx.x % PER) * 8;
     live = c < D;
+    whole = D == DP;
     off = (uint32_t)((rev ? kC - 1 - r : r) * (int32_t)st + c * 2);
   }
   // rows [base, base + cnt) (virtual positions); others read as zero
   __device__ __forceinline__ void fetch(uint4 (&x)[NP], int base, int cnt) const {
     const int r = threadIdx.x / (DP / 8);
     const char* at = src + base * step;
+    if (cnt == kC && whole) {  // (no lane left out)
+#pragma unroll
+      for (int j = 0; j < NP; ++j, at += RT * step) x[j] = *reinterpret_cast<const uint4*>(at + off);
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < NP; ++j, at += RT * step) {
       x[j] = make_uint4(0, 0, 0, 0);
@@ -497,7 +517,6 @@ struct Rows {
 template <int DP, int CW, bool LAG, bool SUMS, typename LDS>
 __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const Sums* sm, LDS& lds) {
   constexpr int NW = DP / (16 * CW), NT = DP / 16, KS = DP / 32, MT = (10 + NW - 1) / NW;
-  constexpr int RP = LAG ? 3 : 2;  // parts of the state where it is read
   using R = Rows<DP, CW>;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, q4 = (lane >> 4) * 4;
   const int seg = blockIdx.x % g.nseg, bh = blockIdx.x / g.nseg, b = bh / g.H, h = bh - b * g.H;
@@ -511,7 +530,11 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
   rv.open(SUMS ? sm->v : p->v, b, h, Db, n, rev);
   if constexpr (!SUMS) rq.open(p->q, b, h, Da, n, rev);
   if constexpr (!SUMS && LAG) rx.open(p->x, b, h, Db, n, rev);
-  for (int i = threadIdx.x; i < 2 * kC + 1; i += 64 * NW) lds.dec[i] = i < kC ? 0.f : decay(l2, i - kC);
+  for (int i = threadIdx.x; i < 2 * kC + 1; i += 64 * NW) {
+    const float d = i < kC ? 0.f : decay(l2, i - kC);
+    lds.dec[i] = d;
+    lds.dev[i] = d * vscale;
+  }
   const int col0 = 16 * CW * w;  // this wave's columns
   const int NC = (T + kC - 1) / kC;
   const int ch0 = seg * g.cps, ch1 = ch0 + g.cps < NC ? ch0 + g.cps : NC;
@@ -539,19 +562,12 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
     const int ia = p->seg ? p->sga : p->ia, ib = p->seg ? p->sgb : p->ib;
     if (s0) {
 #pragma unroll
-      for (int k = 0; k < CW; ++k)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const int a = 16 * t + q4 + v, col = col0 + 16 * k + c;
-            if (a < Da && col < Db) {
-              S[k][t][v] = s0[(size_t)a * ia + (size_t)col * ib];
-              if constexpr (LAG) {
-                if (p->seg) L[k][t][v] = s0[dd + (size_t)a * ia + (size_t)col * ib];
-              }
-            }
-          }
+      for (int k = 0; k < CW; ++k) {
+        load_state(S[k], s0, ia, ib, Da, Db, col0 + 16 * k + c, q4);
+        if constexpr (LAG) {
+          if (p->seg) load_state(L[k], s0 + dd, ia, ib, Da, Db, col0 + 16 * k + c, q4);
+        }
+      }
     }
     // the two 16x16 tiles of P above the diagonal that a 32-deep product reads stay zero
     for (int i = threadIdx.x; i < 128; i += 64 * NW) {
@@ -605,8 +621,8 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
           const int lag0 = 16 * (it - jt) + c - q4;
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            const float d = lds.dec[kC + lag0 - v] * (vscale * oscale);
-            x[v] = lag0 >= v ? acc[v] * d : 0.f;  // (a select: what lies above the diagonal may be infinite)
+            const float d = lds.dev[kC + lag0 - v];
+            x[v] = lag0 >= v ? acc[v] * (d * oscale) : 0.f;  // (a select: what lies above the diagonal may be infinite)
             if constexpr (LAG) drc = lag0 > v ? fmaf((float)(lag0 - v) * x[v], ax[v], drc) : drc;
           }
           uint2 p1, p2;
@@ -627,17 +643,17 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
           }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          b8 sp[CW][RP], lp[LAG ? CW : 1][RP];
+          b8 sp[CW][2], lp[LAG ? CW : 1][2];
 #pragma unroll
           for (int k = 0; k < CW; ++k) {
-            split<RP>(S[k][2 * s], S[k][2 * s + 1], sp[k]);
-            if constexpr (LAG) split<RP>(L[k][2 * s], L[k][2 * s + 1], lp[k]);
+            split(S[k][2 * s], S[k][2 * s + 1], sp[k]);
+            if constexpr (LAG) split(L[k][2 * s], L[k][2 * s + 1], lp[k]);
           }
 #pragma unroll
           for (int it = 0; it < 4; ++it) {
             const b8 bq = lds8x2(&lds.Q.r[16 * it + c][32 * s + q4]);
 #pragma unroll
-            for (int i = 0; i < RP; ++i)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
               for (int k = 0; k < CW; ++k) {
                 O[k][it] = mma32(sp[k][i], bq, O[k][it]);
@@ -667,10 +683,9 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
           for (int s = 0; s <= it / 2; ++s) {
             const b8 x1 = lds16(&lds.P1[16 * it + c][32 * s + 2 * q4]), x2 = lds16(&lds.P2[16 * it + c][32 * s + 2 * q4]);
 #pragma unroll
-            for (int k = 0; k < CW; ++k) {
-              O[k][it] = mma32(vf[k][s], x1, O[k][it]);
-              O[k][it] = mma32(vf[k][s], x2, O[k][it]);
-            }
+            for (int k = 0; k < CW; ++k) O[k][it] = mma32(vf[k][s], x1, O[k][it]);
+#pragma unroll
+            for (int k = 0; k < CW; ++k) O[k][it] = mma32(vf[k][s], x2, O[k][it]);
           }
       }
     }
@@ -709,25 +724,25 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
         }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        b8 vp[CW][3], lp[LAG ? CW : 1][3];
-        const float* dl = &lds.dec[kC + cnt - 1 - q4 - 51];  // (51: the largest position of this lane's values)
+        b8 vp[CW][2], lp[LAG ? CW : 1][2];
+        const float* dl = &lds.dev[kC + cnt - 1 - q4 - 51];  // (51: the largest position of this lane's values)
 #pragma unroll
         for (int k = 0; k < CW; ++k) {
           float x[8], y[8];
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
             const int j = 32 * s + 16 * (u >> 2) + (u & 3);
-            x[u] = (float)vf[k][s][u] * (dl[51 - j] * vscale);
+            x[u] = (float)vf[k][s][u] * dl[51 - j];
             if constexpr (LAG) y[u] = x[u] * (float)(cnt - 1 - q4 - j);  // (0 behind the last valid position)
           }
-          split<3>(x, vp[k]);
-          if constexpr (LAG) split<3>(y, lp[k]);
+          split(x, vp[k]);
+          if constexpr (LAG) split(y, lp[k]);
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const b8 ak = lds_col(lds.K.r, 32 * s, 16 * t, lane);
 #pragma unroll
-          for (int i = 0; i < 3; ++i)
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int k = 0; k < CW; ++k) {
               S[k][t] = mma32(ak, vp[k][i], S[k][t]);
@@ -832,16 +847,17 @@ __global__ __launch_bounds__(256) void k_lattn_join(JoinArgs a) {
   const int z = blockIdx.y, D = a.D[z], G = a.H / a.Hk;
   const Mat& o = a.out[z];
   const int V = o.vec ? 4 : 1;
-  const uint32_t per = D / V;
-  const uint32_t rows = (uint32_t)a.T;
+  const int per = D / V;
+  const int64_t n = (int64_t)a.T * per;
   const int hk = blockIdx.z % a.Hk, b = blockIdx.z / a.Hk;
   const float* part = a.part[z] + ((int64_t)b * a.H + (int64_t)hk * G) * a.T * D;
   const int64_t hs = (int64_t)a.T * D;
   T* out = (T*)o.p + (int64_t)b * o.sb + (int64_t)hk * o.sh;
-  for (uint32_t r = blockIdx.x * 256 + threadIdx.x; r < rows * per; r += gridDim.x * 256) {
-    const uint32_t t = r / per, j = (r - t * per) * V;
-    const float* x = part + (int64_t)t * D + j;
-    T* y = out + (int64_t)t * o.st + j;
+  for (int64_t r = blockIdx.x * 256 + threadIdx.x; r < n; r += gridDim.x * 256) {
+    const int64_t t = n < (1ll << 31) ? (uint32_t)r / (uint32_t)per : r / per;
+    const int j = (int)(r - t * per) * V;
+    const float* x = part + t * D + j;
+    T* y = out + t * o.st + j;
     if (V == 4) {
       v4f v = ld4(x);
       for (int gi = 1; gi < G; ++gi) v += ld4(x + gi * hs);
