@@ -88,29 +88,109 @@ __device__ __forceinline__ const T* row_base(const Mat& m, int b, int h) {
   return (const T*)m.p + (int64_t)b * m.sb + (int64_t)(h / m.group) * m.sh;
 }
 
-// rows [t0, t0 + kC) (virtual positions; rows >= cnt read as zero) of width D -> fp32 tile with padded rows
-template <typename T, int DP, int NT>
-__device__ __forceinline__ void stage(float (*dst)[DP + 4], const T* src, const Mat& m, int D, int base, int cnt, int n, int rev) {
-  constexpr int VE = 16 / (int)sizeof(T), PER = DP / VE;
-  for (int i = threadIdx.x; i < kC * PER; i += NT) {
-    const int r = i / PER, c = (i - r * PER) * VE;
-    T e[VE];
-    *reinterpret_cast<uint4*>(e) = make_uint4(0, 0, 0, 0);
-    if (r < cnt) {
-      const T* row = src + (int64_t)(rev ? n - 1 - (base + r) : base + r) * m.st;
-      if (m.vec) {
-        if (c < D) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(row + c);
-      } else {
+// Rows of one matrix as a workgroup reads them: 16-byte pieces, RT rows at a time.  A chunk's address is uniform, base
+// positions times `step` behind `src`; a lane's place in the chunk is fixed (a 32-bit byte offset: 64 rows span less than 2^31
+// bytes, checked on the host).  In a reversed pass step < 0 and src is 63 rows below the first position's, so that the lanes'
+// offsets count down and stay positive.  Pieces stay in registers until their tile is free (fetch, then put).
+__device__ __forceinline__ const char* chunk_src(const char* rows, int64_t st, int n, int rev) { return rows + (rev ? (int64_t)(n - kC) * st : 0); }
+template <typename T, int DP, int NTH>
+struct RowsF {
+  static constexpr int VE = 16 / (int)sizeof(T), PER = DP / VE, RT = NTH / PER, NP = kC / RT;
+  const char* src;
+  int64_t step;
+  uint32_t off;        // this lane's piece of row threadIdx / PER
+  int32_t D;
+  bool rev, vec, whole;  // whole: (uniform) 16-byte accesses, no lane outside the row
+  __device__ __forceinline__ void open(const Mat& m, int b, int h, int D_, int n, int rev_) {
+    const int64_t st = m.st * (int)sizeof(T);
+    rev = rev_;
+    src = chunk_src((const char*)row_base<T>(m, b, h), st, n, rev);
+    step = rev ? -st : st;
+    D = D_;
+    vec = m.vec;
+    whole = vec && D == DP;
+    const int r = threadIdx.x / PER, c = (threadIdx.x % PER) * VE;
+    off = (uint32_t)((rev ? kC - 1 - r : r) * (int32_t)st + c * (int)sizeof(T));
+  }
+  // rows [base, base + cnt) (virtual positions); others read as zero
+  __device__ __forceinline__ void fetch(uint4 (&x)[NP], int base, int cnt) const {
+    const char* at = src + base * step;
+    if (cnt == kC && whole) {
 #pragma unroll
-        for (int u = 0; u < VE; ++u)
-          if (c + u < D) e[u] = row[c + u];
+      for (int j = 0; j < NP; ++j, at += RT * step) x[j] = *reinterpret_cast<const uint4*>(at + off);
+      return;
+    }
+    const int r = threadIdx.x / PER, c = (threadIdx.x % PER) * VE;
+#pragma unroll
+    for (int j = 0; j < NP; ++j, at += RT * step) {
+      x[j] = make_uint4(0, 0, 0, 0);
+      if (c < D && r + RT * j < cnt) {
+        if (vec) {
+          x[j] = *reinterpret_cast<const uint4*>(at + off);
+        } else {  // element by element; columns behind the row read its first one and count as zero
+          const T* e = (const T*)(at + off);
+          T y[VE];
+#pragma unroll
+          for (int u = 0; u < VE; ++u) {
+            const T v = e[c + u < D ? u : 0];
+            y[u] = c + u < D ? v : ic_from_f<T>(0.f);
+          }
+          x[j] = *reinterpret_cast<uint4*>(y);
+        }
       }
     }
-#pragma unroll
-    for (int u = 0; u < VE; u += 4)
-      *reinterpret_cast<float4*>(&dst[r][c + u]) = make_float4(ic_to_f(e[u]), ic_to_f(e[u + 1]), ic_to_f(e[u + 2]), ic_to_f(e[u + 3]));
   }
-}
+  static __device__ __forceinline__ void put(float (*dst)[DP + 4], const uint4 (&x)[NP]) {
+    const int r = threadIdx.x / PER, c = (threadIdx.x % PER) * VE;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      T e[VE];
+      *reinterpret_cast<uint4*>(e) = x[j];
+#pragma unroll
+      for (int u = 0; u < VE; u += 4)
+        *reinterpret_cast<float4*>(&dst[r + RT * j][c + u]) = make_float4(ic_to_f(e[u]), ic_to_f(e[u + 1]), ic_to_f(e[u + 2]), ic_to_f(e[u + 3]));
+    }
+  }
+};
+// The value columns of a wave, as operands: element [16 s + q4 + u][col], straight from memory (16 lanes side by side)
+template <typename T>
+struct ColsF {
+  const char* src;
+  int64_t step;
+  uint32_t off;
+  int32_t row0;  // bytes from the chunk's address to virtual row 0
+  int32_t q4;
+  bool in, whole;
+  __device__ __forceinline__ void open(const Mat& m, int b, int h, int D, int n, int rev, int col, int q4_, int DP) {
+    const int64_t st = m.st * (int)sizeof(T);
+    src = chunk_src((const char*)row_base<T>(m, b, h), st, n, rev);
+    step = rev ? -st : st;
+    in = col < D;
+    whole = D == DP;
+    q4 = q4_;
+    row0 = (rev ? kC - 1 : 0) * (int32_t)st + (in ? col : 0) * (int)sizeof(T);
+    off = (uint32_t)(row0 + q4 * (int32_t)step);
+  }
+  __device__ __forceinline__ void fetch(v4f (&x)[4], int base, int cnt) const {
+    const char* at = src + base * step;
+    if (cnt == kC && whole) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[s][u] = ic_to_f(*reinterpret_cast<const T*>(at + (16 * s + u) * step + off));
+      return;
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = 16 * s + q4 + u;
+        const bool ok = in && j < cnt;
+        const float v = ic_to_f(*reinterpret_cast<const T*>(at + row0 + (ok ? j : 0) * step));
+        x[s][u] = ok ? v : 0.f;
+      }
+  }
+};
 
 __device__ __forceinline__ v4f mma(float a, float b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 // sum over 16 k-indices: a, b hold k = 4 (lane / 16) + 0..3
@@ -126,11 +206,13 @@ struct Lds {
   float Ks[kC][DP + 4];  // (padded rows: 16-byte reads of 16 rows and 4-byte reads of 4 rows spread over the banks)
   float Qs[kC][DP + 4];
   float Ps[kC][kC + 4];
+  float dec[2 * kC + 1], dev[2 * kC + 1];  // dec[kC + lag] = e^{-r lag}, 0 for lag < 0; dev = dec * vscale
   double red[DP / 16];
 };
 template <int DP>
 struct LdsSums {
   float Ks[kC][DP + 4];
+  float dec[2 * kC + 1], dev[2 * kC + 1];
 };
 
 // A wave's slice of a state: elements (16 t + q4 + v, col) at a * ia + b * ib of src.  Out of range: zero, read at a clamped
@@ -203,31 +285,38 @@ __device__ __forceinline__ void write_drate(const Geo& g, const Pass* p, double*
 
 template <typename T, int DP, bool LAG, bool SUMS, typename LDS>
 __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Sums* sm, LDS& lds) {
-  constexpr int NT = DP * 4, NW = DP / 16, KS = DP / 16;
+  constexpr int NT = DP * 4, NW = DP / 16, KS = DP / 16, MT = (10 + NW - 1) / NW;
+  using R = RowsF<T, DP, NT>;
   auto& Ks = lds.Ks;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, q4 = (lane >> 4) * 4;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, q4 = (lane >> 4) * 4;
   const int seg = blockIdx.x % g.nseg, bh = blockIdx.x / g.nseg, b = bh / g.H, h = bh - b * g.H;
-  const int n = valid_of(g, b);
+  const int n = valid_of(g, b), T_ = g.T;
   const float l2 = -g.rate[h] * 1.44269504088896340736f;
-  const Mat& mk = SUMS ? sm->k : p->k;
-  const Mat& mv = SUMS ? sm->v : p->v;
   const int Da = SUMS ? sm->Da : p->Da, Db = SUMS ? sm->Db : p->Db;
   const int rev = SUMS ? sm->rev : p->rev;
-  const float vscale = SUMS ? sm->vscale : p->vscale;
-  const T* K = row_base<T>(mk, b, h);
-  const T* V = row_base<T>(mv, b, h);
+  const float vscale = SUMS ? sm->vscale : p->vscale, oscale = SUMS ? 1.f : p->oscale;
   const int col = 16 * w + c;  // this lane's value column
-  const int NC = (g.T + kC - 1) / kC;
+  R rk, rq;
+  ColsF<T> cv;
+  rk.open(SUMS ? sm->k : p->k, b, h, Da, n, rev);
+  cv.open(SUMS ? sm->v : p->v, b, h, Db, n, rev, col, q4, DP);
+  if constexpr (!SUMS) rq.open(p->q, b, h, Da, n, rev);
+  for (int i = threadIdx.x; i < 2 * kC + 1; i += NT) {
+    const float d = i < kC ? 0.f : decay(l2, i - kC);
+    lds.dec[i] = d;
+    lds.dev[i] = d * vscale;
+  }
+  const int NC = (T_ + kC - 1) / kC;
   const int ch0 = seg * g.cps, ch1 = ch0 + g.cps < NC ? ch0 + g.cps : NC;
+  const size_t dd = (size_t)Da * Db;
 
   v4f S[KS], L[LAG ? KS : 1];
 #pragma unroll
   for (int t = 0; t < KS; ++t) {
     S[t] = v4f{0.f, 0.f, 0.f, 0.f};
-    if (LAG) L[t] = S[t];
+    if constexpr (LAG) L[t] = S[t];
   }
-  const size_t dd = (size_t)Da * Db;
-  if (!SUMS) {
+  if constexpr (!SUMS) {
     const float* s0 = p->seg ? p->seg + ((size_t)bh * g.nseg + seg) * p->nst * dd : p->init ? p->init + (size_t)bh * dd : nullptr;
     const int ia = p->seg ? p->sga : p->ia, ib = p->seg ? p->sgb : p->ib;
     if (s0) {
@@ -238,144 +327,160 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
     }
   }
   double dr = 0.0;
+  uint4 fk[R::NP], fq[SUMS ? 1 : R::NP];
+  v4f vf[4];
+  auto fetch = [&](int base) {
+    const int cnt = n - base < kC ? n - base : kC;
+    rk.fetch(fk, base, cnt);
+    if constexpr (!SUMS) rq.fetch(fq, base, cnt);
+    cv.fetch(vf, base, cnt);
+  };
+  if (ch0 * kC < n) fetch(ch0 * kC);
   for (int ch = ch0; ch < ch1; ++ch) {
     const int base = ch * kC;
     const int cnt = n - base < 0 ? 0 : n - base < kC ? n - base : kC;
     if (SUMS && cnt == 0) break;
-    // the gradient of the final state enters the reversed recurrence without a step of decay in front of it
-    const int off = rev && ch == 0 ? 1 : 0;
+    const int off = rev && ch == 0 ? 1 : 0;  // (the gradient of the final state enters without a step of decay)
+    v4f O[4], vw[4];
+    float drc = 0.f;
     if (cnt > 0) {
-      stage<T, DP, NT>(Ks, K, mk, Da, base, cnt, n, rev);
-      if constexpr (!SUMS) stage<T, DP, NT>(lds.Qs, row_base<T>(p->q, b, h), p->q, Da, base, cnt, n, rev);
-    }
-    v4f vf[4];  // V[16 s + q4 + u][col]
+      R::put(Ks, fk);
+      if constexpr (!SUMS) R::put(lds.Qs, fq);
+      v4f v0[4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+      for (int s = 0; s < 4; ++s) v0[s] = vf[s];
+      __syncthreads();
+      if (ch + 1 < ch1 && base + kC < n) fetch(base + kC);
+      const float* dl = &lds.dev[kC + cnt - 1 - q4 - 51];  // (51: the largest position of this lane's values)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int j = 16 * s + q4 + u;
-        vf[s][u] = j < cnt && col < Db ? ic_to_f(V[(int64_t)(rev ? n - 1 - (base + j) : base + j) * mv.st + col]) : 0.f;
-      }
-    __syncthreads();
-    if constexpr (!SUMS) {
-      auto& Ps = lds.Ps;
-      auto& Qs = lds.Qs;
-      v4f O[4], E[LAG ? 4 : 1];
+      for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        O[it] = v4f{0.f, 0.f, 0.f, 0.f};
-        if (LAG) E[it] = O[it];
-      }
-      if (cnt > 0) {
+        for (int u = 0; u < 4; ++u) vw[s][u] = v0[s][u] * dl[51 - 16 * s - u];
+      if constexpr (!SUMS) {
+        auto& Ps = lds.Ps;
+        auto& Qs = lds.Qs;
+        v4f E[LAG ? 4 : 1];
         // P[i][j] = e^{-r(i-j)} q_i . k_j for the ten 16x16 tiles with a j <= i, formed transposed (rows j)
-        for (int t = w; t < 10; t += NW) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int t = w + i * NW;
+          if (t >= 10) break;
           const int it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2;
           v4f acc = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int s = 0; s < KS; ++s) acc = mma16(ld4(&Ks[16 * jt + c][16 * s + q4]), ld4(&Qs[16 * it + c][16 * s + q4]), acc);
+          const int lag0 = 16 * (it - jt) + c - q4;
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            const int lag = 16 * (it - jt) + c - q4 - v;
-            acc[v] = lag >= 0 ? acc[v] * decay(l2, lag) * vscale : 0.f;
+            const float d = lds.dev[kC + lag0 - v];
+            acc[v] = lag0 >= v ? acc[v] * (d * oscale) : 0.f;  // (a select: what lies above the diagonal may be infinite)
           }
           *reinterpret_cast<v4f*>(&Ps[16 * it + c][16 * jt + q4]) = acc;
         }
         // what the state at the chunk's border adds
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
+          O[it] = v4f{0.f, 0.f, 0.f, 0.f};
+          if constexpr (LAG) E[it] = O[it];
+        }
 #pragma unroll
-          for (int s = 0; s < KS; ++s) {
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
             const v4f bq = ld4(&Qs[16 * it + c][16 * s + q4]);
             O[it] = mma16(S[s], bq, O[it]);
-            if (LAG) E[it] = mma16(L[s], bq, E[it]);
+            if constexpr (LAG) E[it] = mma16(L[s], bq, E[it]);
           }
-          const int ex = 16 * it + c + 1 - off;
-          const float f = decay(l2, ex);
-          if (LAG) E[it] = f * (E[it] + (float)ex * O[it]);
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const float f = lds.dec[kC + 16 * it + c + 1 - off] * oscale;
           O[it] = f * O[it];
+          if constexpr (LAG) E[it] = f * E[it] + (float)(16 * it + c + 1) * O[it];
         }
-      }
-      __syncthreads();
-      float drc = 0.f;
-      if (cnt > 0) {
+        __syncthreads();
 #pragma unroll
         for (int it = 0; it < 4; ++it)
 #pragma unroll
           for (int s = 0; s <= it; ++s) {
             v4f bp = ld4(&Ps[16 * it + c][16 * s + q4]);
-            O[it] = mma16(vf[s], bp, O[it]);
-            if (LAG) {
+            O[it] = mma16(v0[s], bp, O[it]);
+            if constexpr (LAG) {
 #pragma unroll
               for (int u = 0; u < 4; ++u) bp[u] *= (float)(16 * (it - s) + c - q4 - u);  // (0 above the diagonal stays 0)
-              E[it] = mma16(vf[s], bp, E[it]);
+              E[it] = mma16(v0[s], bp, E[it]);
             }
           }
+        if constexpr (LAG) {
+          const int64_t xst = (rev ? -1 : 1) * p->x.st;
+          const T* x0 = row_base<T>(p->x, b, h) + (int64_t)(rev ? n - 1 : 0) * p->x.st;
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            const int i = 16 * it + c;
+            const T* x = x0 + (base + (i < cnt ? i : 0)) * xst;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const float xv = ic_to_f(x[16 * w + q4 + v < Db ? 16 * w + q4 + v : 0]);
+              drc = i < cnt && 16 * w + q4 + v < Db ? fmaf(E[it][v], xv, drc) : drc;
+            }
+          }
+          dr -= (double)drc;
+        }
       }
+    }
+    if constexpr (!SUMS) {
+      const int b0 = 16 * w + q4;  // this lane's four columns of a row
+      const int64_t ob = (int64_t)b * p->out.sb + (int64_t)h * p->out.sh;
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
         const int i = base + 16 * it + c;
-        if (i >= g.T) continue;
+        if (i >= T_ || b0 >= Db) continue;
         const bool live = i < n;
-        const int64_t t = rev && live ? n - 1 - i : i;
-        const int b0 = 16 * w + q4;  // this lane's four columns of row i
-        if (LAG && live) {
-          const T* x = row_base<T>(p->x, b, h) + t * p->x.st;
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            if (b0 + v < Db) drc = fmaf(E[it][v], ic_to_f(x[b0 + v]), drc);
-        }
-        float o[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) o[v] = live ? O[it][v] * p->oscale : 0.f;
-        if (p->out32) {
-          float* row = (float*)p->out.p + (int64_t)b * p->out.sb + (int64_t)h * p->out.sh + t * p->out.st;
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            if (b0 + v < Db) row[b0 + v] = o[v];
-        } else {
-          T* row = (T*)p->out.p + (int64_t)b * p->out.sb + (int64_t)h * p->out.sh + t * p->out.st;
-          if (p->out.vec) {
-            if (b0 < Db) {
-              T e[4] = {ic_from_f<T>(o[0]), ic_from_f<T>(o[1]), ic_from_f<T>(o[2]), ic_from_f<T>(o[3])};
-              if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(row + b0) = *reinterpret_cast<uint4*>(e);
-              else *reinterpret_cast<uint2*>(row + b0) = *reinterpret_cast<uint2*>(e);
-            }
+        const int64_t at = ob + (rev && live ? n - 1 - i : i) * p->out.st + b0;
+        const v4f o = live ? O[it] : v4f{0.f, 0.f, 0.f, 0.f};
+        if (p->out.vec) {
+          if (sizeof(T) == 4 || p->out32) {
+            *reinterpret_cast<v4f*>((float*)p->out.p + at) = o;
           } else {
+            union { T e[4]; uint2 u; } x;
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (b0 + v < Db) row[b0 + v] = ic_from_f<T>(o[v]);
+            for (int v = 0; v < 4; ++v) x.e[v] = ic_from_f<T>(o[v]);
+            *reinterpret_cast<uint2*>((T*)p->out.p + at) = x.u;
           }
+        } else {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (b0 + v < Db) {
+              if (p->out32) ((float*)p->out.p)[at + v] = o[v];
+              else ((T*)p->out.p)[at + v] = ic_from_f<T>(o[v]);
+            }
         }
       }
-      if (LAG) dr -= (double)drc * (double)p->oscale;
     }
     if (cnt > 0) {  // the state behind the chunk
-      const float carry = decay(l2, cnt - off);
+      const float carry = lds.dec[kC + cnt - off];
 #pragma unroll
       for (int t = 0; t < KS; ++t) {
-        if (LAG) L[t] = carry * (L[t] + (float)cnt * S[t]);
+        if constexpr (LAG) L[t] = carry * (L[t] + (float)cnt * S[t]);
         S[t] = carry * S[t];
       }
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         v4f vl;
+        if constexpr (LAG) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int left = cnt - 1 - (16 * s + q4 + u);
-          vf[s][u] = left >= 0 ? vf[s][u] * (decay(l2, left) * vscale) : 0.f;
-          vl[u] = vf[s][u] * (float)left;  // (0 where left < 0)
+          for (int u = 0; u < 4; ++u) vl[u] = vw[s][u] * (float)(cnt - 1 - q4 - 16 * s - u);  // (0 behind the last valid position)
         }
 #pragma unroll
         for (int t = 0; t < KS; ++t) {
           v4f ak;
 #pragma unroll
           for (int u = 0; u < 4; ++u) ak[u] = Ks[16 * s + q4 + u][16 * t + c];
-          S[t] = mma16(ak, vf[s], S[t]);
-          if (LAG) L[t] = mma16(ak, vl, L[t]);
+          S[t] = mma16(ak, vw[s], S[t]);
+          if constexpr (LAG) L[t] = mma16(ak, vl, L[t]);
         }
       }
+      __syncthreads();
     }
-    __syncthreads();
   }
   if constexpr (SUMS) {
     write_sums<LAG>(g, sm, S, L, dd, Da, Db, col, q4, bh, seg);
@@ -467,11 +572,7 @@ __device__ __forceinline__ void store4(char* row, const v4f& o, bool f32) {
   else *reinterpret_cast<uint2*>(row) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
 }
 
-// Rows of one matrix as a workgroup of 4 DP threads reads them: 16-byte pieces, 32 rows at a time.  A chunk's address is
-// uniform, base positions times `step` behind `src`; a lane's place in the chunk is fixed (a 32-bit byte offset: 64 rows span
-// less than 2^31 bytes, checked on the host).  In a reversed pass step < 0 and src is 63 rows below the first position's, so
-// that the lanes' offsets count down and stay positive.
-__device__ __forceinline__ const char* chunk_src(const char* rows, int64_t st, int n, int rev) { return rows + (rev ? (int64_t)(n - kC) * st : 0); }
+// RowsF for bf16 tiles that stay bf16 (16-byte accesses only)
 template <int DP, int CW>
 struct Rows {
   static constexpr int RT = 32 / CW, NP = 2 * CW;  // rows at a time, times
