@@ -221,20 +221,38 @@ template <int NT>
 __device__ __forceinline__ void load_state(v4f (&S)[NT], const float* src, int ia, int ib, int Da, int Db, int col, int q4) {
   const bool in = col < Db;
   const float* at = src + (size_t)(in ? col : 0) * ib;
+  if (Da == 16 * NT) {  // (uniform: no row left out)
+    at += (size_t)q4 * ia;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float x = at[(size_t)(16 * t + v) * ia];
+        S[t][v] = in ? x : 0.f;
+      }
+    return;
+  }
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const int a = 16 * t + q4 + v;
-      const bool ok = in && a < Da;
-      const float x = at[(size_t)(ok ? a : 0) * ia];
-      S[t][v] = ok ? x : 0.f;
+      const float x = at[(size_t)(a < Da ? a : 0) * ia];
+      S[t][v] = in && a < Da ? x : 0.f;
     }
 }
 template <int NT>
 __device__ __forceinline__ void store_state(const v4f (&S)[NT], float* dst, int ia, int ib, int Da, int Db, int col, int q4, float f) {
   if (col >= Db) return;
   float* at = dst + (size_t)col * ib;
+  if (Da == 16 * NT) {
+    at += (size_t)q4 * ia;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) at[(size_t)(16 * t + v) * ia] = S[t][v] * f;
+    return;
+  }
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -870,6 +888,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
 template <int DP, bool LAG, bool W16>
 constexpr int cw_of() { return W16 && DP == 128 && !LAG ? 2 : 1; }
 
+// LAG: the pass that carries the lag-weighted state, a launch of its own (its registers and LDS would bound the others).
 template <typename T, int DP, bool LAG, bool W16>
 __global__ __launch_bounds__((DP * 4 / cw_of<DP, LAG, W16>()), 2) void k_lattn(PassArgs a) {
   if constexpr (W16) {
@@ -884,10 +903,12 @@ template <typename T, int DP, bool LAG, bool W16>
 __global__ __launch_bounds__(DP * 4) void k_lattn_sums(SumArgs a) {
   if constexpr (W16) {
     __shared__ __align__(16) LdsSums16<DP> lds;
-    lattn_body16<DP, 1, LAG, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
+    if (LAG && blockIdx.y == 0) lattn_body16<DP, 1, LAG, true>(a.g, nullptr, &a.s[0], lds);
+    else lattn_body16<DP, 1, false, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
   } else {
     __shared__ __align__(16) LdsSums<DP> lds;
-    lattn_body<T, DP, LAG, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
+    if (LAG && blockIdx.y == 0) lattn_body<T, DP, LAG, true>(a.g, nullptr, &a.s[0], lds);
+    else lattn_body<T, DP, false, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
   }
 }
 
@@ -1088,6 +1109,7 @@ Geo geo_of(const ic_lattn_args* a, int passes, int slots) {
   }
   return g;
 }
+// (bf16 rows that take the fp32 kernels for want of 16-byte accesses are planned like the others)
 int slots_of(const ic_lattn_args* a, bool lag) {
   const int dp = pad_of(a);
   return 256 * (dp == 32 ? 4 : dp == 64 ? 2 : a->dtype == IC_DT_BF16 && !lag ? 2 : 1);
@@ -1226,14 +1248,8 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
     s.s[0] = Sums{v, k, Dv, Dk, 0, lag, 1.f, seg_s};
     s.s[1] = Sums{q, o, Dk, Dv, 1, 0, a->scale, seg_r};
 #define IC_BODY(T, DP)                                                                                                                        \
-  if (lag) {                                                                                                                                   \
-    IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, true, W16>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, s));         \
-    SumArgs s1 = s;                                                                                                                            \
-    s1.s[0] = s.s[1];                                                                                                                          \
-    IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, s1));       \
-  } else {                                                                                                                                     \
-    IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, s));        \
-  }
+  if (lag) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, true, W16>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, s)); \
+  else IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, s))
     IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
     IC_LAUNCH_CHECK("ic_lattn_bwd");
@@ -1279,18 +1295,22 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
     pv.seg = seg_r; pv.sga = Dv; pv.sgb = 1; pv.nst = 1;
     pk.seg = seg_r; pk.sga = 1; pk.sgb = Dv; pk.nst = 1;
   }
-#define IC_BODY(T, DP)                                                                                                              \
-  if (lag) {                                                                                                                       \
-    IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, true, W16>), dim3(bh * g.nseg, 1), dim3(DP * 4 / cw_of<DP, true, W16>()), 0, st, p));   \
-    PassArgs p1 = p;                                                                                                               \
-    p1.p[0] = p.p[1];                                                                                                              \
-    p1.p[1] = p.p[2];                                                                                                              \
-    IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false, W16>), dim3(bh * g.nseg, 2), dim3(DP * 4 / cw_of<DP, false, W16>()), 0, st, p1)); \
-  } else {                                                                                                                         \
-    IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false, W16>), dim3(bh * g.nseg, 3), dim3(DP * 4 / cw_of<DP, false, W16>()), 0, st, p));  \
+#define IC_LATTN_BWD(T, DP, LAG, PASSES, ARGS)                                                                                  \
+  IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, LAG, W16>), dim3(bh * g.nseg, PASSES),                      \
+                                                    dim3(DP * 4 / cw_of<DP, LAG, W16>()), 0, st, ARGS))
+#define IC_BODY(T, DP)                          \
+  if (!lag) {                                   \
+    IC_LATTN_BWD(T, DP, false, 3, p);           \
+  } else {                                      \
+    IC_LATTN_BWD(T, DP, true, 1, p);            \
+    PassArgs p1 = p;                            \
+    p1.p[0] = p.p[1];                           \
+    p1.p[1] = p.p[2];                           \
+    IC_LATTN_BWD(T, DP, false, 2, p1);          \
   }
   IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
+#undef IC_LATTN_BWD
   IC_LAUNCH_CHECK("ic_lattn_bwd");
   if (G > 1) {
     JoinArgs j{};
