@@ -920,7 +920,18 @@ DTYPES = {torch.float32: ENUMS["IC_DT_F32"], torch.bfloat16: ENUMS["IC_DT_BF16"]
 ROPE_LAYOUTS = {"interleaved": ENUMS["IC_ROPE_INTERLEAVED"], "half": ENUMS["IC_ROPE_HALF"]}
 ROPE_MAX_D = 512
 ROPE_PARTS = 1024  # workgroups (partial sums of the norm weights' gradients) of ic_rope_bwd: ic_rope_parts()
-_pack_rope, _pack_rope_bwd = packer("ic_rope_args"), packer("ic_rope_bwd_args")
+_pack_rope, _pack_rope_bwd = packer("ic_rope_args")[0], packer("ic_rope_bwd_args")[0]
+
+
+def _once(fn):
+    """staticmethod of a backward that cannot be differentiated itself: a second derivative raises, as with
+    once_differentiable, whose wrapper costs 6 us a call and is only needed where the backward is being recorded."""
+    recorded = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+
+    return staticmethod(backward)
 
 
 def _launch(name: str, blob: bytes, device: torch.device) -> None:
@@ -969,8 +980,8 @@ def _wants_grad(*ts) -> bool:
 
 
 def _angles(who, q, cos, sin, positions, freqs, layout, scale):
-    """Checked angles of a rotation -- tables cos / sin, or positions and frequencies -- as the fields of ic_rope_args, and
-    the tensors that hold them."""
+    """Checked angles of a rotation -- tables cos / sin, or positions and frequencies -- as fields of ic_rope_args: (m, layout,
+    pos64, freq64, scale), (cos, sin, cs_sb, positions, pos_sb, freqs); and the tensors that hold them."""
     B, _, T, D = q.shape
     if layout not in ROPE_LAYOUTS:
         raise ValueError(f"{who}: layout {layout!r} (one of {sorted(ROPE_LAYOUTS)})")
@@ -979,7 +990,7 @@ def _angles(who, q, cos, sin, positions, freqs, layout, scale):
     if cos is not None and positions is not None:
         raise ValueError(f"{who}: positions go with freqs, not with cos / sin")
     _same_device(who, q, cos=cos, sin=sin, positions=positions, freqs=freqs)
-    f = dict(layout=ROPE_LAYOUTS[layout], scale=float(scale))
+    lay, pos64, freq64 = ROPE_LAYOUTS[layout], 0, 0
     if cos is not None:
         for n, t in (("cos", cos), ("sin", sin)):
             if t.dtype != torch.float32 or t.shape != cos.shape or t.dim() not in (2, 3) or t.shape[-2] != T or (t.dim() == 3 and t.shape[0] not in (1, B)):
@@ -988,7 +999,7 @@ def _angles(who, q, cos, sin, positions, freqs, layout, scale):
             raise RuntimeError(f"{who}: no gradient reaches the angles (cos, sin): detach them")
         m = cos.shape[-1]
         cos, sin = cos.contiguous(), sin.contiguous()
-        f.update(m=m, cos=cos.data_ptr(), sin=sin.data_ptr(), cs_sb=T * m if cos.dim() == 3 and cos.shape[0] == B and B > 1 else 0)
+        src = (cos.data_ptr(), sin.data_ptr(), T * m if cos.dim() == 3 and cos.shape[0] == B and B > 1 else 0, 0, 0, 0)
         hold = (cos, sin)
     else:
         if freqs.dim() != 1 or freqs.dtype not in (torch.float32, torch.float64):
@@ -997,41 +1008,44 @@ def _angles(who, q, cos, sin, positions, freqs, layout, scale):
             raise RuntimeError(f"{who}: no gradient reaches the angles (freqs): detach them")
         m = freqs.shape[0]
         freqs = freqs.contiguous()
-        f.update(m=m, freqs=freqs.data_ptr(), freq64=int(freqs.dtype == torch.float64))
-        hold = (freqs,)
+        freq64 = int(freqs.dtype == torch.float64)
+        hold, src = (freqs,), (0, 0, 0, 0, 0, freqs.data_ptr())
         if positions is not None:
             if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((T,), (1, T), (B, T)):
                 raise ValueError(f"{who}: positions is {positions.dtype} {tuple(positions.shape)}, needs int32 or int64 [T], [1,T] or [B,T] with B={B}, T={T}")
             positions = positions.contiguous()
-            f.update(positions=positions.data_ptr(), pos64=int(positions.dtype == torch.int64),
-                     pos_sb=T if positions.dim() == 2 and positions.shape[0] == B and B > 1 else 0)
+            pos64 = int(positions.dtype == torch.int64)
             hold = (freqs, positions)
+            src = (0, 0, 0, positions.data_ptr(), T if positions.dim() == 2 and positions.shape[0] == B and B > 1 else 0, freqs.data_ptr())
     if 2 * m > D:
         raise ValueError(f"{who}: {m} rotated pairs do not fit rows of {D} channels")
-    return f, hold
+    return ((m, lay, pos64, freq64, float(scale)), src), hold
 
 
-def _rope_fields(ang, q, k, yq=None, yk=None, wq=None, wk=None, eps: float = 0.0, inverse: int = 0, pre: str = "") -> dict:
-    """Fields of ic_rope_args (`pre`: as a member of another struct)."""
-    B, H, T, D = q.shape
-    f = dict(ang, B=B, T=T, D=D, dtype=DTYPES[q.dtype], inverse=inverse, eps=eps)
-    for n, x, y, w in (("q", q, yq, wq), ("k", k, yk, wk)):
-        if x is None:
-            continue
-        f[n + "_H"], f[n + "_x"] = x.shape[1], x.data_ptr()
-        f[n + "_x_sb"], f[n + "_x_sh"], f[n + "_x_st"], _ = x.stride()
-        if y is not None:
-            f[n + "_y"] = y.data_ptr()
-            f[n + "_y_sb"], f[n + "_y_sh"], f[n + "_y_st"], _ = y.stride()
-        if w is not None:
-            f[n + "_w"], f[n + "_w_dtype"] = w.data_ptr(), DTYPES[w.dtype]
-    return {pre + n: v for n, v in f.items()} if pre else f
+_NO_ROWS = (0,) * 11
+
+
+def _rope_rows(x, y, w) -> tuple:
+    """ic_rope_rows"""
+    if x is None:
+        return _NO_ROWS
+    xb, xh, xt, _ = x.stride()
+    yb, yh, yt, _ = (0, 0, 0, 0) if y is None else y.stride()
+    return (x.data_ptr(), 0 if y is None else y.data_ptr(), 0 if w is None else w.data_ptr(), xb, xh, xt, yb, yh, yt, x.shape[1],
+            0 if w is None else DTYPES[w.dtype])
+
+
+def _rope_values(ang, q, k, yq=None, yk=None, wq=None, wk=None, eps: float = 0.0, inverse: int = 0) -> tuple:
+    """ic_rope_args"""
+    (m, layout, pos64, freq64, scale), src = ang
+    B, _, T, D = q.shape
+    return (B, T, D, m, DTYPES[q.dtype], layout, inverse, pos64, freq64, scale, eps, *src, *_rope_rows(q, yq, wq), *_rope_rows(k, yk, wk))
 
 
 def _rope_run(ang, q, k, wq=None, wk=None, eps: float = 0.0):
-    yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    yk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    _launch("ic_rope_fwd", _pack_rope(**_rope_fields(ang, q, k, yq, yk, wq, wk, eps)), q.device)
+    yq = q.new_empty(q.shape)
+    yk = None if k is None else k.new_empty(k.shape)
+    _launch("ic_rope_fwd", _pack_rope(*_rope_values(ang, q, k, yq, yk, wq, wk, eps)), q.device)
     return yq, yk
 
 
@@ -1045,14 +1059,13 @@ class RopeFn(torch.autograd.Function):
         ctx.order = [_dense_order(t) for t in (q, k) if t is not None]
         return _rope_run(ang, q, k)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, gq, gk):
         hold = ctx.saved_tensors
         gq, gk = _rows4(gq), _rows4(gk) if len(ctx.order) > 1 else None
-        oq = torch.empty_strided(gq.shape, ctx.order[0], dtype=gq.dtype, device=gq.device)
-        ok = None if gk is None else torch.empty_strided(gk.shape, ctx.order[1], dtype=gk.dtype, device=gk.device)
-        _launch("ic_rope_fwd", _pack_rope(**_rope_fields(ctx.ang, gq, gk, oq, ok, inverse=1)), gq.device)
+        oq = gq.new_empty_strided(gq.shape, ctx.order[0])
+        ok = None if gk is None else gk.new_empty_strided(gk.shape, ctx.order[1])
+        _launch("ic_rope_fwd", _pack_rope(*_rope_values(ctx.ang, gq, gk, oq, ok, inverse=1)), gq.device)
         return (oq, ok, None) + (None,) * len(hold)
 
 
@@ -1066,26 +1079,18 @@ class QKNormRopeFn(torch.autograd.Function):
         ctx.ang, ctx.eps = ang, eps
         return _rope_run(ang, q, k, wq, wk, eps)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, gq, gk):
         q, k, wq, wk, *hold = ctx.saved_tensors
-        dev = q.device
-        f = _rope_fields(ctx.ang, q, k, None, None, wq, wk, ctx.eps, pre="f_")
-        part = torch.empty(ROPE_PARTS * q.shape[3], device=dev)
-        f["part"] = part.data_ptr()
-        gws, outs, keep = [], [], []
-        for n, x, w, g in (("q", q, wq, gq), ("k", k, wk, gk)):
-            g = _rows4(g)
-            gx = torch.empty_strided(x.shape, _dense_order(x), dtype=x.dtype, device=dev)
-            gw = torch.empty_like(w)
-            f[n + "_g"], f[n + "_gx"], f[n + "_gw"] = g.data_ptr(), gx.data_ptr(), gw.data_ptr()
-            f[n + "_g_sb"], f[n + "_g_sh"], f[n + "_g_st"], _ = g.stride()
-            f[n + "_gx_sb"], f[n + "_gx_sh"], f[n + "_gx_st"], _ = gx.stride()
-            keep.append(g)
+        part = torch.empty(ROPE_PARTS * q.shape[3], device=q.device)
+        vals, outs, gws, keep = [], [], [], []
+        for x, w, g in ((q, wq, gq), (k, wk, gk)):  # ic_rope_grad
+            g, gx, gw = _rows4(g), x.new_empty_strided(x.shape, _dense_order(x)), torch.empty_like(w)
+            vals += (g.data_ptr(), gx.data_ptr(), gw.data_ptr(), *g.stride()[:3], *gx.stride()[:3])
             outs.append(gx)
             gws.append(gw)
-        _launch("ic_rope_bwd", _pack_rope_bwd(**f), dev)
+            keep.append(g)
+        _launch("ic_rope_bwd", _pack_rope_bwd(*_rope_values(ctx.ang, q, k, None, None, wq, wk, ctx.eps), *vals, part.data_ptr()), q.device)
         return (*outs, *gws, None, None) + (None,) * len(hold)
 
 
@@ -1138,48 +1143,42 @@ def qk_norm_rope(q, k, q_weight, k_weight, *, eps: float = 1e-5, cos=None, sin=N
 # ---------------------------------------------------------------- linear attention with a decay for each head
 LATTN_MAX_D = 128        # channels of a head's keys and values
 LATTN_STEP_MAX_D = 1024  # the same for single positions
-_pack_lattn, _pack_lattn_bwd, _pack_lattn_step = packer("ic_lattn_args"), packer("ic_lattn_bwd_args"), packer("ic_lattn_step_args")
+_pack_lattn, _pack_lattn_bwd, _pack_lattn_step = packer("ic_lattn_args")[0], packer("ic_lattn_bwd_args")[0], packer("ic_lattn_step_args")[0]
 
 
-def _lattn_fields(q, k, v, rate, valid_len, state, scale) -> dict:
+def _lattn_values(q, k, v, rate, valid_len, state, scale, out=None, state_out=None, ws=None) -> tuple:
+    """ic_lattn_args"""
     B, H, T, Dk = q.shape
-    f = dict(B=B, H=H, Hk=k.shape[1], T=T, Dk=Dk, Dv=v.shape[3], dtype=DTYPES[q.dtype], scale=scale, q=q.data_ptr(), k=k.data_ptr(),
-             v=v.data_ptr(), rate=rate.data_ptr(), valid_len=_addr(valid_len), state=_addr(state))
-    f["q_sb"], f["q_sh"], f["q_st"], _ = q.stride()
-    f["k_sb"], f["k_sh"], f["k_st"], _ = k.stride()
-    f["v_sb"], f["v_sh"], f["v_st"], _ = v.stride()
-    return f
+    ob, oh, ot, _ = (0, 0, 0, 0) if out is None else out.stride()
+    return (B, H, k.shape[1], T, Dk, v.shape[3], DTYPES[q.dtype], scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3],
+            *k.stride()[:3], *v.stride()[:3], rate.data_ptr(), _addr(valid_len), _addr(state), _addr(out), ob, oh, ot, _addr(state_out), _addr(ws))
 
 
 _LATTN_WS: Dict[tuple, int] = {}  # workspace floats by sizes (a pure function of them)
 
 
-def _lattn_ws(f: dict, backward: int, device) -> Optional[torch.Tensor]:
+def _lattn_ws(q, k, v, backward: int) -> Optional[torch.Tensor]:
     """Workspace of a call (held by the caller until its launches are queued; the allocator orders reuse on the stream)."""
-    key = (f["B"], f["H"], f["Hk"], f["T"], f["Dk"], f["Dv"], f["dtype"], backward)
+    key = (q.shape, k.shape[1], v.shape[3], q.dtype, backward)
     n = _LATTN_WS.get(key)
     if n is None:
+        B, H, T, Dk = q.shape
         got = ctypes.c_int64(0)
-        check(lib().ic_lattn_ws(_pack_lattn(**f), backward, ctypes.byref(got)), "ic_lattn_ws")
+        a = new("ic_lattn_args", B=B, H=H, Hk=k.shape[1], T=T, Dk=Dk, Dv=v.shape[3], dtype=DTYPES[q.dtype])
+        check(lib().ic_lattn_ws(ctypes.byref(a), backward, ctypes.byref(got)), "ic_lattn_ws")
         if len(_LATTN_WS) > 4096:
             _LATTN_WS.clear()
         n = _LATTN_WS[key] = got.value
-    if n == 0:
-        return None
-    ws = torch.empty(n, dtype=torch.float32, device=device)
-    f["ws"] = ws.data_ptr()
-    return ws
+    return torch.empty(n, dtype=torch.float32, device=q.device) if n else None
 
 
 def _lattn_run(q, k, v, rate, state, valid_len, scale):
     B, H, T, Dk = q.shape
-    Dv, dev = v.shape[3], q.device
-    out = torch.empty((B, T, H, Dv), dtype=q.dtype, device=dev).transpose(1, 2)
-    state_out = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=dev)
-    f = _lattn_fields(q, k, v, rate, valid_len, state, scale)
-    ws = _lattn_ws(f, 0, dev)  # noqa: F841
-    sb, sh, st, _ = out.stride()
-    _launch("ic_lattn_fwd", _pack_lattn(**f, out=out.data_ptr(), o_sb=sb, o_sh=sh, o_st=st, state_out=state_out.data_ptr()), dev)
+    Dv = v.shape[3]
+    out = q.new_empty((B, T, H, Dv)).transpose(1, 2)
+    state_out = rate.new_empty((B, H, Dk, Dv))
+    ws = _lattn_ws(q, k, v, 0)
+    _launch("ic_lattn_fwd", _pack_lattn(*_lattn_values(q, k, v, rate, valid_len, state, scale, out, state_out, ws)), q.device)
     return out, state_out
 
 
@@ -1193,31 +1192,22 @@ class LinearAttnFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return _lattn_run(q, k, v, rate, state, valid_len, scale)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, gout, gstate):
         q, k, v, rate, state, valid_len = ctx.saved_tensors
         if gout is None and gstate is None:
             return (None,) * 7
         B, H, T, Dk = q.shape
-        dev = q.device
-        gout = torch.zeros((B, H, T, v.shape[3]), dtype=q.dtype, device=dev) if gout is None else _rows4(gout)
+        gout = torch.zeros((B, H, T, v.shape[3]), dtype=q.dtype, device=q.device) if gout is None else _rows4(gout)
         gstate = None if gstate is None else gstate.contiguous()
         drate = torch.empty_like(rate) if ctx.needs_input_grad[3] else None
         dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
-        f = _lattn_fields(q, k, v, rate, valid_len, state, ctx.scale)
-        ws = _lattn_ws(f, 1, dev)  # noqa: F841
-        f = {"f_" + n: x for n, x in f.items()}
-        f.update(dout=gout.data_ptr(), dstate_out=_addr(gstate), drate=_addr(drate), dstate=_addr(dstate))
-        f["do_sb"], f["do_sh"], f["do_st"], _ = gout.stride()
-        outs = []
-        for n, t in (("dq", q), ("dk", k), ("dv", v)):
-            g = torch.empty_strided(t.shape, _dense_order(t), dtype=t.dtype, device=dev)
-            f[n] = g.data_ptr()
-            f[n + "_sb"], f[n + "_sh"], f[n + "_st"], _ = g.stride()
-            outs.append(g)
-        _launch("ic_lattn_bwd", _pack_lattn_bwd(**f), dev)
-        return (*outs, drate, dstate, None, None)
+        ws = _lattn_ws(q, k, v, 1)
+        dq, dk, dv = (t.new_empty_strided(t.shape, _dense_order(t)) for t in (q, k, v))
+        _launch("ic_lattn_bwd", _pack_lattn_bwd(
+            *_lattn_values(q, k, v, rate, valid_len, state, ctx.scale, ws=ws), gout.data_ptr(), *gout.stride()[:3], _addr(gstate),
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], _addr(drate), _addr(dstate)), q.device)
+        return dq, dk, dv, drate, dstate, None, None
 
 
 def _check_linear(who, q, k, v, rate, state, dims: int, most: int):
@@ -1281,21 +1271,20 @@ def linear_attention_step(q, k, v, rate, state, *, scale: float = 1.0, active=No
     if not state.is_contiguous():
         raise ValueError("linear_attention_step: the state is updated in place and has to be dense")
     B, H, Dk = q.shape
-    Dv, dev = v.shape[2], q.device
+    Dv = v.shape[2]
     if active is not None:
         _same_device("linear_attention_step", q, active=active)
         if active.shape != (B,) or active.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"linear_attention_step: active is {active.dtype} {tuple(active.shape)}, needs bool or uint8 [{B}]")
         active = active.contiguous()
-    out = torch.empty((B, H, Dv), dtype=q.dtype, device=dev)
+    out = q.new_empty((B, H, Dv))
     if B * H == 0:
         return out
     q, k, v, rate = _rows4(q), _rows4(k), _rows4(v), rate.contiguous()
     (q_sb, q_sh, _), (k_sb, k_sh, _), (v_sb, v_sh, _) = q.stride(), k.stride(), v.stride()
     _launch("ic_lattn_step", _pack_lattn_step(
-        B=B, H=H, Hk=k.shape[1], Dk=Dk, Dv=Dv, dtype=DTYPES[q.dtype], scale=scale, q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(),
-        q_sb=q_sb, q_sh=q_sh, k_sb=k_sb, k_sh=k_sh, v_sb=v_sb, v_sh=v_sh, rate=rate.data_ptr(), active=_addr(active),
-        state=state.data_ptr(), out=out.data_ptr(), o_sb=H * Dv, o_sh=Dv), dev)
+        B, H, k.shape[1], Dk, Dv, DTYPES[q.dtype], scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_sb, q_sh, k_sb, k_sh, v_sb, v_sh,
+        rate.data_ptr(), _addr(active), state.data_ptr(), out.data_ptr(), H * Dv, Dv), q.device)
     torch.autograd.graph.increment_version(state)
     return out
 
