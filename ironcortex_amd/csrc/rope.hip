@@ -62,7 +62,7 @@ __device__ __forceinline__ void load_pairs(const T* row, int l, int D, int m, in
   }
 }
 
-template <typename T, int MODE, int NP>
+template <typename T, int MODE, int NP, bool PAST = false>  // PAST: past the caches
 __device__ __forceinline__ void store_pairs(T* row, int l, int D, int m, int layout, const float (&a)[NP], const float (&b)[NP]) {
   if constexpr (MODE == M_ANY) {
 #pragma unroll
@@ -84,8 +84,16 @@ __device__ __forceinline__ void store_pairs(T* row, int l, int D, int m, int lay
       if (half) { e[i] = va; e[NP + i] = vb; }
       else { e[2 * i] = va; e[2 * i + 1] = vb; }
     }
-    *reinterpret_cast<uint4*>(row + c0) = *reinterpret_cast<uint4*>(e);
-    *reinterpret_cast<uint4*>(row + c1) = *reinterpret_cast<uint4*>(e + NP);
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    u4* d0 = reinterpret_cast<u4*>(row + c0);
+    u4* d1 = reinterpret_cast<u4*>(row + c1);
+    if constexpr (PAST) {
+      __builtin_nontemporal_store(*reinterpret_cast<u4*>(e), d0);
+      __builtin_nontemporal_store(*reinterpret_cast<u4*>(e + NP), d1);
+    } else {
+      *d0 = *reinterpret_cast<u4*>(e);
+      *d1 = *reinterpret_cast<u4*>(e + NP);
+    }
   }
 }
 
@@ -139,9 +147,10 @@ struct RopePlan {
   int G;       // lanes of a token (a power of two, divides 64)
   int hc;      // heads a lane group walks over
   int nq, nk;  // head chunks of q and of k: blockIdx.y < nq is a chunk of q
+  int past;    // outputs that no cache holds until they are read are written past the caches
 };
 
-template <typename T, int MODE, bool NORM>
+template <typename T, int MODE, bool NORM, bool PAST>
 __global__ __launch_bounds__(kThreads) void k_rope_fwd(ic_rope_args a, RopePlan p) {
   constexpr int NP = Own<T, MODE>::NP;
   constexpr int UH = 2;  // rows in flight
@@ -192,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void k_rope_fwd(ic_rope_args a, RopePlan 
         ya[i] = rot ? xa[u][i] * c[i] - xb[u][i] * s[i] : xa[u][i];
         yb[i] = rot ? xa[u][i] * s[i] + xb[u][i] * c[i] : xb[u][i];
       }
-      store_pairs<T, MODE, NP>(Y + (int64_t)(h + u) * r.y_sh, l, a.D, a.m, a.layout, ya, yb);
+      store_pairs<T, MODE, NP, PAST>(Y + (int64_t)(h + u) * r.y_sh, l, a.D, a.m, a.layout, ya, yb);
     }
 #pragma unroll
     for (int u = 0; u < UH; ++u)
@@ -202,7 +211,7 @@ __global__ __launch_bounds__(kThreads) void k_rope_fwd(ic_rope_args a, RopePlan 
 
 // Backward with norms: u = w xhat, xhat = x inv; with h = R^T g:  gw = sum h xhat,  gx = inv (w h - xhat mean(w h xhat)).
 // A workgroup walks over tokens (grid stride), so that gw leaves it as ONE partial sum per channel.
-template <typename T, int MODE>
+template <typename T, int MODE, bool PAST>
 __global__ __launch_bounds__(kThreads) void k_rope_norm_bwd(ic_rope_bwd_args ba, RopePlan p) {
   constexpr int NP = Own<T, MODE>::NP;
   __shared__ float red[kThreads / 64][512];
@@ -260,7 +269,7 @@ __global__ __launch_bounds__(kThreads) void k_rope_norm_bwd(ic_rope_bwd_args ba,
         ga[i] = inv * (wa[i] * ga[i] - na * mean);
         gb[i] = inv * (wb[i] * gb[i] - nb * mean);
       }
-      store_pairs<T, MODE, NP>(GX + (int64_t)h * g.gx_sh, l, a.D, a.m, a.layout, ga, gb);
+      store_pairs<T, MODE, NP, PAST>(GX + (int64_t)h * g.gx_sh, l, a.D, a.m, a.layout, ga, gb);
     }
   }
   // the workgroup's sum of each channel, in a fixed order: lane groups of a wave, then the four waves
@@ -368,6 +377,10 @@ RopePlan plan_of(const ic_rope_args& a, int mode, bool limit_blocks, int* gx) {
   while (p.hc > 1 && blocks * (ic_ceil_div(a.q.H, p.hc) + ic_ceil_div(a.k.H, p.hc)) < 1024) p.hc = (p.hc + 1) / 2;
   p.nq = ic_ceil_div(a.q.H, p.hc);
   p.nk = ic_ceil_div(a.k.H, p.hc);
+  // Outputs of more than half of the 256 MB cache, with norms: a pass forward and backward over 32768 positions of 16 + 4
+  // heads of 128 bf16 channels (168 MB a tensor) takes 192 us with them past the caches, 205 us through them, 206 us with
+  // only the backward's past them; without norms (a copy's pattern) 147 against 141 us, so not there.
+  p.past = a.q.w && (int64_t)a.B * a.T * (a.q.H + a.k.H) * a.D * ic_dt_size(a.dtype) > (128 << 20);
   int64_t n = blocks;
   if (limit_blocks) {  // (heads enough to fill kParts on their own: one token column of workgroups walks over all tokens)
     const int64_t most = kParts / (p.nq + p.nk);
@@ -409,11 +422,14 @@ extern "C" int ic_rope_fwd(const ic_rope_args* a, ic_stream_t stream) {
   const RopePlan p = plan_of(*a, mode, false, &gx);
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid(gx, p.nq + p.nk);
-#define IC_BODY(T)                                                                                                  \
-  if (a->q.w) IC_TIMED(IC_KID_rope_fwd, st, hipLaunchKernelGGL((k_rope_fwd<T, MODE, true>), grid, dim3(kThreads), 0, st, *a, p)); \
-  else IC_TIMED(IC_KID_rope_fwd, st, hipLaunchKernelGGL((k_rope_fwd<T, MODE, false>), grid, dim3(kThreads), 0, st, *a, p))
+#define IC_ROPE_FWD(T, NORM, PAST) IC_TIMED(IC_KID_rope_fwd, st, hipLaunchKernelGGL((k_rope_fwd<T, MODE, NORM, PAST>), grid, dim3(kThreads), 0, st, *a, p))
+#define IC_BODY(T)                                     \
+  if (!a->q.w) { IC_ROPE_FWD(T, false, false); }       \
+  else if (p.past) { IC_ROPE_FWD(T, true, true); }     \
+  else { IC_ROPE_FWD(T, true, false); }
   IC_ROPE_DISPATCH(a->dtype, mode, IC_BODY);
 #undef IC_BODY
+#undef IC_ROPE_FWD
   IC_LAUNCH_CHECK("ic_rope_fwd");
   return IC_OK;
 }
@@ -439,7 +455,9 @@ extern "C" int ic_rope_bwd(const ic_rope_bwd_args* b, ic_stream_t stream) {
   const RopePlan p = plan_of(*a, mode, true, &gx);
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid(gx, p.nq + p.nk);
-#define IC_BODY(T) IC_TIMED(IC_KID_rope_bwd, st, hipLaunchKernelGGL((k_rope_norm_bwd<T, MODE>), grid, dim3(kThreads), 0, st, *b, p))
+#define IC_BODY(T)                                                                                                            \
+  if (p.past) IC_TIMED(IC_KID_rope_bwd, st, hipLaunchKernelGGL((k_rope_norm_bwd<T, MODE, true>), grid, dim3(kThreads), 0, st, *b, p)); \
+  else IC_TIMED(IC_KID_rope_bwd, st, hipLaunchKernelGGL((k_rope_norm_bwd<T, MODE, false>), grid, dim3(kThreads), 0, st, *b, p))
   IC_ROPE_DISPATCH(a->dtype, mode, IC_BODY);
 #undef IC_BODY
   IC_LAUNCH_CHECK("ic_rope_bwd");

@@ -7,6 +7,7 @@ gradients are deferred to one ic_*_wgrad launch per backward pass through a tape
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Callable, Dict, List, Optional
 
@@ -964,15 +965,19 @@ def _rows4(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _dense_order(t: torch.Tensor) -> list:
-    """Strides of a dense [B,H,T,D] tensor whose dimensions lie in memory in the order of t's, channels side by side: the
-    gradient of a [B,T,H,D]-ordered view comes back in that order."""
-    shape, stride = t.shape, t.stride()
+@functools.lru_cache(maxsize=1024)
+def _dense_strides(shape: torch.Size, stride: tuple) -> tuple:
     out, n = [0, 0, 0, 1], shape[3]
     for i in sorted((0, 1, 2), key=stride.__getitem__):
         out[i] = n
         n *= shape[i]
-    return out
+    return tuple(out)
+
+
+def _dense_order(t: torch.Tensor) -> tuple:
+    """Strides of a dense [B,H,T,D] tensor whose dimensions lie in memory in the order of t's, channels side by side: the
+    gradient of a [B,T,H,D]-ordered view comes back in that order."""
+    return _dense_strides(t.shape, t.stride())
 
 
 def _wants_grad(*ts) -> bool:
