@@ -331,6 +331,66 @@ class AdaptiveFilterAttention(FastAttrs, nn.Module):
                 "attn_entropy_mean": float(self.last_attn_entropy)}
 
 
+class DecayLinearAttention(nn.Module):
+    """Causal linear attention with a learned decay for each head, next to the two softmax attentions: cost linear in the
+    length, and a state [B,H,hd,hd] instead of a cache for the positions that follow.  The decay is the region cells'
+    (region.py:87,128-135: softplus of a raw parameter), one for each head; queries and keys are normed per head and rotated.
+
+    forward(x) reads whole sequences (training, prompts), step(x) one position of each (serving); both hand the state on:
+        y, state = att(prompt)                     # [B,T,C]
+        y = att.step(x, state, positions)          # [B,C], state updated in place, positions [B]
+    n_kv_head < n_head: keys and values shared by groups of heads.  rope_m channel pairs of a head are rotated (None: all)."""
+
+    def __init__(self, n_embd: int, n_head: int, n_kv_head: Optional[int] = None, *, rope_m: Optional[int] = None,
+                 rope_base: float = 10000.0, rope_layout: str = "half", rope_scaling: str = "none", rope_factor: float = 1.0,
+                 trained_len: int = 0, eps: float = 1e-5):
+        super().__init__()
+        n_kv_head = n_head if n_kv_head is None else n_kv_head
+        assert n_embd % n_head == 0 and n_head % n_kv_head == 0
+        self.n_head, self.n_kv_head, self.head_dim, self.eps = n_head, n_kv_head, n_embd // n_head, eps
+        self.scale = self.head_dim ** -0.5
+        self.c_attn = nn.Linear(n_embd, (n_head + 2 * n_kv_head) * self.head_dim)
+        self.c_proj = nn.Linear(n_embd, n_embd)
+        self.q_weight, self.k_weight = nn.Parameter(torch.ones(self.head_dim)), nn.Parameter(torch.ones(self.head_dim))
+        rate = 0.5 ** torch.linspace(1.0, 9.0, n_head)  # memories of 2 .. 512 positions
+        self.raw_decay = nn.Parameter(torch.log(torch.expm1(rate)))
+        m = self.head_dim // 2 if rope_m is None else rope_m
+        self.rope_layout = rope_layout
+        self._freqs, self.rope_scale = rope_freqs(m, rope_base, scaling=rope_scaling, factor=rope_factor, trained_len=trained_len)
+
+    def rate(self) -> torch.Tensor:
+        """[n_head] fp32 decay rates."""
+        return F.softplus(self.raw_decay.float())
+
+    def _qkv(self, x: torch.Tensor, positions: Optional[torch.Tensor]):
+        """Normed and rotated q [B,H,T,hd], k [B,Hk,T,hd], and v [B,Hk,T,hd] of x [B,T,C]."""
+        if self._freqs.device != x.device:
+            self._freqs = self._freqs.to(x.device)  # (fp64, and no buffer: module.bfloat16() must not round it)
+        B, T, _ = x.shape
+        H, Hk, hd = self.n_head, self.n_kv_head, self.head_dim
+        q, k, v = (t.view(B, T, -1, hd).transpose(1, 2) for t in self.c_attn(x).split([H * hd, Hk * hd, Hk * hd], dim=2))
+        q, k = ops.qk_norm_rope(q, k, self.q_weight, self.k_weight, eps=self.eps, positions=positions, freqs=self._freqs,
+                                layout=self.rope_layout, scale=self.rope_scale)
+        return q, k, v
+
+    def forward(self, x: torch.Tensor, state: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                valid_len: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """x [B,T,C] -> (y [B,T,C], state [B,H,hd,hd] fp32 behind position valid_len - 1).  positions: integers [T] or [B,T]
+        (None: 0 .. T-1; with a state, the positions at which x continues)."""
+        B, T, C = x.shape
+        q, k, v = self._qkv(x, positions)
+        y, state = ops.linear_attention(q, k, v, self.rate(), scale=self.scale, state=state, valid_len=valid_len)
+        return self.c_proj(y.transpose(1, 2).reshape(B, T, C)), state
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, state: torch.Tensor, positions: torch.Tensor, active: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x [B,C] at positions [B] -> y [B,C]; state is updated in place (active [B]: only where it is set)."""
+        B, C = x.shape
+        q, k, v = self._qkv(x.unsqueeze(1), positions.view(B, 1))
+        y = ops.linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], self.rate(), state, scale=self.scale, active=active)
+        return self.c_proj(y.reshape(B, C))
+
+
 class LocalTokenMixer(FastAttrs, nn.Module):
     """Anchor tokens + one attention block; returns the mean of the focused positions
     (iron_rope.py:254-374)."""

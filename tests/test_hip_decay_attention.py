@@ -1,0 +1,164 @@
+"""The token-mixing operators as they are used together (mixer.DecayLinearAttention: projection, norms and rotation of queries
+and keys, linear attention, projection), for whole sequences and position by position, and at sizes that pass 32-bit offsets
+and the cache."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+DEV = "cuda:0"
+pytestmark = pytest.mark.gpu
+
+
+def module(**kw):
+    from ironcortex_amd.mixer import DecayLinearAttention
+    torch.manual_seed(21)
+    att = DecayLinearAttention(96, 6, **kw).to(DEV)
+    with torch.no_grad():
+        att.q_weight.add_(0.3 * torch.randn_like(att.q_weight))
+        att.k_weight.add_(0.3 * torch.randn_like(att.k_weight))
+    return att
+
+
+def plain(P, x, att, positions, valid):
+    """The block in 64 bits from its formulas, position by position; P: its parameters in 64 bits."""
+    B, T, C = x.shape
+    H, Hk, hd = att.n_head, att.n_kv_head, att.head_dim
+    q, k, v = (F.linear(x, P["c_attn.weight"], P["c_attn.bias"])).split([H * hd, Hk * hd, Hk * hd], dim=2)
+    q, k, v = (t.reshape(B, T, -1, hd).transpose(1, 2) for t in (q, k, v))
+    f = att._freqs.to(x.device)
+    m = f.shape[0]
+    ang = positions.double().view(1, 1, -1, 1) * f
+    c, s = torch.cos(ang) * att.rope_scale, torch.sin(ang) * att.rope_scale
+
+    def norm_rotate(t, w):
+        t = t / torch.sqrt(t.square().mean(-1, keepdim=True) + att.eps) * w
+        if att.rope_layout == "half":
+            a, b = t[..., :m], t[..., m:2 * m]
+            r = torch.cat([a * c - b * s, a * s + b * c], dim=-1)
+        else:
+            a, b = t[..., 0:2 * m:2], t[..., 1:2 * m:2]
+            r = torch.stack([a * c - b * s, a * s + b * c], dim=-1).flatten(-2)
+        return torch.cat([r, t[..., 2 * m:]], dim=-1)
+
+    q, k = norm_rotate(q, P["q_weight"]), norm_rotate(k, P["k_weight"])
+    k, v = k.repeat_interleave(H // Hk, 1), v.repeat_interleave(H // Hk, 1)
+    lam = torch.exp(-F.softplus(P["raw_decay"])).view(1, H, 1, 1)
+    S, ys = torch.zeros(B, H, hd, hd, dtype=x.dtype, device=x.device), []
+    for t in range(T):
+        live = (valid > t).view(B, 1, 1, 1)
+        S = torch.where(live, lam * S + k[:, :, t].unsqueeze(-1) * v[:, :, t].unsqueeze(-2), S)
+        ys.append(torch.where(live[..., 0], (q[:, :, t].unsqueeze(-2) @ S).squeeze(-2), 0.0) / math.sqrt(hd))
+    y = torch.stack(ys, 2).transpose(1, 2).reshape(B, T, C)
+    return F.linear(y, P["c_proj.weight"], P["c_proj.bias"]), S
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(n_kv_head=2, rope_m=4, rope_layout="interleaved"), dict(n_kv_head=1, rope_scaling="ramp", rope_factor=4.0, trained_len=64)])
+def test_block_forward_and_gradients(kw):
+    """fp32 against 64 bits: every quantity passes some 16 + 96 + 200 roundings of u = 2^-24 at most; 2e-5 of the largest
+    magnitude is 335 u."""
+    att = module(**kw)
+    B, T = 3, 150
+    x = torch.randn(B, T, 96, device=DEV, requires_grad=True)
+    valid = torch.tensor([150, 97, 0], device=DEV)
+    gy, gS = torch.randn(B, T, 96, device=DEV), torch.randn(B, 6, 16, 16, device=DEV)
+    y, S = att(x, valid_len=valid)
+    names = [n for n, _ in att.named_parameters()]
+    grads = torch.autograd.grad((y, S), [x] + list(att.parameters()), (gy, gS))
+    P = {n: p.detach().double().requires_grad_(True) for n, p in att.named_parameters()}
+    xd = x.detach().double().requires_grad_(True)
+    yw, Sw = plain(P, xd, att, torch.arange(T, device=DEV), valid)
+    want = torch.autograd.grad((yw, Sw), [xd] + [P[n] for n in names], (gy.double(), gS.double()))
+    for n, a, b in [("y", y, yw), ("state", S, Sw)] + list(zip(["x"] + names, grads, want)):
+        err = float((a.detach().double() - b.detach()).abs().max() / b.detach().abs().max().clamp_min(1e-30))
+        assert err <= 2e-5, (n, err)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prompt_then_steps_equals_one_call(dtype):
+    """A ragged batch of prompts, then position by position (some sequences paused), against whole sequences read at once.
+    fp32: the same sums in another order; bf16: every row is rounded to bf16 at the same places in both (projections, normed
+    rows, outputs: four roundings of 2^-8 of values that a projection of 96 sums adds up)."""
+    att = module(n_kv_head=3).to(dtype)
+    B, T, n = 4, 90, 7
+    x = torch.randn(B, T, 96, device=DEV).to(dtype)
+    start = torch.tensor([60, 3, 83, 1], device=DEV)
+    with torch.no_grad():
+        _, state = att(x, valid_len=start)
+        got = []
+        pos = start.clone()
+        for i in range(n + 2):
+            active = pos < start + n
+            active[1] &= i != 2  # (a pause)
+            xi = x[torch.arange(B, device=DEV), pos.clamp(max=T - 1)]
+            before = state.clone()
+            y = att.step(xi, state, pos, active=active)
+            assert torch.equal(state[~active], before[~active])
+            got.append((y, pos.clone(), active))
+            pos = pos + active
+        whole, last = att(x, valid_len=start + n)
+    assert bool((pos == start + n).all())
+    scale = float(whole.float().abs().max())
+    tol = 1e-5 if dtype == torch.float32 else 4 * 2.0 ** -8
+    for y, p, active in got:
+        w = whole[torch.arange(B, device=DEV), p.clamp(max=T - 1)]
+        assert float((y.float() - w.float())[active].abs().max() if bool(active.any()) else 0.0) <= tol * scale
+    assert float((state - last).abs().max()) <= tol * float(last.abs().max())
+
+
+def test_block_trains_in_bf16_and_keeps_its_frequencies():
+    att = module().bfloat16()
+    x = torch.randn(2, 70, 96, device=DEV, dtype=torch.bfloat16)
+    y, S = att(x)
+    y.float().square().mean().backward()
+    assert y.dtype == torch.bfloat16 and S.dtype == torch.float32 and att._freqs.dtype == torch.float64
+    assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in att.parameters())
+
+
+def test_rows_beyond_the_cache_equal_their_pieces():
+    """168 MB of rows (written past the caches) against the same rows in pieces, bit for bit; the weights' gradients as sums of
+    the pieces' within the rounding of sums of 2^16 terms."""
+    from ironcortex_amd.hip import ops
+    g = torch.Generator(device=DEV).manual_seed(3)
+    T, H, D = 70001, 3, 128
+    q, k = (torch.randn(1, T, h, D, generator=g, device=DEV).transpose(1, 2).requires_grad_(True) for h in (H, 2))
+    w = [torch.randn(D, generator=g, device=DEV).requires_grad_(True) for _ in (0, 1)]
+    f = torch.rand(40, generator=g, device=DEV)
+    go = [torch.randn(1, h, T, D, generator=g, device=DEV) for h in (H, 2)]
+    pos = torch.arange(T, device=DEV)
+    y = ops.qk_norm_rope(q, k, *w, positions=pos, freqs=f, layout="half")
+    gr = torch.autograd.grad(y, (q, k, *w), go)
+    sums, mags = [0.0, 0.0], [0.0, 0.0]
+    for a, b in ((0, 30000), (30000, T)):
+        qa, ka = q[:, :, a:b].detach().requires_grad_(True), k[:, :, a:b].detach().requires_grad_(True)
+        ya = ops.qk_norm_rope(qa, ka, *w, positions=pos[a:b], freqs=f, layout="half")
+        ga = torch.autograd.grad(ya, (qa, ka, *w), [t[:, :, a:b] for t in go])
+        for i in (0, 1):
+            assert torch.equal(ya[i], y[i][:, :, a:b]) and torch.equal(ga[i], gr[i][:, :, a:b])
+            sums[i] = sums[i] + ga[2 + i].double()
+            mags[i] = mags[i] + ga[2 + i].abs().double()
+    for i in (0, 1):  # random signs: a sum of n = 2.1e5 terms of size ~1 is off by about sqrt(n) u sqrt(n)
+        assert float((gr[2 + i].double() - sums[i]).abs().max()) <= 2.0 ** -24 * 2.1e5
+
+
+def test_offsets_beyond_32_bits():
+    """Rows of more than 2^31 elements (4.3 GB of bf16): the last positions against a small call on them alone."""
+    from ironcortex_amd.hip import ops
+    T, D, n = (1 << 24) + 77, 128, 300
+    x = torch.empty(1, 1, T, D, device=DEV, dtype=torch.bfloat16)
+    for i in range(0, T, 1 << 20):
+        x[:, :, i:i + (1 << 20)] = torch.randn(1, 1, min(1 << 20, T - i), D, device=DEV).bfloat16()
+    f = 10000.0 ** (-torch.arange(64, device=DEV, dtype=torch.float64) / 64)
+    y = ops.rope(x, freqs=f, layout="half")
+    pos = torch.arange(T - n, T, device=DEV)
+    assert torch.equal(y[:, :, T - n:], ops.rope(x[:, :, T - n:], positions=pos, freqs=f, layout="half"))
+    assert torch.equal(y[:, :, :n], ops.rope(x[:, :, :n], freqs=f, layout="half"))
+    del y
+    rate = torch.tensor([0.05], device=DEV)  # what lies 1000 positions back counts e^-50
+    out, S = ops.linear_attention(x, x, x, rate, scale=0.01)
+    m = 64 * 40 + 77 % 64  # (chunks at the same places)
+    o2, S2 = ops.linear_attention(x[:, :, T - m:], x[:, :, T - m:], x[:, :, T - m:], rate, scale=0.01)
+    a, b = out[:, :, T - n:].float(), o2[:, :, m - n:].float()
+    assert float((a - b).abs().max()) <= 2.0 ** -8 * float(b.abs().max())
+    assert float((S - S2).abs().max()) <= 1e-5 * float(S2.abs().max())
