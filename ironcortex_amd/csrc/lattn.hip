@@ -359,21 +359,15 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
     const int cnt = n - base < 0 ? 0 : n - base < kC ? n - base : kC;
     if (SUMS && cnt == 0) break;
     const int off = rev && ch == 0 ? 1 : 0;  // (the gradient of the final state enters without a step of decay)
-    v4f O[4], vw[4];
+    v4f O[4], v0[4];
     float drc = 0.f;
     if (cnt > 0) {
       R::put(Ks, fk);
       if constexpr (!SUMS) R::put(lds.Qs, fq);
-      v4f v0[4];
 #pragma unroll
       for (int s = 0; s < 4; ++s) v0[s] = vf[s];
       __syncthreads();
       if (ch + 1 < ch1 && base + kC < n) fetch(base + kC);
-      const float* dl = &lds.dev[kC + cnt - 1 - q4 - 51];  // (51: the largest position of this lane's values)
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) vw[s][u] = v0[s][u] * dl[51 - 16 * s - u];
       if constexpr (!SUMS) {
         auto& Ps = lds.Ps;
         auto& Qs = lds.Qs;
@@ -481,19 +475,21 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
         if constexpr (LAG) L[t] = carry * (L[t] + (float)cnt * S[t]);
         S[t] = carry * S[t];
       }
+      const float* dl = &lds.dev[kC + cnt - 1 - q4 - 51];  // (51: the largest position of this lane's values)
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        v4f vl;
-        if constexpr (LAG) {
+        v4f vw, vl;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) vl[u] = vw[s][u] * (float)(cnt - 1 - q4 - 16 * s - u);  // (0 behind the last valid position)
+        for (int u = 0; u < 4; ++u) {
+          vw[u] = v0[s][u] * dl[51 - 16 * s - u];
+          if constexpr (LAG) vl[u] = vw[u] * (float)(cnt - 1 - q4 - 16 * s - u);  // (0 behind the last valid position)
         }
 #pragma unroll
         for (int t = 0; t < KS; ++t) {
           v4f ak;
 #pragma unroll
           for (int u = 0; u < 4; ++u) ak[u] = Ks[16 * s + q4 + u][16 * t + c];
-          S[t] = mma16(ak, vw[s], S[t]);
+          S[t] = mma16(ak, vw, S[t]);
           if constexpr (LAG) L[t] = mma16(ak, vl, L[t]);
         }
       }
