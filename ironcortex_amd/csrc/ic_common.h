@@ -225,11 +225,11 @@ enum IcKid {
   IC_KID_lattn_scan,
   IC_KID_lattn_fwd,
   IC_KID_lattn_bwd,
-  IC_KID_lattn_join,
+  IC_KID_lattn_drate,
   IC_KID_lattn_step,
   IC_KID_COUNT
 };
-#define IC_KID_NAMES {"region_pro", "region_rkv", "region_out", "region_fin", "kwta_rows", "region_fin_bwd", "region_out_bwd", "region_mid_bwd", "region_rkv_bwd", "region_pro_bwd", "wgrad_region", "router_edge_fwd", "router_combine", "router_fwd", "router_comb_bwd", "router_mat_bwd", "router_gather_bwd", "wgrad_edge", "hebbian", "gate_scores", "gate_select", "mul", "rmsnorm_fwd", "rmsnorm_bwd", "goodness_fwd", "goodness_bwd", "gemv", "ws_write", "token_rows", "logits_combine", "branch_score", "steer_select", "router_mfma", "wgrad_mfma", "region_state", "attn_fwd", "attn_bwd_kv", "attn_bwd_q", "linear_bwd", "loop_steer", "rope_fwd", "rope_bwd", "lattn_sums", "lattn_scan", "lattn_fwd", "lattn_bwd", "lattn_join", "lattn_step"}
+#define IC_KID_NAMES {"region_pro", "region_rkv", "region_out", "region_fin", "kwta_rows", "region_fin_bwd", "region_out_bwd", "region_mid_bwd", "region_rkv_bwd", "region_pro_bwd", "wgrad_region", "router_edge_fwd", "router_combine", "router_fwd", "router_comb_bwd", "router_mat_bwd", "router_gather_bwd", "wgrad_edge", "hebbian", "gate_scores", "gate_select", "mul", "rmsnorm_fwd", "rmsnorm_bwd", "goodness_fwd", "goodness_bwd", "gemv", "ws_write", "token_rows", "logits_combine", "branch_score", "steer_select", "router_mfma", "wgrad_mfma", "region_state", "attn_fwd", "attn_bwd_kv", "attn_bwd_q", "linear_bwd", "loop_steer", "rope_fwd", "rope_bwd", "lattn_sums", "lattn_scan", "lattn_fwd", "lattn_bwd", "lattn_drate", "lattn_step"}
 
 // Optional live kernel timing with HIP events on the launch stream (ic_prof_* in the header).
 extern bool g_ic_prof_on;

@@ -21,6 +21,8 @@
 // l holds rows 4 (l / 16) + 0..3 of column l % 16, and as an operand k-indices 4 (l / 16) + 0..3 of row / column l % 16).
 // Several segments per sequence only where sequences and heads do not fill the chip: their sums are formed first
 // (k_lattn SUMS), scanned (k_lattn_scan), and each segment starts from its own prefix.
+#include <type_traits>
+
 #include "ic_types.h"
 
 namespace {
@@ -36,11 +38,17 @@ struct Mat {  // rows [B,heads,T,D] of one of q, k, v, dout, ...
   int32_t vec;    // 16-byte accesses are allowed
 };
 
+struct Span {
+  int32_t nseg, cps;        // segments of a sequence, chunks of a segment
+};
+
 struct Pass {
   Mat q, k, v, out, x;      // x: the rows that the lag-weighted output is multiplied with (d rate)
+  Span sp;
+  int32_t G;                // query heads whose outputs are one output (gradients of shared heads): a workgroup takes them in turn,
+  float* part;              // keeping the sum so far in fp32 rows [B,H/G,T,Db] that only its own lanes touch
   int32_t Da, Db;           // channels of q / k rows and of v / out rows
   int32_t rev;              // positions from the last valid one down
-  int32_t out32;            // out is fp32 whatever the rows' type (partial sums of shared heads)
   float oscale, vscale;
   const float* init;        // start state: element (b*H + h) * Dk*Dv + a*ia + b*ib, or NULL: zero
   int32_t ia, ib;
@@ -54,13 +62,14 @@ struct Pass {
 
 struct Sums {               // segment sums of one state
   Mat k, v;
+  Span sp;
   int32_t Da, Db, rev, lag;
   float vscale;
   float* seg;
 };
 
 struct Geo {
-  int32_t B, H, T, nseg, cps;  // cps: chunks of a segment
+  int32_t B, H, T;
   const float* rate;
   const int32_t* valid_len;
 };
@@ -274,40 +283,57 @@ __device__ __forceinline__ double dot_state(const v4f (&S)[NT], const float* src
 }
 // the end of a segment: its sums, or (last segment) the end state and its share of d rate; d rate's partial sum.
 template <bool LAG, int NT, int NL>
-__device__ __forceinline__ void write_sums(const Geo& g, const Sums* sm, const v4f (&S)[NT], const v4f (&L)[NL], size_t dd, int Da, int Db, int col, int q4, int bh, int seg) {
-  float* dst = sm->seg + ((size_t)bh * g.nseg + seg) * (LAG ? 2 : 1) * dd;
+__device__ __forceinline__ void write_sums(const Sums* sm, const v4f (&S)[NT], const v4f (&L)[NL], size_t dd, int Da, int Db, int col, int q4, int bh, int seg) {
+  float* dst = sm->seg + ((size_t)bh * sm->sp.nseg + seg) * (LAG ? 2 : 1) * dd;
   store_state(S, dst, Db, 1, Da, Db, col, q4, 1.f);
   if constexpr (LAG) store_state(L, dst + dd, Db, 1, Da, Db, col, q4, 1.f);
 }
 template <bool LAG, int NT, int NL>
-__device__ __forceinline__ double write_end(const Geo& g, const Pass* p, const v4f (&S)[NT], const v4f (&L)[NL], size_t dd, int Da, int Db, int col, int q4, int bh, int seg, int n, float l2) {
+__device__ __forceinline__ double write_end(const Pass* p, const v4f (&S)[NT], const v4f (&L)[NL], size_t dd, int Da, int Db, int col, int q4, int bh, int seg, int n, float l2) {
   double dr = 0.0;
-  if (seg != g.nseg - 1) return dr;
+  if (seg != p->sp.nseg - 1) return dr;
   if (p->fin) store_state(S, p->fin + (size_t)bh * dd, p->ia, p->ib, Da, Db, col, q4, p->fin_decay && n > 0 ? decay(l2, 1) : 1.f);
   if constexpr (LAG) {
     if (p->gfin) dr -= dot_state(L, p->gfin + (size_t)bh * dd, p->ia, p->ib, Da, Db, col, q4);
   }
   return dr;
 }
+// four columns of a shared output: the sum of the heads so far comes from, or goes to, the fp32 rows
+__device__ __forceinline__ v4f add_part(const Pass* p, v4f o, int64_t at, int gi, int c0, int D) {
+  float* part = p->part + at;
+  if (D % 4 == 0) {
+    if (gi > 0) o += ld4(part);
+    if (gi < p->G - 1) *reinterpret_cast<v4f*>(part) = o;
+  } else {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      if (c0 + v >= D) continue;
+      if (gi > 0) o[v] += part[v];
+      if (gi < p->G - 1) part[v] = o[v];
+    }
+  }
+  return o;
+}
 template <int NW>
-__device__ __forceinline__ void write_drate(const Geo& g, const Pass* p, double* red, double dr, int bh, int seg) {
+__device__ __forceinline__ void write_drate(const Pass* p, double* red, double dr, int bh, int seg) {
   for (int o = 32; o; o >>= 1) dr += __shfl_xor(dr, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = dr;
   __syncthreads();
   if (threadIdx.x == 0) {
     double t = 0.0;
     for (int i = 0; i < NW; ++i) t += red[i];
-    p->dr[(size_t)bh * g.nseg + seg] = t;
+    p->dr[(size_t)bh * p->sp.nseg + seg] = t;
   }
 }
 
-template <typename T, int DP, bool LAG, bool SUMS, typename LDS>
-__device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Sums* sm, LDS& lds) {
+template <typename T, int DP, bool LAG, bool SUMS, bool SHARED, typename LDS>
+__device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Sums* sm, LDS& lds, int b, int h, int seg) {
   constexpr int NT = DP * 4, NW = DP / 16, KS = DP / 16, MT = (10 + NW - 1) / NW;
   using R = RowsF<T, DP, NT>;
   auto& Ks = lds.Ks;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, q4 = (lane >> 4) * 4;
-  const int seg = blockIdx.x % g.nseg, bh = blockIdx.x / g.nseg, b = bh / g.H, h = bh - b * g.H;
+  const int bh = b * g.H + h;
+  const Span sp = SUMS ? sm->sp : p->sp;
   const int n = valid_of(g, b), T_ = g.T;
   const float l2 = -g.rate[h] * 1.44269504088896340736f;
   const int Da = SUMS ? sm->Da : p->Da, Db = SUMS ? sm->Db : p->Db;
@@ -325,7 +351,7 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
     lds.dev[i] = d * vscale;
   }
   const int NC = (T_ + kC - 1) / kC;
-  const int ch0 = seg * g.cps, ch1 = ch0 + g.cps < NC ? ch0 + g.cps : NC;
+  const int ch0 = seg * sp.cps, ch1 = ch0 + sp.cps < NC ? ch0 + sp.cps : NC;
   const size_t dd = (size_t)Da * Db;
 
   v4f S[KS], L[LAG ? KS : 1];
@@ -335,7 +361,7 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
     if constexpr (LAG) L[t] = S[t];
   }
   if constexpr (!SUMS) {
-    const float* s0 = p->seg ? p->seg + ((size_t)bh * g.nseg + seg) * p->nst * dd : p->init ? p->init + (size_t)bh * dd : nullptr;
+    const float* s0 = p->seg ? p->seg + ((size_t)bh * sp.nseg + seg) * p->nst * dd : p->init ? p->init + (size_t)bh * dd : nullptr;
     const int ia = p->seg ? p->sga : p->ia, ib = p->seg ? p->sgb : p->ib;
     if (s0) {
       load_state(S, s0, ia, ib, Da, Db, col, q4);
@@ -441,30 +467,30 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
     }
     if constexpr (!SUMS) {
       const int b0 = 16 * w + q4;  // this lane's four columns of a row
-      const int64_t ob = (int64_t)b * p->out.sb + (int64_t)h * p->out.sh;
+      const int64_t ob = (int64_t)b * p->out.sb + (int64_t)(h / p->out.group) * p->out.sh;
+      const int gi = SHARED ? h % p->G : 0;
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
         const int i = base + 16 * it + c;
         if (i >= T_ || b0 >= Db) continue;
         const bool live = i < n;
-        const int64_t at = ob + (rev && live ? n - 1 - i : i) * p->out.st + b0;
-        const v4f o = live ? O[it] : v4f{0.f, 0.f, 0.f, 0.f};
+        const int64_t t = rev && live ? n - 1 - i : i;
+        v4f o = live ? O[it] : v4f{0.f, 0.f, 0.f, 0.f};
+        if constexpr (SHARED) {
+          o = add_part(p, o, ((int64_t)(bh / p->G) * T_ + t) * Db + b0, gi, b0, Db);
+          if (gi < p->G - 1) continue;
+        }
+        T* row = (T*)p->out.p + ob + t * p->out.st + b0;
         if (p->out.vec) {
-          if (sizeof(T) == 4 || p->out32) {
-            *reinterpret_cast<v4f*>((float*)p->out.p + at) = o;
-          } else {
-            union { T e[4]; uint2 u; } x;
+          union { T e[4]; uint4 u4; uint2 u2; } x;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) x.e[v] = ic_from_f<T>(o[v]);
-            *reinterpret_cast<uint2*>((T*)p->out.p + at) = x.u;
-          }
+          for (int v = 0; v < 4; ++v) x.e[v] = ic_from_f<T>(o[v]);
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(row) = x.u4;
+          else *reinterpret_cast<uint2*>(row) = x.u2;
         } else {
 #pragma unroll
           for (int v = 0; v < 4; ++v)
-            if (b0 + v < Db) {
-              if (p->out32) ((float*)p->out.p)[at + v] = o[v];
-              else ((T*)p->out.p)[at + v] = ic_from_f<T>(o[v]);
-            }
+            if (b0 + v < Db) row[v] = ic_from_f<T>(o[v]);
         }
       }
     }
@@ -497,10 +523,10 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
     }
   }
   if constexpr (SUMS) {
-    write_sums<LAG>(g, sm, S, L, dd, Da, Db, col, q4, bh, seg);
+    write_sums<LAG>(sm, S, L, dd, Da, Db, col, q4, bh, seg);
   } else {
-    dr += write_end<LAG>(g, p, S, L, dd, Da, Db, col, q4, bh, seg, n, l2);
-    if constexpr (LAG) write_drate<NW>(g, p, lds.red, dr, bh, seg);
+    dr += write_end<LAG>(p, S, L, dd, Da, Db, col, q4, bh, seg, n, l2);
+    if constexpr (LAG) write_drate<NW>(p, lds.red, dr, bh, seg);
   }
 }
 
@@ -581,9 +607,8 @@ __device__ __forceinline__ void split(const v4f& a, const v4f& b, b8 (&out)[2]) 
 }
 
 // four consecutive columns of an output row
-__device__ __forceinline__ void store4(char* row, const v4f& o, bool f32) {
-  if (f32) *reinterpret_cast<v4f*>(row) = o;
-  else *reinterpret_cast<uint2*>(row) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
+__device__ __forceinline__ void store4(char* row, const v4f& o) {
+  *reinterpret_cast<uint2*>(row) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
 }
 
 // RowsF for bf16 tiles that stay bf16 (16-byte accesses only)
@@ -629,12 +654,13 @@ struct Rows {
 };
 
 // A wave owns CW tiles of 16 value columns; a workgroup has DP / (16 CW) waves.
-template <int DP, int CW, bool LAG, bool SUMS, typename LDS>
-__device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const Sums* sm, LDS& lds) {
+template <int DP, int CW, bool LAG, bool SUMS, bool SHARED, typename LDS>
+__device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const Sums* sm, LDS& lds, int b, int h, int seg) {
   constexpr int NW = DP / (16 * CW), NT = DP / 16, KS = DP / 32, MT = (10 + NW - 1) / NW;
   using R = Rows<DP, CW>;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, q4 = (lane >> 4) * 4;
-  const int seg = blockIdx.x % g.nseg, bh = blockIdx.x / g.nseg, b = bh / g.H, h = bh - b * g.H;
+  const int bh = b * g.H + h;
+  const Span sp = SUMS ? sm->sp : p->sp;
   const int n = valid_of(g, b), T = g.T;
   const float l2 = -g.rate[h] * 1.44269504088896340736f;
   const int Da = SUMS ? sm->Da : p->Da, Db = SUMS ? sm->Db : p->Db;
@@ -652,7 +678,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
   }
   const int col0 = 16 * CW * w;  // this wave's columns
   const int NC = (T + kC - 1) / kC;
-  const int ch0 = seg * g.cps, ch1 = ch0 + g.cps < NC ? ch0 + g.cps : NC;
+  const int ch0 = seg * sp.cps, ch1 = ch0 + sp.cps < NC ? ch0 + sp.cps : NC;
   const size_t dd = (size_t)Da * Db;
 
   v4f S[CW][NT], L[LAG ? CW : 1][LAG ? NT : 1];
@@ -666,14 +692,11 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
   char* out = nullptr;
   int64_t ost = 0;
   uint32_t ooff = 0;
-  bool o32 = false;
   if constexpr (!SUMS) {
-    o32 = p->out32;
-    const int esz = o32 ? 4 : 2;
-    ost = p->out.st * esz;
-    out = (char*)p->out.p + ((int64_t)b * p->out.sb + (int64_t)h * p->out.sh) * esz;
-    ooff = (uint32_t)((rev ? kC - 1 - c : c) * (int32_t)ost + (col0 + q4) * esz);
-    const float* s0 = p->seg ? p->seg + ((size_t)bh * g.nseg + seg) * p->nst * dd : p->init ? p->init + (size_t)bh * dd : nullptr;
+    ost = p->out.st * 2;
+    out = (char*)p->out.p + ((int64_t)b * p->out.sb + (int64_t)(h / p->out.group) * p->out.sh) * 2;
+    ooff = (uint32_t)((rev ? kC - 1 - c : c) * (int32_t)ost + (col0 + q4) * 2);
+    const float* s0 = p->seg ? p->seg + ((size_t)bh * sp.nseg + seg) * p->nst * dd : p->init ? p->init + (size_t)bh * dd : nullptr;
     const int ia = p->seg ? p->sga : p->ia, ib = p->seg ? p->sgb : p->ib;
     if (s0) {
 #pragma unroll
@@ -805,25 +828,39 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
       }
     }
     if constexpr (!SUMS) {
-      const int esz = o32 ? 4 : 2;
-      if (cnt == kC) {  // a whole chunk
+      if constexpr (SHARED) {  // the sum of the heads so far in fp32 rows
+        const int gi = h % p->G;
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const int i = base + 16 * it + c;
+          const bool live = i < n;
+          const int64_t t = rev && live ? n - 1 - i : i;
+#pragma unroll
+          for (int k = 0; k < CW; ++k) {
+            const int b0 = col0 + 16 * k + q4;
+            if (i >= T || b0 >= Db) continue;
+            const v4f o = add_part(p, live ? O[k][it] : v4f{0.f, 0.f, 0.f, 0.f}, ((int64_t)(bh / p->G) * T + t) * Db + b0, gi, b0, Db);
+            if (gi == p->G - 1) store4(out + t * ost + b0 * 2, o);
+          }
+        }
+      } else if (cnt == kC) {  // a whole chunk
         const int64_t step = rev ? -ost : ost;
         char* at = const_cast<char*>(chunk_src(out, ost, n, rev)) + base * step;
 #pragma unroll
         for (int it = 0; it < 4; ++it, at += 16 * step)
 #pragma unroll
           for (int k = 0; k < CW; ++k)
-            if (col0 + 16 * k + q4 < Db) store4(at + ooff + 16 * k * esz, O[k][it], o32);
+            if (col0 + 16 * k + q4 < Db) store4(at + ooff + 32 * k, O[k][it]);
       } else {
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
           const int i = base + 16 * it + c;
           const bool live = i < n;
-          char* at = out + (rev && live ? n - 1 - i : i) * ost + (col0 + q4) * esz;
+          char* at = out + (rev && live ? n - 1 - i : i) * ost + (col0 + q4) * 2;
 #pragma unroll
           for (int k = 0; k < CW; ++k) {
             if (!live) O[k][it] = v4f{0.f, 0.f, 0.f, 0.f};
-            if (i < T && col0 + 16 * k + q4 < Db) store4(at + 16 * k * esz, O[k][it], o32);
+            if (i < T && col0 + 16 * k + q4 < Db) store4(at + 32 * k, O[k][it]);
           }
         }
       }
@@ -870,11 +907,11 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
   }
   if constexpr (SUMS) {
 #pragma unroll
-    for (int k = 0; k < CW; ++k) write_sums<LAG>(g, sm, S[k], L[LAG ? k : 0], dd, Da, Db, col0 + 16 * k + c, q4, bh, seg);
+    for (int k = 0; k < CW; ++k) write_sums<LAG>(sm, S[k], L[LAG ? k : 0], dd, Da, Db, col0 + 16 * k + c, q4, bh, seg);
   } else {
 #pragma unroll
-    for (int k = 0; k < CW; ++k) dr += write_end<LAG>(g, p, S[k], L[LAG ? k : 0], dd, Da, Db, col0 + 16 * k + c, q4, bh, seg, n, l2);
-    if constexpr (LAG) write_drate<NW>(g, p, lds.red, dr, bh, seg);
+    for (int k = 0; k < CW; ++k) dr += write_end<LAG>(p, S[k], L[LAG ? k : 0], dd, Da, Db, col0 + 16 * k + c, q4, bh, seg, n, l2);
+    if constexpr (LAG) write_drate<NW>(p, lds.red, dr, bh, seg);
   }
 }
 
@@ -885,31 +922,43 @@ template <int DP, bool LAG, bool W16>
 constexpr int cw_of() { return W16 && DP == 128 && !LAG ? 2 : 1; }
 
 // LAG: the pass that carries the lag-weighted state, a launch of its own (its registers and LDS would bound the others).
-template <typename T, int DP, bool LAG, bool W16>
-__global__ __launch_bounds__((DP * 4 / cw_of<DP, LAG, W16>()), 2) void k_lattn(PassArgs a) {
-  if constexpr (W16) {
-    __shared__ __align__(16) Lds16<DP, LAG> lds;
-    lattn_body16<DP, cw_of<DP, LAG, W16>(), LAG, false>(a.g, &a.p[blockIdx.y], nullptr, lds);
+template <typename T, int DP, bool LAG, bool W16, bool SHARED>
+__global__ __launch_bounds__((DP * 4 / cw_of<DP, LAG, W16>()), (DP == 64 && !LAG ? 3 : 2)) void k_lattn(PassArgs a) {
+  __shared__ __align__(16) std::conditional_t<W16, Lds16<DP, LAG>, Lds<DP>> lds;
+  const Pass* p = &a.p[blockIdx.y];
+  const int seg = blockIdx.x % p->sp.nseg, u = blockIdx.x / p->sp.nseg;
+  auto body = [&](int b, int h) __attribute__((always_inline)) {
+    if constexpr (W16) lattn_body16<DP, cw_of<DP, LAG, W16>(), LAG, false, SHARED>(a.g, p, nullptr, lds, b, h, seg);
+    else lattn_body<T, DP, LAG, false, SHARED>(a.g, p, nullptr, lds, b, h, seg);
+  };
+  if constexpr (SHARED) {
+    const int U = a.g.H / p->G, b = u / U;
+    for (int gi = 0; gi < p->G; ++gi) body(b, (u - b * U) * p->G + gi);
   } else {
-    __shared__ __align__(16) Lds<DP> lds;
-    lattn_body<T, DP, LAG, false>(a.g, &a.p[blockIdx.y], nullptr, lds);
+    const int b = u / a.g.H;
+    if (b < a.g.B) body(b, u - b * a.g.H);  // (a launch is as wide as its widest pass)
   }
 }
+// (the last segment's sum is not needed)
 template <typename T, int DP, bool LAG, bool W16>
 __global__ __launch_bounds__(DP * 4) void k_lattn_sums(SumArgs a) {
+  __shared__ __align__(16) std::conditional_t<W16, LdsSums16<DP>, LdsSums<DP>> lds;
+  const Sums& z = a.s[blockIdx.y];
+  const int n = z.sp.nseg - 1;
+  if ((int)blockIdx.x >= a.g.B * a.g.H * n) return;
+  const int seg = blockIdx.x % n, bh = blockIdx.x / n, b = bh / a.g.H, h = bh - b * a.g.H;
   if constexpr (W16) {
-    __shared__ __align__(16) LdsSums16<DP> lds;
-    if (LAG && blockIdx.y == 0) lattn_body16<DP, 1, LAG, true>(a.g, nullptr, &a.s[0], lds);
-    else lattn_body16<DP, 1, false, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
+    if (LAG && blockIdx.y == 0) lattn_body16<DP, 1, LAG, true, false>(a.g, nullptr, &z, lds, b, h, seg);
+    else lattn_body16<DP, 1, false, true, false>(a.g, nullptr, &z, lds, b, h, seg);
   } else {
-    __shared__ __align__(16) LdsSums<DP> lds;
-    if (LAG && blockIdx.y == 0) lattn_body<T, DP, LAG, true>(a.g, nullptr, &a.s[0], lds);
-    else lattn_body<T, DP, false, true>(a.g, nullptr, &a.s[blockIdx.y], lds);
+    if (LAG && blockIdx.y == 0) lattn_body<T, DP, LAG, true, false>(a.g, nullptr, &z, lds, b, h, seg);
+    else lattn_body<T, DP, false, true, false>(a.g, nullptr, &z, lds, b, h, seg);
   }
 }
 
 // segment sums -> start states: seg[s] <- state in front of segment s
 struct ScanState {
+  Span sp;
   float* seg;
   const float* init;
   int32_t Da, Db, ia, ib, lag, rev;
@@ -921,26 +970,26 @@ struct ScanArgs {
 __global__ __launch_bounds__(256) void k_lattn_scan(ScanArgs a) {
   const ScanState& z = a.s[blockIdx.z];
   const int dd = z.Da * z.Db, e = blockIdx.x * 256 + threadIdx.x, bh = blockIdx.y;
-  if (e >= dd) return;
-  const int b = bh / a.g.H, h = bh - b * a.g.H, n = valid_of(a.g, b), len = a.g.cps * kC;
+  if (e >= dd || z.sp.nseg <= 1) return;
+  const int b = bh / a.g.H, h = bh - b * a.g.H, n = valid_of(a.g, b), len = z.sp.cps * kC;
   const float l2 = -a.g.rate[h] * 1.44269504088896340736f;
   const int nst = z.lag ? 2 : 1;
-  float* at = z.seg + (size_t)bh * a.g.nseg * nst * dd + e;
+  float* at = z.seg + (size_t)bh * z.sp.nseg * nst * dd + e;
   float S = z.init ? z.init[(size_t)bh * dd + (size_t)(e / z.Db) * z.ia + (size_t)(e % z.Db) * z.ib] : 0.f, L = 0.f;
   const size_t next = (size_t)nst * dd;
   constexpr int U = 8;  // sums in flight: the chain of states would wait for each of them in turn otherwise
-  for (int s0 = 0; s0 < a.g.nseg; s0 += U, at += U * next) {
+  for (int s0 = 0; s0 < z.sp.nseg; s0 += U, at += U * next) {
     float ls[U], ll[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool more = s0 + u + 1 < a.g.nseg;  // (the last segment's sum is not formed)
+      const bool more = s0 + u + 1 < z.sp.nseg;  // (the last segment's sum is not formed)
       ls[u] = more ? at[u * next] : 0.f;
       ll[u] = more && z.lag ? at[u * next + dd] : 0.f;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int s = s0 + u;
-      if (s >= a.g.nseg) break;
+      if (s >= z.sp.nseg) break;
       int cnt = n - s * len;
       cnt = cnt < 0 ? 0 : cnt < len ? cnt : len;
       at[u * next] = S;
@@ -952,42 +1001,6 @@ __global__ __launch_bounds__(256) void k_lattn_scan(ScanArgs a) {
   }
 }
 
-// gradients of shared key / value heads: sum over the query heads of a group, fp32 [B,H,T,D] -> rows of the type
-struct JoinArgs {
-  const float* part[2];
-  Mat out[2];
-  int32_t D[2];
-  int32_t B, H, Hk, T;
-};
-// memory-bound; four channels a thread where the rows allow it
-template <typename T>
-__global__ __launch_bounds__(256) void k_lattn_join(JoinArgs a) {
-  const int z = blockIdx.y, D = a.D[z], G = a.H / a.Hk;
-  const Mat& o = a.out[z];
-  const int V = o.vec ? 4 : 1;
-  const int per = D / V;
-  const int64_t n = (int64_t)a.T * per;
-  const int hk = blockIdx.z % a.Hk, b = blockIdx.z / a.Hk;
-  const float* part = a.part[z] + ((int64_t)b * a.H + (int64_t)hk * G) * a.T * D;
-  const int64_t hs = (int64_t)a.T * D;
-  T* out = (T*)o.p + (int64_t)b * o.sb + (int64_t)hk * o.sh;
-  for (int64_t r = blockIdx.x * 256 + threadIdx.x; r < n; r += gridDim.x * 256) {
-    const int64_t t = n < (1ll << 31) ? (uint32_t)r / (uint32_t)per : r / per;
-    const int j = (int)(r - t * per) * V;
-    const float* x = part + t * D + j;
-    T* y = out + t * o.st + j;
-    if (V == 4) {
-      v4f v = ld4(x);
-      for (int gi = 1; gi < G; ++gi) v += ld4(x + gi * hs);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) y[u] = ic_from_f<T>(v[u]);
-    } else {
-      float v = *x;
-      for (int gi = 1; gi < G; ++gi) v += x[gi * hs];
-      *y = ic_from_f<T>(v);
-    }
-  }
-}
 // d rate of a head: over sequences and segments, in 64 bits
 __global__ __launch_bounds__(64) void k_lattn_drate(const double* part, float* drate, int B, int H, int nseg) {
   const int h = blockIdx.x;
@@ -1080,14 +1093,10 @@ int pad_of(const ic_lattn_args* a) {
 // Segments of a sequence: the number for which the last of the launch's workgroups ends first, counted in chunks.  A chip of
 // 256 compute units holds `slots` workgroups at a time (LDS and registers: see the kernels); every round of them takes the
 // chunks of a segment and about one more (start state, first loads), and with more than one segment their sums come first,
-// at 0.4 of a chunk's time each.  (passes x B x H = 64, 64 chunks, 512 slots: 8 segments, 9.0 + 3.2 chunks against 65.)
-Geo geo_of(const ic_lattn_args* a, int passes, int slots) {
-  Geo g;
-  g.B = a->B; g.H = a->H; g.T = a->T;
-  g.rate = a->rate;
-  g.valid_len = a->valid_len;
-  const int NC = ic_ceil_div(a->T, kC);
-  const int64_t bh = (int64_t)a->B * a->H, have = bh * passes;
+// at 0.4 of a chunk's time each.  (64 sequences and heads of 64 chunks, 512 slots: 8 segments, 9.0 + 3.2 chunks against 65.)
+Span span_of(int T, int64_t have, int slots) {
+  Span g;
+  const int NC = ic_ceil_div(T, kC);
   double best = 0.0;
   g.nseg = 1;
   g.cps = NC;
@@ -1105,14 +1114,23 @@ Geo geo_of(const ic_lattn_args* a, int passes, int slots) {
   }
   return g;
 }
-// (bf16 rows that take the fp32 kernels for want of 16-byte accesses are planned like the others)
+// workgroups at a time (bf16 rows that take the fp32 kernels for want of 16-byte accesses are planned like the others)
 int slots_of(const ic_lattn_args* a, bool lag) {
   const int dp = pad_of(a);
-  return 256 * (dp == 32 ? 4 : dp == 64 ? 2 : a->dtype == IC_DT_BF16 && !lag ? 2 : 1);
+  return 256 * (dp == 32 ? 4 : dp == 64 ? (lag ? 2 : 3) : a->dtype == IC_DT_BF16 && !lag ? 2 : 1);
 }
-Geo geo_fwd(const ic_lattn_args* a) { return geo_of(a, 1, slots_of(a, false)); }
-// (with d rate the dq pass is a launch of its own, and the smaller of the two)
-Geo geo_bwd(const ic_lattn_args* a, bool lag) { return geo_of(a, lag ? 1 : 3, slots_of(a, lag)); }
+Span span_fwd(const ic_lattn_args* a) { return span_of(a->T, (int64_t)a->B * a->H, slots_of(a, false)); }
+// the dq pass, and the dv and dk passes, whose workgroups take all query heads of a key head
+Span span_q(const ic_lattn_args* a, bool lag) { return span_of(a->T, (int64_t)a->B * a->H, slots_of(a, lag)); }
+Span span_kv(const ic_lattn_args* a) { return span_of(a->T, 2 * (int64_t)a->B * a->Hk, slots_of(a, false)); }
+
+Geo geo_of(const ic_lattn_args* a) {
+  Geo g;
+  g.B = a->B; g.H = a->H; g.T = a->T;
+  g.rate = a->rate;
+  g.valid_len = a->valid_len;
+  return g;
+}
 
 Mat mat(const void* p, int64_t sb, int64_t sh, int64_t st, int group, int D, int esz) {
   Mat m;
@@ -1125,21 +1143,22 @@ Mat mat(const void* p, int64_t sb, int64_t sh, int64_t st, int group, int D, int
 }
 
 // floats of workspace: the segments' states (backward: the forward state and, for d rate, its lag-weighted companion, and the
-// reversed state), partial sums of d rate (doubles), partial gradients of shared heads
+// reversed state), partial sums of d rate (doubles), sums of shared heads' gradients
 int64_t ws_floats(const ic_lattn_args* a, int backward) {
   const int64_t bh = (int64_t)a->B * a->H, dd = (int64_t)a->Dk * a->Dv;
   if (!backward) {
-    const Geo g = geo_fwd(a);
-    return g.nseg > 1 ? bh * g.nseg * dd : 0;
+    const int ns = span_fwd(a).nseg;
+    return ns > 1 ? bh * ns * dd : 0;
   }
   int64_t n = 0;
   for (int lag = 0; lag < 2; ++lag) {  // (whether d rate is wanted is the call's matter, not the sizes')
-    const Geo g = geo_bwd(a, lag);
-    const int64_t m = (lag ? 2 * bh * g.nseg : 0) + (g.nseg > 1 ? bh * g.nseg * dd * (lag ? 3 : 2) : 0);
+    const int ns = span_q(a, lag).nseg;
+    const int64_t m = (lag ? 2 * bh * ns : 0) + (ns > 1 ? bh * ns * dd * (lag ? 2 : 1) : 0);
     n = n > m ? n : m;
   }
-  n += 2;
-  if (a->H != a->Hk) n += bh * a->T * (int64_t)(a->Dk + a->Dv) + 8;
+  const int nr = span_kv(a).nseg;
+  n += (nr > 1 ? bh * nr * dd : 0) + 2;
+  if (a->H != a->Hk) n += (int64_t)a->B * a->Hk * a->T * (a->Dk + a->Dv) + 8;
   return n;
 }
 
@@ -1173,24 +1192,25 @@ extern "C" int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream) {
   IC_REQUIRE(a->ws || ws_floats(a, 0) == 0, "ic_lattn_fwd: NULL workspace");
   if ((rc = check_stride(a->q_st, "ic_lattn_fwd", "q")) || (rc = check_stride(a->k_st, "ic_lattn_fwd", "k")) ||
       (rc = check_stride(a->v_st, "ic_lattn_fwd", "v")) || (rc = check_stride(a->o_st, "ic_lattn_fwd", "out"))) return rc;
-  const Geo g = geo_fwd(a);
+  const Geo g = geo_of(a);
+  const Span sp = span_fwd(a);
   const int esz = ic_dt_size(a->dtype), G = a->H / a->Hk, dp = pad_of(a), bh = a->B * a->H;
   hipStream_t st = (hipStream_t)stream;
   const Mat q = mat(a->q, a->q_sb, a->q_sh, a->q_st, 1, a->Dk, esz), k = mat(a->k, a->k_sb, a->k_sh, a->k_st, G, a->Dk, esz);
   const Mat v = mat(a->v, a->v_sb, a->v_sh, a->v_st, G, a->Dv, esz), o = mat(a->out, a->o_sb, a->o_sh, a->o_st, 1, a->Dv, esz);
   const bool wide = a->dtype == IC_DT_BF16 && q.vec && k.vec && v.vec && o.vec;
-  if (g.nseg > 1) {
+  if (sp.nseg > 1) {
     SumArgs s{};
     s.g = g;
-    s.s[0] = Sums{k, v, a->Dk, a->Dv, 0, 0, 1.f, a->ws};
-#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * g.nseg, 1), dim3(DP * 4), 0, st, s))
+    s.s[0] = Sums{k, v, sp, a->Dk, a->Dv, 0, 0, 1.f, a->ws};
+#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * (sp.nseg - 1)), dim3(DP * 4), 0, st, s))
 #define IC_BODY_T(T) IC_LATTN_DP(dp, T, IC_BODY)
     IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
     IC_LAUNCH_CHECK("ic_lattn_fwd");
     ScanArgs sc{};
     sc.g = g;
-    sc.s[0] = ScanState{a->ws, a->state, a->Dk, a->Dv, a->Dv, 1, 0, 0};
+    sc.s[0] = ScanState{sp, a->ws, a->state, a->Dk, a->Dv, a->Dv, 1, 0, 0};
     IC_TIMED(IC_KID_lattn_scan, st, hipLaunchKernelGGL(k_lattn_scan, dim3(ic_ceil_div(a->Dk * a->Dv, 256), bh, 1), dim3(256), 0, st, sc));
     IC_LAUNCH_CHECK("ic_lattn_fwd");
   }
@@ -1198,12 +1218,13 @@ extern "C" int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream) {
   p.g = g;
   Pass& f = p.p[0];
   f.q = q; f.k = k; f.v = v; f.out = o;
+  f.sp = sp; f.G = 1;
   f.Da = a->Dk; f.Db = a->Dv;
   f.oscale = a->scale; f.vscale = 1.f;
   f.init = a->state; f.ia = a->Dv; f.ib = 1;
   f.fin = a->state_out;
-  if (g.nseg > 1) { f.seg = a->ws; f.sga = a->Dv; f.sgb = 1; f.nst = 1; }
-#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_fwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false, W16>), dim3(bh * g.nseg, 1), dim3(DP * 4 / cw_of<DP, false, W16>()), 0, st, p))
+  if (sp.nseg > 1) { f.seg = a->ws; f.sga = a->Dv; f.sgb = 1; f.nst = 1; }
+#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_fwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false, W16, false>), dim3(bh * sp.nseg), dim3(DP * 4 / cw_of<DP, false, W16>()), 0, st, p))
   IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
   IC_LAUNCH_CHECK("ic_lattn_fwd");
@@ -1223,8 +1244,9 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
       (rc = check_stride(ba->dq_st, "ic_lattn_bwd", "dq")) || (rc = check_stride(ba->dk_st, "ic_lattn_bwd", "dk")) ||
       (rc = check_stride(ba->dv_st, "ic_lattn_bwd", "dv"))) return rc;
   const bool lag = ba->drate != nullptr;
-  const Geo g = geo_bwd(a, lag);
-  const int esz = ic_dt_size(a->dtype), G = a->H / a->Hk, dp = pad_of(a), bh = a->B * a->H, Dk = a->Dk, Dv = a->Dv;
+  const Geo g = geo_of(a);
+  const Span sq = span_q(a, lag), skv = span_kv(a);
+  const int esz = ic_dt_size(a->dtype), G = a->H / a->Hk, dp = pad_of(a), bh = a->B * a->H, bk = a->B * a->Hk, Dk = a->Dk, Dv = a->Dv;
   const int64_t dd = (int64_t)Dk * Dv;
   hipStream_t st = (hipStream_t)stream;
   const Mat q = mat(a->q, a->q_sb, a->q_sh, a->q_st, 1, Dk, esz), k = mat(a->k, a->k_sb, a->k_sh, a->k_st, G, Dk, esz);
@@ -1234,35 +1256,36 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
   const bool wide = a->dtype == IC_DT_BF16 && q.vec && k.vec && v.vec && o.vec && dq.vec && dk.vec && dv.vec;
   const int nst = lag ? 2 : 1;
   double* dr = (double*)a->ws;
-  float* seg_s = a->ws + (lag ? 2 * (int64_t)bh * g.nseg : 0);  // S (and L): transposed, [Dv][Dk]
-  float* seg_r = seg_s + (int64_t)bh * g.nseg * dd * nst;       // the reversed state, [Dk][Dv]
-  float* ws = g.nseg > 1 ? seg_r + (int64_t)bh * g.nseg * dd : seg_s;
-  ws += -(((uintptr_t)ws / 4)) & 3;  // (the partial gradients' rows on 16 bytes)
-  if (g.nseg > 1) {
+  float* seg_s = a->ws + (lag ? 2 * (int64_t)bh * sq.nseg : 0);                 // S (and L): transposed, [Dv][Dk]
+  float* seg_r = seg_s + (sq.nseg > 1 ? (int64_t)bh * sq.nseg * dd * nst : 0);  // the reversed state, [Dk][Dv]
+  float* part_k = seg_r + (skv.nseg > 1 ? (int64_t)bh * skv.nseg * dd : 0);
+  part_k += -((uintptr_t)part_k / 4) & 3;  // (rows on 16 bytes)
+  float* part_v = part_k + (((int64_t)bk * a->T * Dk + 3) & ~(int64_t)3);
+  const int nmax = sq.nseg > skv.nseg ? sq.nseg : skv.nseg;
+  if (nmax > 1) {
     SumArgs s{};
     s.g = g;
-    s.s[0] = Sums{v, k, Dv, Dk, 0, lag, 1.f, seg_s};
-    s.s[1] = Sums{q, o, Dk, Dv, 1, 0, a->scale, seg_r};
-#define IC_BODY(T, DP)                                                                                                                        \
-  if (lag) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, true, W16>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, s)); \
-  else IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * g.nseg, 2), dim3(DP * 4), 0, st, s))
+    s.s[0] = Sums{v, k, sq, Dv, Dk, 0, lag, 1.f, seg_s};
+    s.s[1] = Sums{q, o, skv, Dk, Dv, 1, 0, a->scale, seg_r};
+#define IC_BODY(T, DP)                                                                                                                                \
+  if (lag) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, true, W16>), dim3(bh * (nmax - 1), 2), dim3(DP * 4), 0, st, s)); \
+  else IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * (nmax - 1), 2), dim3(DP * 4), 0, st, s))
     IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
     IC_LAUNCH_CHECK("ic_lattn_bwd");
     ScanArgs sc{};
     sc.g = g;
-    sc.s[0] = ScanState{seg_s, a->state, Dv, Dk, 1, Dv, lag, 0};
-    sc.s[1] = ScanState{seg_r, ba->dstate_out, Dk, Dv, Dv, 1, 0, 1};
+    sc.s[0] = ScanState{sq, seg_s, a->state, Dv, Dk, 1, Dv, lag, 0};
+    sc.s[1] = ScanState{skv, seg_r, ba->dstate_out, Dk, Dv, Dv, 1, 0, 1};
     IC_TIMED(IC_KID_lattn_scan, st, hipLaunchKernelGGL(k_lattn_scan, dim3(ic_ceil_div(Dk * Dv, 256), bh, 2), dim3(256), 0, st, sc));
     IC_LAUNCH_CHECK("ic_lattn_bwd");
   }
-  float* part_k = ws;
-  float* part_v = ws + (int64_t)bh * a->T * Dk;
   PassArgs p{};
   p.g = g;
   Pass& pq = p.p[0];  // dq
   pq.q = o; pq.k = v; pq.v = k; pq.x = q;
   pq.out = dq;
+  pq.sp = sq; pq.G = 1;
   pq.Da = Dv; pq.Db = Dk;
   pq.oscale = a->scale; pq.vscale = 1.f;
   pq.init = a->state; pq.ia = 1; pq.ib = Dv;
@@ -1270,6 +1293,7 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
   pq.dr = dr;
   Pass& pv = p.p[1];  // dv
   pv.q = k; pv.k = q; pv.v = o; pv.out = dv;
+  pv.sp = skv; pv.G = G; pv.part = part_v;
   pv.Da = Dk; pv.Db = Dv;
   pv.rev = 1;
   pv.oscale = 1.f; pv.vscale = a->scale;
@@ -1277,52 +1301,37 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
   pv.fin = ba->dstate; pv.fin_decay = 1;
   Pass& pk = p.p[2];  // dk
   pk.q = v; pk.k = o; pk.v = q; pk.out = dk;
+  pk.sp = skv; pk.G = G; pk.part = part_k;
   pk.Da = Dv; pk.Db = Dk;
   pk.rev = 1;
   pk.oscale = 1.f; pk.vscale = a->scale;
   pk.init = ba->dstate_out; pk.ia = 1; pk.ib = Dv;
-  if (G > 1) {
-    pk.out = mat(part_k, (int64_t)a->H * a->T * Dk, (int64_t)a->T * Dk, Dk, 1, Dk, 4);
-    pv.out = mat(part_v, (int64_t)a->H * a->T * Dv, (int64_t)a->T * Dv, Dv, 1, Dv, 4);
-    pk.out32 = pv.out32 = 1;
-  }
-  if (g.nseg > 1) {
-    pq.seg = seg_s; pq.sga = Dk; pq.sgb = 1; pq.nst = nst;
+  if (sq.nseg > 1) { pq.seg = seg_s; pq.sga = Dk; pq.sgb = 1; pq.nst = nst; }
+  if (skv.nseg > 1) {
     pv.seg = seg_r; pv.sga = Dv; pv.sgb = 1; pv.nst = 1;
     pk.seg = seg_r; pk.sga = 1; pk.sgb = Dv; pk.nst = 1;
   }
-#define IC_LATTN_BWD(T, DP, LAG, PASSES, ARGS)                                                                                  \
-  IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, LAG, W16>), dim3(bh * g.nseg, PASSES),                      \
-                                                    dim3(DP * 4 / cw_of<DP, LAG, W16>()), 0, st, ARGS))
-#define IC_BODY(T, DP)                          \
-  if (!lag) {                                   \
-    IC_LATTN_BWD(T, DP, false, 3, p);           \
-  } else {                                      \
-    IC_LATTN_BWD(T, DP, true, 1, p);            \
-    PassArgs p1 = p;                            \
-    p1.p[0] = p.p[1];                           \
-    p1.p[1] = p.p[2];                           \
-    IC_LATTN_BWD(T, DP, false, 2, p1);          \
+  const int nq = bh * sq.nseg, nkv = bk * skv.nseg;
+  PassArgs pkv = p;
+  pkv.p[0] = p.p[1];
+  pkv.p[1] = p.p[2];
+#define IC_LATTN_BWD(T, DP, LAG, SHARED, GRID, ARGS) \
+  IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, LAG, W16, SHARED>), GRID, dim3(DP * 4 / cw_of<DP, LAG, W16>()), 0, st, ARGS))
+#define IC_BODY(T, DP)                                                              \
+  if (!lag && G == 1) {                                                             \
+    IC_LATTN_BWD(T, DP, false, false, dim3(nq > nkv ? nq : nkv, 3), p);             \
+  } else {                                                                          \
+    if (lag) { IC_LATTN_BWD(T, DP, true, false, dim3(nq), p); }                     \
+    else { IC_LATTN_BWD(T, DP, false, false, dim3(nq), p); }                        \
+    if (G == 1) { IC_LATTN_BWD(T, DP, false, false, dim3(nkv, 2), pkv); }           \
+    else { IC_LATTN_BWD(T, DP, false, true, dim3(nkv, 2), pkv); }                   \
   }
   IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
 #undef IC_LATTN_BWD
   IC_LAUNCH_CHECK("ic_lattn_bwd");
-  if (G > 1) {
-    JoinArgs j{};
-    j.part[0] = part_k; j.part[1] = part_v;
-    j.out[0] = dk; j.out[1] = dv;
-    j.D[0] = Dk; j.D[1] = Dv;
-    j.B = a->B; j.H = a->H; j.Hk = a->Hk; j.T = a->T;
-    const int64_t most = ((int64_t)a->T * (Dk > Dv ? Dk : Dv) + 2047) / 2048;  // (eight elements a thread)
-    const int blocks = (int)(most < 4096 ? most : 4096);
-#define IC_BODY(T) IC_TIMED(IC_KID_lattn_join, st, hipLaunchKernelGGL(k_lattn_join<T>, dim3(blocks, 2, a->B * a->Hk), dim3(256), 0, st, j));
-    IC_LATTN_T(a->dtype, false, IC_BODY);
-#undef IC_BODY
-    IC_LAUNCH_CHECK("ic_lattn_bwd");
-  }
   if (lag) {
-    IC_TIMED(IC_KID_lattn_join, st, hipLaunchKernelGGL(k_lattn_drate, dim3(a->H), dim3(64), 0, st, dr, ba->drate, a->B, a->H, g.nseg));
+    IC_TIMED(IC_KID_lattn_drate, st, hipLaunchKernelGGL(k_lattn_drate, dim3(a->H), dim3(64), 0, st, dr, ba->drate, a->B, a->H, sq.nseg));
     IC_LAUNCH_CHECK("ic_lattn_bwd");
   }
   return IC_OK;
