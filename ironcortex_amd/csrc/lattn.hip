@@ -534,8 +534,9 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
 // Rows that allow 16-byte accesses (others take the body above).
 // The same map on bf16 matrix instructions (16x16x32: sixteen times the fp32 rate).  Products of rows (q . k) are exact
 // there.  Operands that are computed in fp32 -- the decayed products P, the state, the decay-weighted values -- are split
-// into two bf16 parts (x = x1 + x2, x2 the rounded rest: 16 bits of the value; an error of at most 2^-18 of a term, 2^-20.5
-// in the mean square, where the outputs' own rounding is 2^-9 and the fp32 state keeps 20 bits of a sum of such terms).
+// into bf16 parts (x = x1 + x2 [+ x3], each the rounded rest of the one before, 8 bits apiece): two where the sum ends in a
+// bf16 output (2^-17 of a term at most, against the output's own 2^-9), three where it ends in an fp32 one, the state that
+// is carried on and d rate (with two the state was off by 2.4e-6 in the mean square, with fp32 products by 2e-7).
 // Rows lie in LDS as they come; column operands (k^T, v^T) are read with the transposing LDS load
 // (16 lanes x 8 bytes of four rows -> four rows of one column per lane).  A 32-deep operand of a lane is therefore k-indices
 // 4 q .. 4 q + 3 of either 16-row half, on both sides of a product; products of rows use contiguous eights instead.
@@ -591,17 +592,18 @@ __device__ __forceinline__ uint32_t take2(float& a, float& b) {
   b -= __uint_as_float(u & 0xffff0000u);
   return u;
 }
-__device__ __forceinline__ void split(float (&x)[8], b8 (&out)[2]) {
-  union { uint32_t u[4]; b8 b; } y, z;
+template <int N>
+__device__ __forceinline__ void split(float (&x)[8], b8 (&out)[N]) {
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    y.u[u] = take2(x[2 * u], x[2 * u + 1]);
-    z.u[u] = pack2(x[2 * u], x[2 * u + 1]);
+  for (int i = 0; i < N; ++i) {
+    union { uint32_t u[4]; b8 b; } y;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) y.u[u] = i + 1 < N ? take2(x[2 * u], x[2 * u + 1]) : pack2(x[2 * u], x[2 * u + 1]);
+    out[i] = y.b;
   }
-  out[0] = y.b;
-  out[1] = z.b;
 }
-__device__ __forceinline__ void split(const v4f& a, const v4f& b, b8 (&out)[2]) {
+template <int N>
+__device__ __forceinline__ void split(const v4f& a, const v4f& b, b8 (&out)[N]) {
   float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   split(x, out);
 }
@@ -653,10 +655,11 @@ struct Rows {
   }
 };
 
-// A wave owns CW tiles of 16 value columns; a workgroup has DP / (16 CW) waves.
-template <int DP, int CW, bool LAG, bool SUMS, bool SHARED, typename LDS>
+// A wave owns CW tiles of 16 value columns; a workgroup has DP / (16 CW) waves.  UP: parts of the values in the state's update.
+template <int DP, int CW, bool LAG, bool SUMS, bool SHARED, int UP, typename LDS>
 __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const Sums* sm, LDS& lds, int b, int h, int seg) {
   constexpr int NW = DP / (16 * CW), NT = DP / 16, KS = DP / 32, MT = (10 + NW - 1) / NW;
+  constexpr int RP = LAG ? 3 : 2;  // parts of the state where it is read
   using R = Rows<DP, CW>;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, q4 = (lane >> 4) * 4;
   const int bh = b * g.H + h;
@@ -781,7 +784,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
           }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          b8 sp[CW][2], lp[LAG ? CW : 1][2];
+          b8 sp[CW][RP], lp[LAG ? CW : 1][RP];
 #pragma unroll
           for (int k = 0; k < CW; ++k) {
             split(S[k][2 * s], S[k][2 * s + 1], sp[k]);
@@ -791,7 +794,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
           for (int it = 0; it < 4; ++it) {
             const b8 bq = lds8x2(&lds.Q.r[16 * it + c][32 * s + q4]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < RP; ++i)
 #pragma unroll
               for (int k = 0; k < CW; ++k) {
                 O[k][it] = mma32(sp[k][i], bq, O[k][it]);
@@ -876,7 +879,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
         }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        b8 vp[CW][2], lp[LAG ? CW : 1][2];
+        b8 vp[CW][UP], lp[LAG ? CW : 1][UP];
         const float* dl = &lds.dev[kC + cnt - 1 - q4 - 51];  // (51: the largest position of this lane's values)
 #pragma unroll
         for (int k = 0; k < CW; ++k) {
@@ -894,7 +897,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
         for (int t = 0; t < NT; ++t) {
           const b8 ak = lds_col(lds.K.r, 32 * s, 16 * t, lane);
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < UP; ++i)
 #pragma unroll
             for (int k = 0; k < CW; ++k) {
               S[k][t] = mma32(ak, vp[k][i], S[k][t]);
@@ -922,13 +925,14 @@ template <int DP, bool LAG, bool W16>
 constexpr int cw_of() { return W16 && DP == 128 && !LAG ? 2 : 1; }
 
 // LAG: the pass that carries the lag-weighted state, a launch of its own (its registers and LDS would bound the others).
-template <typename T, int DP, bool LAG, bool W16, bool SHARED>
+// UP: the reversed passes take two parts where only bf16 rows come of their state (three for dstate).
+template <typename T, int DP, bool LAG, bool W16, bool SHARED, int UP>
 __global__ __launch_bounds__((DP * 4 / cw_of<DP, LAG, W16>()), (DP == 64 && !LAG ? 3 : 2)) void k_lattn(PassArgs a) {
   __shared__ __align__(16) std::conditional_t<W16, Lds16<DP, LAG>, Lds<DP>> lds;
   const Pass* p = &a.p[blockIdx.y];
   const int seg = blockIdx.x % p->sp.nseg, u = blockIdx.x / p->sp.nseg;
   auto body = [&](int b, int h) __attribute__((always_inline)) {
-    if constexpr (W16) lattn_body16<DP, cw_of<DP, LAG, W16>(), LAG, false, SHARED>(a.g, p, nullptr, lds, b, h, seg);
+    if constexpr (W16) lattn_body16<DP, cw_of<DP, LAG, W16>(), LAG, false, SHARED, UP>(a.g, p, nullptr, lds, b, h, seg);
     else lattn_body<T, DP, LAG, false, SHARED>(a.g, p, nullptr, lds, b, h, seg);
   };
   if constexpr (SHARED) {
@@ -940,7 +944,7 @@ __global__ __launch_bounds__((DP * 4 / cw_of<DP, LAG, W16>()), (DP == 64 && !LAG
   }
 }
 // (the last segment's sum is not needed)
-template <typename T, int DP, bool LAG, bool W16>
+template <typename T, int DP, bool LAG, bool W16, int UP>
 __global__ __launch_bounds__(DP * 4) void k_lattn_sums(SumArgs a) {
   __shared__ __align__(16) std::conditional_t<W16, LdsSums16<DP>, LdsSums<DP>> lds;
   const Sums& z = a.s[blockIdx.y];
@@ -948,8 +952,8 @@ __global__ __launch_bounds__(DP * 4) void k_lattn_sums(SumArgs a) {
   if ((int)blockIdx.x >= a.g.B * a.g.H * n) return;
   const int seg = blockIdx.x % n, bh = blockIdx.x / n, b = bh / a.g.H, h = bh - b * a.g.H;
   if constexpr (W16) {
-    if (LAG && blockIdx.y == 0) lattn_body16<DP, 1, LAG, true, false>(a.g, nullptr, &z, lds, b, h, seg);
-    else lattn_body16<DP, 1, false, true, false>(a.g, nullptr, &z, lds, b, h, seg);
+    if (LAG && blockIdx.y == 0) lattn_body16<DP, 1, LAG, true, false, 3>(a.g, nullptr, &z, lds, b, h, seg);
+    else lattn_body16<DP, 1, false, true, false, UP>(a.g, nullptr, &z, lds, b, h, seg);
   } else {
     if (LAG && blockIdx.y == 0) lattn_body<T, DP, LAG, true, false>(a.g, nullptr, &z, lds, b, h, seg);
     else lattn_body<T, DP, false, true, false>(a.g, nullptr, &z, lds, b, h, seg);
@@ -1203,7 +1207,7 @@ extern "C" int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream) {
     SumArgs s{};
     s.g = g;
     s.s[0] = Sums{k, v, sp, a->Dk, a->Dv, 0, 0, 1.f, a->ws};
-#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * (sp.nseg - 1)), dim3(DP * 4), 0, st, s))
+#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16, 3>), dim3(bh * (sp.nseg - 1)), dim3(DP * 4), 0, st, s))
 #define IC_BODY_T(T) IC_LATTN_DP(dp, T, IC_BODY)
     IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
@@ -1224,7 +1228,7 @@ extern "C" int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream) {
   f.init = a->state; f.ia = a->Dv; f.ib = 1;
   f.fin = a->state_out;
   if (sp.nseg > 1) { f.seg = a->ws; f.sga = a->Dv; f.sgb = 1; f.nst = 1; }
-#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_fwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false, W16, false>), dim3(bh * sp.nseg), dim3(DP * 4 / cw_of<DP, false, W16>()), 0, st, p))
+#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_fwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false, W16, false, 3>), dim3(bh * sp.nseg), dim3(DP * 4 / cw_of<DP, false, W16>()), 0, st, p))
   IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
   IC_LAUNCH_CHECK("ic_lattn_fwd");
@@ -1267,11 +1271,14 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
     s.g = g;
     s.s[0] = Sums{v, k, sq, Dv, Dk, 0, lag, 1.f, seg_s};
     s.s[1] = Sums{q, o, skv, Dk, Dv, 1, 0, a->scale, seg_r};
-#define IC_BODY(T, DP)                                                                                                                                \
-  if (lag) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, true, W16>), dim3(bh * (nmax - 1), 2), dim3(DP * 4), 0, st, s)); \
-  else IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * (nmax - 1), 2), dim3(DP * 4), 0, st, s))
+#define IC_SUMS(T, DP, LAG, UP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, LAG, W16, UP>), dim3(bh * (nmax - 1), 2), dim3(DP * 4), 0, st, s))
+#define IC_BODY(T, DP)                                          \
+  if (lag && (ba->dstate || !W16)) { IC_SUMS(T, DP, true, 3); } \
+  else if (lag) { IC_SUMS(T, DP, true, (W16 ? 2 : 3)); }        \
+  else { IC_SUMS(T, DP, false, 3); }
     IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
+#undef IC_SUMS
     IC_LAUNCH_CHECK("ic_lattn_bwd");
     ScanArgs sc{};
     sc.g = g;
@@ -1315,19 +1322,23 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
   PassArgs pkv = p;
   pkv.p[0] = p.p[1];
   pkv.p[1] = p.p[2];
-#define IC_LATTN_BWD(T, DP, LAG, SHARED, GRID, ARGS) \
-  IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, LAG, W16, SHARED>), GRID, dim3(DP * 4 / cw_of<DP, LAG, W16>()), 0, st, ARGS))
+#define IC_LATTN_BWD(T, DP, LAG, SHARED, UP, GRID, ARGS) \
+  IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, LAG, W16, SHARED, UP>), GRID, dim3(DP * 4 / cw_of<DP, LAG, W16>()), 0, st, ARGS))
+#define IC_LATTN_KV(T, DP, UP)                                               \
+  if (G == 1) { IC_LATTN_BWD(T, DP, false, false, UP, dim3(nkv, 2), pkv); }  \
+  else { IC_LATTN_BWD(T, DP, false, true, UP, dim3(nkv, 2), pkv); }
 #define IC_BODY(T, DP)                                                              \
   if (!lag && G == 1) {                                                             \
-    IC_LATTN_BWD(T, DP, false, false, dim3(nq > nkv ? nq : nkv, 3), p);             \
+    IC_LATTN_BWD(T, DP, false, false, 3, dim3(nq > nkv ? nq : nkv, 3), p);          \
   } else {                                                                          \
-    if (lag) { IC_LATTN_BWD(T, DP, true, false, dim3(nq), p); }                     \
-    else { IC_LATTN_BWD(T, DP, false, false, dim3(nq), p); }                        \
-    if (G == 1) { IC_LATTN_BWD(T, DP, false, false, dim3(nkv, 2), pkv); }           \
-    else { IC_LATTN_BWD(T, DP, false, true, dim3(nkv, 2), pkv); }                   \
+    if (lag) { IC_LATTN_BWD(T, DP, true, false, 3, dim3(nq), p); }                  \
+    else { IC_LATTN_BWD(T, DP, false, false, 3, dim3(nq), p); }                     \
+    if (ba->dstate || !W16) { IC_LATTN_KV(T, DP, 3) }                               \
+    else { IC_LATTN_KV(T, DP, (W16 ? 2 : 3)) }                                      \
   }
   IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
+#undef IC_LATTN_KV
 #undef IC_LATTN_BWD
   IC_LAUNCH_CHECK("ic_lattn_bwd");
   if (lag) {
