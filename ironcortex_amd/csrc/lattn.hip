@@ -981,7 +981,8 @@ __global__ __launch_bounds__(256) void k_lattn_scan(ScanArgs a) {
   float* at = z.seg + (size_t)bh * z.sp.nseg * nst * dd + e;
   float S = z.init ? z.init[(size_t)bh * dd + (size_t)(e / z.Db) * z.ia + (size_t)(e % z.Db) * z.ib] : 0.f, L = 0.f;
   const size_t next = (size_t)nst * dd;
-  constexpr int U = 8;  // sums in flight: the chain of states would wait for each of them in turn otherwise
+  constexpr int U = 16;  // sums in flight: the chain of states would wait for each of them in turn otherwise
+  const float whole = decay(l2, len);
   for (int s0 = 0; s0 < z.sp.nseg; s0 += U, at += U * next) {
     float ls[U], ll[U];
 #pragma unroll
@@ -993,14 +994,15 @@ __global__ __launch_bounds__(256) void k_lattn_scan(ScanArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int s = s0 + u;
-      if (s >= z.sp.nseg) break;
-      int cnt = n - s * len;
-      cnt = cnt < 0 ? 0 : cnt < len ? cnt : len;
-      at[u * next] = S;
-      if (z.lag) at[u * next + dd] = L;
-      const float carry = decay(l2, cnt > 0 && z.rev && s == 0 ? cnt - 1 : cnt);
-      L = carry * (L + (float)cnt * S) + ll[u];
-      S = carry * S + ls[u];
+      if (s < z.sp.nseg) {
+        int cnt = n - s * len;
+        cnt = cnt < 0 ? 0 : cnt < len ? cnt : len;
+        at[u * next] = S;
+        if (z.lag) at[u * next + dd] = L;
+        const float carry = cnt == len && !(z.rev && s == 0) ? whole : decay(l2, cnt > 0 && z.rev && s == 0 ? cnt - 1 : cnt);
+        L = carry * (L + (float)cnt * S) + ll[u];
+        S = carry * S + ls[u];
+      }
     }
   }
 }
