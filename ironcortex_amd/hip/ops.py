@@ -1148,7 +1148,14 @@ def qk_norm_rope(q, k, q_weight, k_weight, *, eps: float = 1e-5, cos=None, sin=N
 # ---------------------------------------------------------------- linear attention with a decay for each head
 LATTN_MAX_D = 128        # channels of a head's keys and values
 LATTN_STEP_MAX_D = 1024  # the same for single positions
+LATTN_MAX_STRIDE = 1 << 22  # elements from position to position (64 of them are 32-bit offsets in the kernels)
 _pack_lattn, _pack_lattn_bwd, _pack_lattn_step = packer("ic_lattn_args")[0], packer("ic_lattn_bwd_args")[0], packer("ic_lattn_step_args")[0]
+
+
+def _rows_near(t: torch.Tensor) -> torch.Tensor:
+    """_rows4 whose positions lie near enough to each other."""
+    t = _rows4(t)
+    return t if t.stride(2) < LATTN_MAX_STRIDE else t.contiguous()
 
 
 def _lattn_values(q, k, v, rate, valid_len, state, scale, out=None, state_out=None, ws=None) -> tuple:
@@ -1203,7 +1210,7 @@ class LinearAttnFn(torch.autograd.Function):
         if gout is None and gstate is None:
             return (None,) * 7
         B, H, T, Dk = q.shape
-        gout = torch.zeros((B, H, T, v.shape[3]), dtype=q.dtype, device=q.device) if gout is None else _rows4(gout)
+        gout = torch.zeros((B, H, T, v.shape[3]), dtype=q.dtype, device=q.device) if gout is None else _rows_near(gout)
         gstate = None if gstate is None else gstate.contiguous()
         drate = torch.empty_like(rate) if ctx.needs_input_grad[3] else None
         dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
@@ -1256,7 +1263,7 @@ def linear_attention(q, k, v, rate, *, scale: float = 1.0, state=None, valid_len
     if B * H * T == 0:
         st = torch.zeros(B, H, Dk, v.shape[3], device=q.device) if state is None else state.clone()
         return q.new_empty(B, H, T, v.shape[3]) + 0 * (q.sum() + k.sum() + v.sum()), st
-    q, k, v, rate, state = _rows4(q), _rows4(k), _rows4(v), rate.contiguous(), None if state is None else state.contiguous()
+    q, k, v, rate, state = _rows_near(q), _rows_near(k), _rows_near(v), rate.contiguous(), None if state is None else state.contiguous()
     if _wants_grad(q, k, v, rate, state):
         return LinearAttnFn.apply(q, k, v, rate, state, valid_len, float(scale))
     return _lattn_run(q, k, v, rate, state, valid_len, float(scale))
@@ -1290,7 +1297,8 @@ def linear_attention_step(q, k, v, rate, state, *, scale: float = 1.0, active=No
     _launch("ic_lattn_step", _pack_lattn_step(
         B, H, k.shape[1], Dk, Dv, DTYPES[q.dtype], scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_sb, q_sh, k_sb, k_sh, v_sb, v_sh,
         rate.data_ptr(), _addr(active), state.data_ptr(), out.data_ptr(), H * Dv, Dv), q.device)
-    torch.autograd.graph.increment_version(state)
+    if not state.is_inference():  # (inference tensors keep no version)
+        torch.autograd.graph.increment_version(state)
     return out
 
 
