@@ -1107,9 +1107,8 @@ Span span_of(int T, int64_t have, int slots) {
   g.nseg = 1;
   g.cps = NC;
   const int64_t most = (2 * slots + have - 1) / have;
-  for (int ns = 1; ns <= most && ns <= NC; ++ns) {
-    const int cps = ic_ceil_div(NC, ns);
-    if (ic_ceil_div(NC, cps) != ns) continue;
+  for (int ns = 1, cps = NC; ns <= most; ns = ic_ceil_div(NC, --cps)) {  // each number of chunks that differs in its segments
+    cps = ic_ceil_div(NC, ns);
     const double rounds = (double)((have * ns + slots - 1) / slots);
     const double cost = rounds * (cps + 1.0) + (ns > 1 ? 0.4 * rounds * cps + 2.0 : 0.0);
     if (ns == 1 || cost < best) {
@@ -1117,6 +1116,7 @@ Span span_of(int T, int64_t have, int slots) {
       g.nseg = ns;
       g.cps = cps;
     }
+    if (cps == 1) break;
   }
   return g;
 }
