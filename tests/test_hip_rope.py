@@ -210,6 +210,18 @@ def test_rope_rotates_like_the_mixers_plain_formulation_bit_for_bit():
 
 
 @pytest.mark.gpu
+def test_mixer_rotates_other_types_as_before():
+    """Rows that promote with fp32 angles, fp64 rows, angles with a gradient: the plain formulation."""
+    from ironcortex_amd.mixer import rope_rotate_pairs, rotate_qk
+    th = torch.rand(2, 5, 4, device=DEV)
+    for q, c in ((torch.randn(2, 3, 5, 8, device=DEV).bfloat16(), torch.cos(th)), (torch.randn(2, 3, 5, 8, device=DEV).double(), torch.cos(th).double()),
+                 (torch.randn(2, 3, 5, 8, device=DEV), torch.cos(th).requires_grad_(True))):
+        a, b = rotate_qk(q, q, c, c)
+        w = rope_rotate_pairs(q, c.unsqueeze(1), c.unsqueeze(1), 4)
+        assert a.dtype == w.dtype and torch.equal(a, w) and torch.equal(b, w) and a.requires_grad == w.requires_grad
+
+
+@pytest.mark.gpu
 def test_rope_other_stream_empty_rows_and_not_finite_rows():
     from ironcortex_amd.hip import ops
     f = torch.ones(4, device=DEV)
