@@ -63,7 +63,7 @@ struct Pass {
 struct Sums {               // segment sums of one state
   Mat k, v;
   Span sp;
-  int32_t Da, Db, rev, lag;
+  int32_t Da, Db, rev;
   float vscale;
   float* seg;
 };
@@ -326,6 +326,18 @@ __device__ __forceinline__ void write_drate(const Pass* p, double* red, double d
   }
 }
 
+// O += v P^T for the tile on the diagonal, one position at a time and without what lies above: for values that are not all
+// finite
+__device__ __forceinline__ void add_diagonal(v4f& O, const v4f& v, const v4f& P, int c, int q4) {
+#pragma unroll 1
+  for (int j0 = 0; j0 < 16; j0 += 4)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const v4f o = mma(q4 == j0 ? v[u] : 0.f, P[u], O);
+      if (j0 + u <= c) O = o;
+    }
+}
+
 template <typename T, int DP, bool LAG, bool SUMS, bool SHARED, typename LDS>
 __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Sums* sm, LDS& lds, int b, int h, int seg) {
   constexpr int NT = DP * 4, NW = DP / 16, KS = DP / 16, MT = (10 + NW - 1) / NW;
@@ -397,6 +409,15 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
       if constexpr (!SUMS) {
         auto& Ps = lds.Ps;
         auto& Qs = lds.Qs;
+        bool finite = true;  // (0 * a value that is not would reach the rows in front of its own)
+        if constexpr (!LAG && !SHARED) {
+          float bad = 0.f;
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) bad = fmaf(v0[s][u], 0.f, bad);
+          finite = __all(bad == 0.f);
+        }
         v4f E[LAG ? 4 : 1];
         // P[i][j] = e^{-r(i-j)} q_i . k_j for the ten 16x16 tiles with a j <= i, formed transposed (rows j)
 #pragma unroll
@@ -436,6 +457,16 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
           if constexpr (LAG) E[it] = f * E[it] + (float)(16 * it + c + 1) * O[it];
         }
         __syncthreads();
+        if (!finite) {
+#pragma unroll
+          for (int it = 0; it < 4; ++it)
+#pragma unroll
+            for (int s = 0; s <= it; ++s) {
+              const v4f bp = ld4(&Ps[16 * it + c][16 * s + q4]);
+              if (s < it) O[it] = mma16(v0[s], bp, O[it]);
+              else add_diagonal(O[it], v0[s], bp, c, q4);
+            }
+        } else
 #pragma unroll
         for (int it = 0; it < 4; ++it)
 #pragma unroll
@@ -655,6 +686,25 @@ struct Rows {
   }
 };
 
+// O += P v by elements and without the products above the diagonal: for the chunks whose values are not all finite
+template <int CW, int W>
+__device__ __forceinline__ void add_rows_at_or_before(v4f (&O)[CW][4], const uint16_t (*P1)[kPw], const uint16_t (*P2)[kPw], const uint16_t (*V)[W], int cnt, int c, int b0) {
+#pragma unroll 1
+  for (int j = 0; j < cnt; ++j) {
+    const int at = 32 * (j >> 5) + 8 * ((j >> 2) & 3) + 4 * ((j >> 4) & 1) + (j & 3);
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const int i = 16 * it + c;
+      if (j > i) continue;
+      const float pj = __uint_as_float((uint32_t)P1[i][at] << 16) + __uint_as_float((uint32_t)P2[i][at] << 16);
+#pragma unroll
+      for (int k = 0; k < CW; ++k)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) O[k][it][v] = fmaf(pj, __uint_as_float((uint32_t)V[j][b0 + 16 * k + v] << 16), O[k][it][v]);
+    }
+  }
+}
+
 // A wave owns CW tiles of 16 value columns; a workgroup has DP / (16 CW) waves.  UP: parts of the values in the state's update.
 template <int DP, int CW, bool LAG, bool SUMS, bool SHARED, int UP, typename LDS>
 __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const Sums* sm, LDS& lds, int b, int h, int seg) {
@@ -817,7 +867,21 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
           }
         }
         if (LAG) dr -= (double)drc;
+        bool finite = true;  // (0 * a value that is not would reach the rows in front of its own)
+        if constexpr (!LAG && !SHARED) {
+          float bad = 0.f;
+#pragma unroll
+          for (int k = 0; k < CW; ++k)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int u = 0; u < 4; ++u) bad = __builtin_amdgcn_fdot2_f32_bf16((b2){vf[k][s][2 * u], vf[k][s][2 * u + 1]}, (b2){(__bf16)0.f, (__bf16)0.f}, bad, false);
+          finite = __all(bad == 0.f);
+        }
         __syncthreads();
+        if (!finite) {
+          add_rows_at_or_before(O, lds.P1, lds.P2, lds.V.r, cnt, c, col0 + q4);
+        } else
 #pragma unroll
         for (int it = 0; it < 4; ++it)
 #pragma unroll
@@ -1208,7 +1272,7 @@ extern "C" int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream) {
   if (sp.nseg > 1) {
     SumArgs s{};
     s.g = g;
-    s.s[0] = Sums{k, v, sp, a->Dk, a->Dv, 0, 0, 1.f, a->ws};
+    s.s[0] = Sums{k, v, sp, a->Dk, a->Dv, 0, 1.f, a->ws};
 #define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16, 3>), dim3(bh * (sp.nseg - 1)), dim3(DP * 4), 0, st, s))
 #define IC_BODY_T(T) IC_LATTN_DP(dp, T, IC_BODY)
     IC_LATTN_T(a->dtype, wide, IC_BODY_T);
@@ -1271,8 +1335,8 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
   if (nmax > 1) {
     SumArgs s{};
     s.g = g;
-    s.s[0] = Sums{v, k, sq, Dv, Dk, 0, lag, 1.f, seg_s};
-    s.s[1] = Sums{q, o, skv, Dk, Dv, 1, 0, a->scale, seg_r};
+    s.s[0] = Sums{v, k, sq, Dv, Dk, 0, 1.f, seg_s};
+    s.s[1] = Sums{q, o, skv, Dk, Dv, 1, a->scale, seg_r};
 #define IC_SUMS(T, DP, LAG, UP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, LAG, W16, UP>), dim3(bh * (nmax - 1), 2), dim3(DP * 4), 0, st, s))
 #define IC_BODY(T, DP)                                          \
   if (lag && (ba->dstate || !W16)) { IC_SUMS(T, DP, true, 3); } \

@@ -322,6 +322,39 @@ def test_linear_attention_in_captured_graphs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("Dk,Dv", [(32, 24), (64, 64), (128, 128), (33, 65)])
+def test_linear_attention_not_finite_rows_reach_only_what_follows(Dk, Dv, dtype):
+    """A value that is not finite, at a position t: the outputs in front of t are those of finite rows; where it is one of v's,
+    the other columns are, too."""
+    from ironcortex_amd.hip import ops
+    dt, B, T, H = TYPES[dtype], 4, 200, 2
+    g = torch.Generator(device=DEV).manual_seed(14)
+    rows = inputs(g, dt, B, T, H, 1, Dk, Dv, "tokens")
+    rate, scale = torch.tensor([0.0, 0.3], device=DEV), 0.25
+    n = torch.full((B,), T, device=DEV)
+    want, _ = recurrence(*(x.double() for x in rows), rate.double(), scale, None, n)
+    A, _ = recurrence(*(x.double().abs() for x in rows), rate.double(), scale, None, n)
+    b = bound(A, Dk + Dv + 160 + T / 64, dt, want)
+    for which in range(3):
+        for bad in (float("inf"), float("-inf"), float("nan")):
+            x = [r.clone() for r in rows]
+            at = (5, 70, 100, 191)
+            for i, t in enumerate(at):
+                x[which][i, -1, t, 3] = bad
+            got = ops.linear_attention(*x, rate, scale=scale)[0]
+            for i, t in enumerate(at):
+                within(got[i, :, :t], want[i, :, :t], b[i, :, :t], f"in front of {t}")
+                hit = got[i, -1, t, 3 if which == 2 else slice(None)]
+                assert not bool(torch.isfinite(hit).any())
+                if which == 0:  # a query is its own position's only
+                    within(got[i, :, t + 1:], want[i, :, t + 1:], b[i, :, t + 1:], "behind a query")
+                if which == 2:
+                    keep = [c for c in range(Dv) if c != 3]
+                    within(got[i][:, :, keep], want[i][:, :, keep], b[i][:, :, keep], "other columns")
+
+
+@pytest.mark.gpu
 def test_linear_attention_far_apart_positions_inference_mode_and_second_derivatives():
     from ironcortex_amd.hip import ops
     g = torch.Generator(device=DEV).manual_seed(13)
