@@ -364,6 +364,7 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
   }
   const int NC = (T_ + kC - 1) / kC;
   const int ch0 = seg * sp.cps, ch1 = ch0 + sp.cps < NC ? ch0 + sp.cps : NC;
+  const int nend = ch1 * kC < n ? ch1 * kC : n;  // the segment's end
   const size_t dd = (size_t)Da * Db;
 
   v4f S[KS], L[LAG ? KS : 1];
@@ -525,12 +526,16 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
         }
       }
     }
-    if (cnt > 0) {  // the state behind the chunk
-      const float carry = lds.dec[kC + cnt - off];
+    if (cnt > 0) {  // the state behind the chunk; a segment's sums weigh every position from the segment's end, with no carry
+      const int left = SUMS ? nend - base - cnt : 0;
+      const float ahead = SUMS ? decay(l2, left) : 1.f;
+      if constexpr (!SUMS) {
+        const float carry = lds.dec[kC + cnt - off];
 #pragma unroll
-      for (int t = 0; t < KS; ++t) {
-        if constexpr (LAG) L[t] = carry * (L[t] + (float)cnt * S[t]);
-        S[t] = carry * S[t];
+        for (int t = 0; t < KS; ++t) {
+          if constexpr (LAG) L[t] = carry * (L[t] + (float)cnt * S[t]);
+          S[t] = carry * S[t];
+        }
       }
       const float* dl = &lds.dev[kC + cnt - 1 - q4 - 51];  // (51: the largest position of this lane's values)
 #pragma unroll
@@ -538,8 +543,8 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
         v4f vw, vl;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          vw[u] = v0[s][u] * dl[51 - 16 * s - u];
-          if constexpr (LAG) vl[u] = vw[u] * (float)(cnt - 1 - q4 - 16 * s - u);  // (0 behind the last valid position)
+          vw[u] = v0[s][u] * (SUMS ? dl[51 - 16 * s - u] * ahead : dl[51 - 16 * s - u]);
+          if constexpr (LAG) vl[u] = vw[u] * (float)(left + cnt - 1 - q4 - 16 * s - u);  // (0 behind the last valid position)
         }
 #pragma unroll
         for (int t = 0; t < KS; ++t) {
@@ -732,6 +737,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
   const int col0 = 16 * CW * w;  // this wave's columns
   const int NC = (T + kC - 1) / kC;
   const int ch0 = seg * sp.cps, ch1 = ch0 + sp.cps < NC ? ch0 + sp.cps : NC;
+  const int nend = ch1 * kC < n ? ch1 * kC : n;  // the segment's end
   const size_t dd = (size_t)Da * Db;
 
   v4f S[CW][NT], L[LAG ? CW : 1][LAG ? NT : 1];
@@ -932,15 +938,19 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
         }
       }
     }
-    if (cnt > 0) {  // the state behind the chunk
-      const float carry = lds.dec[kC + cnt - off];
+    if (cnt > 0) {  // the state behind the chunk; a segment's sums weigh every position from the segment's end, with no carry
+      const int left = SUMS ? nend - base - cnt : 0;
+      const float ahead = SUMS ? decay(l2, left) : 1.f;
+      if constexpr (!SUMS) {
+        const float carry = lds.dec[kC + cnt - off];
 #pragma unroll
-      for (int k = 0; k < CW; ++k)
+        for (int k = 0; k < CW; ++k)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if constexpr (LAG) L[k][t] = carry * (L[k][t] + (float)cnt * S[k][t]);
-          S[k][t] = carry * S[k][t];
-        }
+          for (int t = 0; t < NT; ++t) {
+            if constexpr (LAG) L[k][t] = carry * (L[k][t] + (float)cnt * S[k][t]);
+            S[k][t] = carry * S[k][t];
+          }
+      }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         b8 vp[CW][UP], lp[LAG ? CW : 1][UP];
@@ -951,8 +961,8 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
             const int j = 32 * s + 16 * (u >> 2) + (u & 3);
-            x[u] = (float)vf[k][s][u] * dl[51 - j];
-            if constexpr (LAG) y[u] = x[u] * (float)(cnt - 1 - q4 - j);  // (0 behind the last valid position)
+            x[u] = (float)vf[k][s][u] * (SUMS ? dl[51 - j] * ahead : dl[51 - j]);
+            if constexpr (LAG) y[u] = x[u] * (float)(left + cnt - 1 - q4 - j);  // (0 behind the last valid position)
           }
           split(x, vp[k]);
           if constexpr (LAG) split(y, lp[k]);
