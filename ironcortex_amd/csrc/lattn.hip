@@ -9,18 +9,32 @@
 //   dq = (q, k, v) := (dout, v, k) with the transposed state;
 //   dv = (k, q, scale dout) and dk = (v, dout, scale q), both from the last position to the first, starting from the
 //   gradient of the final state; dstate is where that reversed recurrence ends.
-// So ONE kernel serves the forward (one pass) and the backward (three passes side by side in one launch).  Against a
-// kernel that forms all three gradients of a chunk at once it multiplies 12 tiles instead of 10, and needs neither the
-// state at every chunk's border in memory nor two states in registers.
+// So ONE kernel serves the forward (one pass) and the backward (three).  Against a kernel that forms all three gradients of a
+// chunk at once it multiplies 12 tiles instead of 10, and needs neither the state at every chunk's border in memory nor two
+// states in registers.  Gradients of shared key / value heads: a workgroup takes their query heads in turn and keeps the sum
+// in fp32 rows that only its own lanes touch (against a partial gradient for each query head and a joining launch: 550
+// instead of 564 us for a forward and backward of 8 x 4096 positions, 8 / 4 bf16 heads of 128, and half the workspace).
 // d rate: -d o / d rate weighs every pair by its lag.  The dq pass carries the lag-weighted state L = sum lag e^{-r lag}
 // k v^T next to S, and sums q_i . (lag-weighted dq_i): every term counted once with its own lag, where a difference of
 // position-weighted q . dq and k . dk would cancel to T times the rounding error.
 //
-// Work split: a workgroup owns (sequence, head, segment of chunks); a wave 16 of the value columns, with its [Dk,16] slice
+// Work split: a workgroup owns (sequence, head, segment of chunks); a wave 16 (or 32) of the value columns, with its slice
 // of the state in the accumulator registers, in the layout that the next product takes as its operand (16x16 tiles: lane
 // l holds rows 4 (l / 16) + 0..3 of column l % 16, and as an operand k-indices 4 (l / 16) + 0..3 of row / column l % 16).
-// Several segments per sequence only where sequences and heads do not fill the chip: their sums are formed first
-// (k_lattn SUMS), scanned (k_lattn_scan), and each segment starts from its own prefix.
+// Several segments per sequence only where sequences and heads do not fill the chip.  Their launches, in order: the sums of
+// all segments but the last (k_lattn_sums), the start states by a scan over them (k_lattn_scan), the pass itself (k_lattn).
+// The sums read k and v a second time; folding the scan into the pass's prologue was slower than its launch.
+//
+// Measured (microseconds; floors are the rows' bytes at the 4.76 TB/s of a large copy and the products at the 153 / 1201
+// TFLOP/s of large fp32 / bf16 matrix products):
+//   one document of 65536 positions, 8 bf16 heads of 128: sums 68 (3.9 TB/s), scan 18, pass 175 (3.1 TB/s); floor 113, and
+//     169 with k and v read twice.  Of the pass's time the matrix instructions are busy for 24%, vector arithmetic for 28%,
+//     half its waves' time waits (rows from memory, LDS round trips between the barriers).  Four waves a SIMD instead of two
+//     (one column tile a wave, 128 registers) spill: 240 us.
+//   forward and backward of 8 x 4096 positions, 8 / 4 bf16 heads of 128: forward 35 + 24 + 94; backward sums 81, scan 24, dq
+//     and d rate 195, dk and dv 215, d rate's sum 5.
+//   forward and backward of 16 x 1024 positions, 4 fp32 heads of 64: forward 14 + 8 + 28; backward 30 + 8 + 52 + 55 + 4; the
+//     products alone take 54 at the fp32 rate, and 2 chunks a workgroup leave half of a pass to its ends.
 #include <type_traits>
 
 #include "ic_types.h"
@@ -42,7 +56,7 @@ struct Span {
   int32_t nseg, cps;        // segments of a sequence, chunks of a segment
 };
 
-struct Pass {
+struct Pass {               // one application of the map
   Mat q, k, v, out, x;      // x: the rows that the lag-weighted output is multiplied with (d rate)
   Span sp;
   int32_t G;                // query heads whose outputs are one output (gradients of shared heads): a workgroup takes them in turn,
@@ -1034,7 +1048,8 @@ __global__ __launch_bounds__(DP * 4) void k_lattn_sums(SumArgs a) {
   }
 }
 
-// segment sums -> start states: seg[s] <- state in front of segment s
+// segment sums -> start states: seg[s] <- state in front of segment s.  A thread owns an element of a state; memory-bound but for
+// the ends of its chain (64 segments of 8 heads of 128 x 128: 67 MB in 18 us, 3.7 TB/s; with eight sums in flight 22.5 us).
 struct ScanState {
   Span sp;
   float* seg;
@@ -1090,7 +1105,8 @@ __global__ __launch_bounds__(64) void k_lattn_drate(const double* part, float* d
   if (threadIdx.x == 0) drate[h] = (float)v;
 }
 
-// One position.  Memory-bound: the state is read and written once.  A workgroup owns (sequence, head, 32 value columns):
+// One position.  Memory-bound: the state is read and written once (256 sequences, 16 heads of 128 x 128: 537 MB in 114 us, 4.7 TB/s,
+// a large copy's rate; a call for 4 heads of 64 x 64 costs its launch, 10 us).  A workgroup owns (sequence, head, 32 value columns):
 // 8 lanes x 4 columns, 32 rows of threads over the key channels; the output's sum over them goes through LDS.
 constexpr int kStepRows = 32;
 template <typename T>
@@ -1173,7 +1189,8 @@ int pad_of(const ic_lattn_args* a) {
 // Segments of a sequence: the number for which the last of the launch's workgroups ends first, counted in chunks.  A chip of
 // 256 compute units holds `slots` workgroups at a time (LDS and registers: see the kernels); every round of them takes the
 // chunks of a segment and about one more (start state, first loads), and with more than one segment their sums come first,
-// at 0.4 of a chunk's time each.  (64 sequences and heads of 64 chunks, 512 slots: 8 segments, 9.0 + 3.2 chunks against 65.)
+// at 0.4 of a chunk's time each.  (One sequence of 1024 chunks and 8 heads, 512 slots: 64 segments, 17 + 8.4 chunks against
+// 1025; 64 sequences and heads of 16 chunks, 768 slots: 8 segments of 2, 3 + 2.8 chunks against 17.)
 Span span_of(int T, int64_t have, int slots) {
   Span g;
   const int NC = ic_ceil_div(T, kC);
@@ -1194,7 +1211,9 @@ Span span_of(int T, int64_t have, int slots) {
   }
   return g;
 }
-// workgroups at a time (bf16 rows that take the fp32 kernels for want of 16-byte accesses are planned like the others)
+// Workgroups at a time: 32 channels 38 KB of LDS, 64 channels 53 KB and 168 registers (232 with the lag-weighted state), 128
+// channels 75 KB and 256 registers for bf16 rows, 86 KB for others.  (bf16 rows that take the fp32 kernels for want of
+// 16-byte accesses are planned like the rest of their type.)
 int slots_of(const ic_lattn_args* a, bool lag) {
   const int dp = pad_of(a);
   return 256 * (dp == 32 ? 4 : dp == 64 ? (lag ? 2 : 3) : a->dtype == IC_DT_BF16 && !lag ? 2 : 1);
