@@ -679,7 +679,7 @@ typedef struct ic_rope_rows {
   int32_t w_dtype;            /* IC_DT_* of w (and of the gradient gw) */
 } ic_rope_rows;
 typedef struct ic_rope_args {
-  int32_t B, T, D, m;         /* D <= 512; 2m <= D; B*T < 2^31 */
+  int32_t B, T, D, m;         /* D <= 512; 2m <= D; B*T < 2^31, < 2^26 for rows without 16-byte accesses */
   int32_t dtype, layout;      /* IC_DT_* of the rows, IC_ROPE_* */
   int32_t inverse;            /* 1: rotate by the negative angles (the transposed map); no norm then */
   int32_t pos64, freq64;      /* positions are int64 (else int32); freqs are fp64 (else fp32) */
@@ -721,7 +721,7 @@ int ic_rope_bwd(const ic_rope_bwd_args* b, ic_stream_t stream);
  * h reads key / value head h / (H / Hk).  A value that is not finite reaches its own and later positions and the state, no
  * earlier output; in the backward it may reach the gradients of every row of its chunk. */
 typedef struct ic_lattn_args {
-  int32_t B, H, Hk, T;        /* H % Hk == 0 */
+  int32_t B, H, Hk, T;        /* H % Hk == 0; B*H <= 2^22 */
   int32_t Dk, Dv;             /* 1 .. 128 */
   int32_t dtype;              /* IC_DT_* of q, k, v, out */
   float scale;
@@ -759,7 +759,7 @@ int ic_lattn_bwd(const ic_lattn_bwd_args* b, ic_stream_t stream);
  * active[b] == 0 keep their state and get zeros.  q [B,H,Dk], k [B,Hk,Dk], v [B,Hk,Dv], out [B,H,Dv] with strides over b
  * and h, state dense. */
 typedef struct ic_lattn_step_args {
-  int32_t B, H, Hk, Dk, Dv, dtype;
+  int32_t B, H, Hk, Dk, Dv, dtype;  /* B*H < 2^24; Dk, Dv 1 .. 1024 */
   float scale;
   const void* q;
   const void* k;

@@ -44,6 +44,7 @@ namespace {
 typedef float v4f __attribute__((ext_vector_type(4)));
 constexpr int kC = 64;
 constexpr int64_t kMaxStride = 1 << 22;  // elements from position to position
+constexpr int64_t kMaxHeads = 1 << 22;   // sequences * heads (a launch has fewer than 2^32 threads)
 
 struct Mat {  // rows [B,heads,T,D] of one of q, k, v, dout, ...
   void* p;
@@ -1062,7 +1063,7 @@ struct ScanArgs {
 };
 __global__ __launch_bounds__(256) void k_lattn_scan(ScanArgs a) {
   const ScanState& z = a.s[blockIdx.z];
-  const int dd = z.Da * z.Db, e = blockIdx.x * 256 + threadIdx.x, bh = blockIdx.y;
+  const int dd = z.Da * z.Db, e = blockIdx.y * 256 + threadIdx.x, bh = blockIdx.x;
   if (e >= dd || z.sp.nseg <= 1) return;
   const int b = bh / a.g.H, h = bh - b * a.g.H, n = valid_of(a.g, b), len = z.sp.cps * kC;
   const float l2 = -a.g.rate[h] * 1.44269504088896340736f;
@@ -1168,7 +1169,7 @@ int check_lattn(const ic_lattn_args* a, const char* who) {
   IC_REQUIRE(a != nullptr, "%s: NULL args", who);
   IC_REQUIRE(a->B >= 1 && a->H >= 1 && a->T >= 1, "%s: B=%d H=%d T=%d", who, a->B, a->H, a->T);
   IC_REQUIRE(a->Hk >= 1 && a->H % a->Hk == 0, "%s: H=%d is no multiple of Hk=%d", who, a->H, a->Hk);
-  IC_REQUIRE((int64_t)a->B * a->H <= 65535, "%s: B*H=%lld (at most 65535)", who, (long long)a->B * a->H);
+  IC_REQUIRE((int64_t)a->B * a->H <= kMaxHeads, "%s: B*H=%lld (at most 2^22)", who, (long long)a->B * a->H);
   IC_REQUIRE(a->T <= (1 << 30), "%s: T=%d (at most 2^30)", who, a->T);
   IC_REQUIRE(a->Dk >= 1 && a->Dk <= 128 && a->Dv >= 1 && a->Dv <= 128, "%s: Dk=%d Dv=%d (need 1 .. 128)", who, a->Dk, a->Dv);
   IC_REQUIRE(ic_dt_ok(a->dtype), "%s: dtype=%d", who, a->dtype);
@@ -1310,7 +1311,7 @@ extern "C" int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream) {
     ScanArgs sc{};
     sc.g = g;
     sc.s[0] = ScanState{sp, a->ws, a->state, a->Dk, a->Dv, a->Dv, 1, 0, 0};
-    IC_TIMED(IC_KID_lattn_scan, st, hipLaunchKernelGGL(k_lattn_scan, dim3(ic_ceil_div(a->Dk * a->Dv, 256), bh, 1), dim3(256), 0, st, sc));
+    IC_TIMED(IC_KID_lattn_scan, st, hipLaunchKernelGGL(k_lattn_scan, dim3(bh, ic_ceil_div(a->Dk * a->Dv, 256), 1), dim3(256), 0, st, sc));
     IC_LAUNCH_CHECK("ic_lattn_fwd");
   }
   PassArgs p{};
@@ -1379,7 +1380,7 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
     sc.g = g;
     sc.s[0] = ScanState{sq, seg_s, a->state, Dv, Dk, 1, Dv, lag, 0};
     sc.s[1] = ScanState{skv, seg_r, ba->dstate_out, Dk, Dv, Dv, 1, 0, 1};
-    IC_TIMED(IC_KID_lattn_scan, st, hipLaunchKernelGGL(k_lattn_scan, dim3(ic_ceil_div(Dk * Dv, 256), bh, 2), dim3(256), 0, st, sc));
+    IC_TIMED(IC_KID_lattn_scan, st, hipLaunchKernelGGL(k_lattn_scan, dim3(bh, ic_ceil_div(Dk * Dv, 256), 2), dim3(256), 0, st, sc));
     IC_LAUNCH_CHECK("ic_lattn_bwd");
   }
   PassArgs p{};
@@ -1445,7 +1446,7 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
 
 extern "C" int ic_lattn_step(const ic_lattn_step_args* a, ic_stream_t stream) {
   IC_REQUIRE(a != nullptr, "ic_lattn_step: NULL args");
-  IC_REQUIRE(a->B >= 1 && a->H >= 1 && (int64_t)a->B * a->H < (1ll << 31), "ic_lattn_step: B=%d H=%d", a->B, a->H);
+  IC_REQUIRE(a->B >= 1 && a->H >= 1 && (int64_t)a->B * a->H < (1ll << 24), "ic_lattn_step: B=%d H=%d (fewer than 2^24 together)", a->B, a->H);
   IC_REQUIRE(a->Hk >= 1 && a->H % a->Hk == 0, "ic_lattn_step: H=%d is no multiple of Hk=%d", a->H, a->Hk);
   IC_REQUIRE(a->Dk >= 1 && a->Dk <= 1024 && a->Dv >= 1 && a->Dv <= 1024, "ic_lattn_step: Dk=%d Dv=%d (need 1 .. 1024)", a->Dk, a->Dv);
   IC_REQUIRE(ic_dt_ok(a->dtype), "ic_lattn_step: dtype=%d", a->dtype);

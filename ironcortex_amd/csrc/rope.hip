@@ -425,6 +425,7 @@ extern "C" int ic_rope_fwd(const ic_rope_args* a, ic_stream_t stream) {
   const int mode = !vec ? M_ANY : a->layout == IC_ROPE_HALF ? M_HALF : M_INTER;
   int gx;
   const RopePlan p = plan_of(*a, mode, false, &gx);
+  IC_REQUIRE(gx < (1 << 24), "ic_rope_fwd: B=%d T=%d (a launch has fewer than 2^32 threads)", a->B, a->T);
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid(gx, p.nq + p.nk);
 #define IC_ROPE_FWD(T, NORM, PAST) IC_TIMED(IC_KID_rope_fwd, st, hipLaunchKernelGGL((k_rope_fwd<T, MODE, NORM, PAST>), grid, dim3(kThreads), 0, st, *a, p))

@@ -355,6 +355,32 @@ def test_linear_attention_not_finite_rows_reach_only_what_follows(Dk, Dv, dtype)
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 65])
+def test_linear_attention_many_sequences(T):
+    """More sequences and heads than a grid's second dimension holds; a piece of them gives the same rows."""
+    from ironcortex_amd.hip import ops
+    B, H, D = 17500, 4, 8
+    g = torch.Generator(device=DEV).manual_seed(15)
+    q, k, v = (torch.randn(B, T, H, D, generator=g, device=DEV).transpose(1, 2) for _ in range(3))
+    rate, st = torch.rand(H, generator=g, device=DEV), torch.randn(B, H, D, D, generator=g, device=DEV)
+    lo = B - 11
+
+    def run(*x):
+        x = [t.detach().requires_grad_(True) for t in x]
+        y, s = ops.linear_attention(x[0], x[1], x[2], rate, state=x[3])
+        return (y.detach(), s.detach(), *torch.autograd.grad((y.square().sum() + s.square().sum()), x))
+
+    for a, b in zip(run(q, k, v, st), run(q[lo:], k[lo:], v[lo:], st[lo:])):
+        # other segments: sums of 65 + 8 terms in another order, twice 73 * 2^-24 = 8.7e-6 of the terms' magnitudes
+        assert float((a[lo:] - b).abs().max()) <= 2e-5 * float(b.abs().max())
+    s2 = st.clone()
+    y = ops.linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], rate, s2)
+    y1, s1 = ops.linear_attention(q[:, :, :1], k[:, :, :1], v[:, :, :1], rate, state=st)
+    for a, b in ((y, y1[:, :, 0]), (s2, s1)):
+        assert float((a - b).abs().max()) <= 2e-5 * float(b.abs().max())
+
+
+@pytest.mark.gpu
 def test_linear_attention_far_apart_positions_inference_mode_and_second_derivatives():
     from ironcortex_amd.hip import ops
     g = torch.Generator(device=DEV).manual_seed(13)
@@ -418,7 +444,7 @@ def test_lattn_refuses_cpu_tensors_and_bad_arguments_of_the_c_entries():
     good = dict(B=1, H=2, Hk=1, T=5, Dk=8, Dv=8, dtype=0, q=8, k=8, v=8, rate=8, out=8)
     EINVAL = hip.ENUMS["IC_EINVAL"]
     for kw, text in ((dict(B=0), "B=0"), (dict(T=0), "T=0"), (dict(H=3, Hk=2), "Hk=2"), (dict(Hk=0), "Hk=0"), (dict(Dk=129), "Dk=129"), (dict(Dv=0), "Dv=0"),
-                     (dict(dtype=7), "dtype=7"), (dict(B=40000), "B*H"), (dict(q=None), "NULL"), (dict(rate=None), "NULL"), (dict(out=None), "NULL"),
+                     (dict(dtype=7), "dtype=7"), (dict(B=1 << 21, H=4), "B*H"), (dict(q=None), "NULL"), (dict(rate=None), "NULL"), (dict(out=None), "NULL"),
                      (dict(state=16, state_out=16), "state_out"), (dict(T=1000), "workspace"), (dict(k_st=1 << 22), "k has"), (dict(o_st=-(1 << 40)), "out has")):
         a = hip.new("ic_lattn_args", **{**good, **kw})
         assert lib.ic_lattn_fwd(ctypes.byref(a), None) == EINVAL and text in lib.ic_last_error().decode(), (kw, lib.ic_last_error())
