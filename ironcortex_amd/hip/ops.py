@@ -985,8 +985,9 @@ def _wants_grad(*ts) -> bool:
 
 
 def _angles(who, q, cos, sin, positions, freqs, layout, scale):
-    """Checked angles of a rotation -- tables cos / sin, or positions and frequencies -- as fields of ic_rope_args: (m, layout,
-    pos64, freq64, scale), (cos, sin, cs_sb, positions, pos_sb, freqs); and the tensors that hold them."""
+    """Checked angles of a rotation -- tables cos / sin, or positions and frequencies -- as fields of ic_rope_args: m, layout,
+    pos64, freq64, scale, elements from one sequence's table or positions to the next; and the tensors: (cos, sin), (freqs,) or
+    (freqs, positions)."""
     B, _, T, D = q.shape
     if layout not in ROPE_LAYOUTS:
         raise ValueError(f"{who}: layout {layout!r} (one of {sorted(ROPE_LAYOUTS)})")
@@ -1004,7 +1005,7 @@ def _angles(who, q, cos, sin, positions, freqs, layout, scale):
             raise RuntimeError(f"{who}: no gradient reaches the angles (cos, sin): detach them")
         m = cos.shape[-1]
         cos, sin = cos.contiguous(), sin.contiguous()
-        src = (cos.data_ptr(), sin.data_ptr(), T * m if cos.dim() == 3 and cos.shape[0] == B and B > 1 else 0, 0, 0, 0)
+        per = T * m if cos.dim() == 3 and cos.shape[0] == B and B > 1 else 0
         hold = (cos, sin)
     else:
         if freqs.dim() != 1 or freqs.dtype not in (torch.float32, torch.float64):
@@ -1014,17 +1015,17 @@ def _angles(who, q, cos, sin, positions, freqs, layout, scale):
         m = freqs.shape[0]
         freqs = freqs.contiguous()
         freq64 = int(freqs.dtype == torch.float64)
-        hold, src = (freqs,), (0, 0, 0, 0, 0, freqs.data_ptr())
+        hold, per = (freqs,), 0
         if positions is not None:
             if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((T,), (1, T), (B, T)):
                 raise ValueError(f"{who}: positions is {positions.dtype} {tuple(positions.shape)}, needs int32 or int64 [T], [1,T] or [B,T] with B={B}, T={T}")
             positions = positions.contiguous()
             pos64 = int(positions.dtype == torch.int64)
             hold = (freqs, positions)
-            src = (0, 0, 0, positions.data_ptr(), T if positions.dim() == 2 and positions.shape[0] == B and B > 1 else 0, freqs.data_ptr())
+            per = T if positions.dim() == 2 and positions.shape[0] == B and B > 1 else 0
     if 2 * m > D:
         raise ValueError(f"{who}: {m} rotated pairs do not fit rows of {D} channels")
-    return ((m, lay, pos64, freq64, float(scale)), src), hold
+    return (m, lay, pos64, freq64, float(scale), per, cos is not None), hold
 
 
 _NO_ROWS = (0,) * 11
@@ -1040,17 +1041,22 @@ def _rope_rows(x, y, w) -> tuple:
             0 if w is None else DTYPES[w.dtype])
 
 
-def _rope_values(ang, q, k, yq=None, yk=None, wq=None, wk=None, eps: float = 0.0, inverse: int = 0) -> tuple:
-    """ic_rope_args"""
-    (m, layout, pos64, freq64, scale), src = ang
+def _rope_values(ang, hold, q, k, yq=None, yk=None, wq=None, wk=None, eps: float = 0.0, inverse: int = 0) -> tuple:
+    """ic_rope_args.  The angles' addresses come from `hold` at every call: a backward's saved tensors may be others than the
+    forward's (torch's hooks for saved tensors, recomputation)."""
+    m, layout, pos64, freq64, scale, per, tables = ang
+    if tables:
+        src = (hold[0].data_ptr(), hold[1].data_ptr(), per, 0, 0, 0)
+    else:
+        src = (0, 0, 0, hold[1].data_ptr() if len(hold) > 1 else 0, per, hold[0].data_ptr())
     B, _, T, D = q.shape
     return (B, T, D, m, DTYPES[q.dtype], layout, inverse, pos64, freq64, scale, eps, *src, *_rope_rows(q, yq, wq), *_rope_rows(k, yk, wk))
 
 
-def _rope_run(ang, q, k, wq=None, wk=None, eps: float = 0.0):
+def _rope_run(ang, hold, q, k, wq=None, wk=None, eps: float = 0.0):
     yq = q.new_empty(q.shape)
     yk = None if k is None else k.new_empty(k.shape)
-    _launch("ic_rope_fwd", _pack_rope(*_rope_values(ang, q, k, yq, yk, wq, wk, eps)), q.device)
+    _launch("ic_rope_fwd", _pack_rope(*_rope_values(ang, hold, q, k, yq, yk, wq, wk, eps)), q.device)
     return yq, yk
 
 
@@ -1062,7 +1068,7 @@ class RopeFn(torch.autograd.Function):
         ctx.save_for_backward(*hold)  # (so that angles changed in place raise)
         ctx.ang = ang
         ctx.order = [_dense_order(t) for t in (q, k) if t is not None]
-        return _rope_run(ang, q, k)
+        return _rope_run(ang, hold, q, k)
 
     @_once
     def backward(ctx, gq, gk):
@@ -1070,7 +1076,7 @@ class RopeFn(torch.autograd.Function):
         gq, gk = _rows4(gq), _rows4(gk) if len(ctx.order) > 1 else None
         oq = gq.new_empty_strided(gq.shape, ctx.order[0])
         ok = None if gk is None else gk.new_empty_strided(gk.shape, ctx.order[1])
-        _launch("ic_rope_fwd", _pack_rope(*_rope_values(ctx.ang, gq, gk, oq, ok, inverse=1)), gq.device)
+        _launch("ic_rope_fwd", _pack_rope(*_rope_values(ctx.ang, hold, gq, gk, oq, ok, inverse=1)), gq.device)
         return (oq, ok, None) + (None,) * len(hold)
 
 
@@ -1082,7 +1088,7 @@ class QKNormRopeFn(torch.autograd.Function):
     def forward(ctx, q, k, wq, wk, ang, eps, *hold):
         ctx.save_for_backward(q, k, wq, wk, *hold)
         ctx.ang, ctx.eps = ang, eps
-        return _rope_run(ang, q, k, wq, wk, eps)
+        return _rope_run(ang, hold, q, k, wq, wk, eps)
 
     @_once
     def backward(ctx, gq, gk):
@@ -1095,7 +1101,7 @@ class QKNormRopeFn(torch.autograd.Function):
             outs.append(gx)
             gws.append(gw)
             keep.append(g)
-        _launch("ic_rope_bwd", _pack_rope_bwd(*_rope_values(ctx.ang, q, k, None, None, wq, wk, ctx.eps), *vals, part.data_ptr()), q.device)
+        _launch("ic_rope_bwd", _pack_rope_bwd(*_rope_values(ctx.ang, hold, q, k, None, None, wq, wk, ctx.eps), *vals, part.data_ptr()), q.device)
         return (*outs, *gws, None, None) + (None,) * len(hold)
 
 
@@ -1120,7 +1126,7 @@ def rope(q, k=None, *, cos=None, sin=None, positions=None, freqs=None, layout: s
     if q.numel() == 0 or (k is not None and k.numel() == 0):
         return (q.clone(), k.clone()) if k is not None else q.clone()
     q, k = _rows4(q), None if k is None else _rows4(k)
-    yq, yk = RopeFn.apply(q, k, ang, *hold) if _wants_grad(q, k) else _rope_run(ang, q, k)
+    yq, yk = RopeFn.apply(q, k, ang, *hold) if _wants_grad(q, k) else _rope_run(ang, hold, q, k)
     return yq if k is None else (yq, yk)
 
 
@@ -1142,12 +1148,13 @@ def qk_norm_rope(q, k, q_weight, k_weight, *, eps: float = 1e-5, cos=None, sin=N
     q, k, q_weight, k_weight = _rows4(q), _rows4(k), q_weight.contiguous(), k_weight.contiguous()
     if _wants_grad(q, k, q_weight, k_weight):
         return QKNormRopeFn.apply(q, k, q_weight, k_weight, ang, float(eps), *hold)
-    return _rope_run(ang, q, k, q_weight, k_weight, float(eps))
+    return _rope_run(ang, hold, q, k, q_weight, k_weight, float(eps))
 
 
 # ---------------------------------------------------------------- linear attention with a decay for each head
 LATTN_MAX_D = 128        # channels of a head's keys and values
 LATTN_STEP_MAX_D = 1024  # the same for single positions
+LATTN_MAX_HEADS = 1 << 22  # sequences * heads
 LATTN_MAX_STRIDE = 1 << 22  # elements from position to position (64 of them are 32-bit offsets in the kernels)
 _pack_lattn, _pack_lattn_bwd, _pack_lattn_step = packer("ic_lattn_args")[0], packer("ic_lattn_bwd_args")[0], packer("ic_lattn_step_args")[0]
 
@@ -1258,8 +1265,8 @@ def linear_attention(q, k, v, rate, *, scale: float = 1.0, state=None, valid_len
         if valid_len.shape != (B,) or valid_len.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"linear_attention: valid_len is {valid_len.dtype} {tuple(valid_len.shape)}, needs int32 or int64 [{B}]")
         valid_len = valid_len.clamp(0, T).to(torch.int32).contiguous() if valid_len.dtype == torch.int64 else valid_len.contiguous()
-    if B * H > 65535:
-        raise ValueError(f"linear_attention: B * H = {B * H} (at most 65535)")
+    if B * H > LATTN_MAX_HEADS:
+        raise ValueError(f"linear_attention: B * H = {B * H} (at most {LATTN_MAX_HEADS})")
     if B * H * T == 0:
         st = torch.zeros(B, H, Dk, v.shape[3], device=q.device) if state is None else state.clone()
         return q.new_empty(B, H, T, v.shape[3]) + 0 * (q.sum() + k.sum() + v.sum()), st

@@ -365,7 +365,8 @@ class DecayLinearAttention(nn.Module):
     def _qkv(self, x: torch.Tensor, positions: Optional[torch.Tensor]):
         """Normed and rotated q [B,H,T,hd], k [B,Hk,T,hd], and v [B,Hk,T,hd] of x [B,T,C]."""
         if self._freqs.device != x.device:
-            self._freqs = self._freqs.to(x.device)  # (fp64, and no buffer: module.bfloat16() must not round it)
+            with torch.inference_mode(False):  # (a tensor that a later training pass may save)
+                self._freqs = self._freqs.to(x.device)  # (fp64, and no buffer: module.bfloat16() must not round it)
         B, T, _ = x.shape
         H, Hk, hd = self.n_head, self.n_kv_head, self.head_dim
         q, k, v = (t.view(B, T, -1, hd).transpose(1, 2) for t in self.c_attn(x).split([H * hd, Hk * hd, Hk * hd], dim=2))

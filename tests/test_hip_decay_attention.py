@@ -116,6 +116,24 @@ def test_block_trains_in_bf16_and_keeps_its_frequencies():
     assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in att.parameters())
 
 
+def test_block_first_used_in_inference_mode_and_recomputed_in_training():
+    from torch.utils.checkpoint import checkpoint
+    att = module(n_kv_head=2)
+    x = torch.randn(2, 130, 96, device=DEV)
+    with torch.inference_mode():
+        y0, st = att(x)
+        att.step(x[:, 0], st, torch.full((2,), 130, device=DEV))
+    res = []
+    for f in (att, lambda *a: checkpoint(att, *a, use_reentrant=False)):
+        att.zero_grad(set_to_none=True)
+        xl = x.clone().requires_grad_(True)
+        y, s = f(xl, None, torch.arange(7, 137, device=DEV))
+        (y.square().sum() + s.sum()).backward()
+        res.append((y.detach(), s.detach(), xl.grad, *(p.grad for p in att.parameters())))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+    assert torch.equal(att(x)[0], y0)
+
+
 def test_rows_beyond_the_cache_equal_their_pieces():
     """168 MB of rows (written past the caches) against the same rows in pieces, bit for bit; the weights' gradients as sums of
     the pieces' within the rounding of sums of 2^16 terms."""

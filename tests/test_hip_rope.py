@@ -210,6 +210,36 @@ def test_rope_rotates_like_the_mixers_plain_formulation_bit_for_bit():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("tables", [False, True])
+def test_rope_backward_takes_the_saved_tensors_it_is_given(norm, tables):
+    """Tensors saved for the backward may come back as others (hooks, recomputation): the forward's angles are gone by then."""
+    from ironcortex_amd.hip import ops
+    g = torch.Generator(device=DEV).manual_seed(21)
+    B, H, T, D, m = 2, 3, 50, 32, 16
+    q, k = (torch.randn(B, n, T, D, generator=g, device=DEV).requires_grad_(True) for n in (H, 1))
+    w = [torch.rand(D, generator=g, device=DEV).requires_grad_(True) for _ in range(2)]
+    go = [torch.randn(B, n, T, D, generator=g, device=DEV) for n in (H, 1)]
+    leaves = [q, k] + (w if norm else [])
+
+    def angles():
+        if tables:
+            a = torch.arange(T, device=DEV).view(1, T, 1) * torch.linspace(0.1, 1.0, m, device=DEV) + torch.arange(B, device=DEV).view(B, 1, 1)
+            return dict(cos=torch.cos(a), sin=torch.sin(a))
+        return dict(positions=torch.arange(B * T, device=DEV).view(B, T), freqs=torch.linspace(0.1, 1.0, m, device=DEV, dtype=torch.float64))
+
+    def run():
+        y = ops.qk_norm_rope(q, k, *w, **angles()) if norm else ops.rope(q, k, **angles())
+        spoil = [torch.full((n,), float("nan"), device=DEV) for n in (B * T * m, B * T * m, 2 * B * T, 2 * m) for _ in range(4)]  # the angles' memory, reused
+        return torch.autograd.grad(y, leaves, go), spoil
+
+    want, _ = run()
+    with torch.autograd.graph.save_on_cpu():
+        got, _ = run()
+    assert all(bool(torch.isfinite(a).all()) and torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_mixer_rotates_other_types_as_before():
     """Rows that promote with fp32 angles, fp64 rows, angles with a gradient: the plain formulation."""
     from ironcortex_amd.mixer import rope_rotate_pairs, rotate_qk
