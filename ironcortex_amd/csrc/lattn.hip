@@ -136,10 +136,11 @@ struct RowsF {
     const int r = threadIdx.x / PER, c = (threadIdx.x % PER) * VE;
     off = (uint32_t)((rev ? kC - 1 - r : r) * (int32_t)st + c * (int)sizeof(T));
   }
-  // rows [base, base + cnt) (virtual positions); others read as zero
+  // rows [base, base + cnt) (virtual positions); others read as zero.  WHOLE: a whole chunk and `whole`
+  template <bool WHOLE>
   __device__ __forceinline__ void fetch(uint4 (&x)[NP], int base, int cnt) const {
     const char* at = src + base * step;
-    if (cnt == kC && whole) {
+    if constexpr (WHOLE) {
 #pragma unroll
       for (int j = 0; j < NP; ++j, at += RT * step) x[j] = *reinterpret_cast<const uint4*>(at + off);
       return;
@@ -195,9 +196,10 @@ struct ColsF {
     row0 = (rev ? kC - 1 : 0) * (int32_t)st + (in ? col : 0) * (int)sizeof(T);
     off = (uint32_t)(row0 + q4 * (int32_t)step);
   }
+  template <bool WHOLE>
   __device__ __forceinline__ void fetch(v4f (&x)[4], int base, int cnt) const {
     const char* at = src + base * step;
-    if (cnt == kC && whole) {
+    if constexpr (WHOLE) {
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -224,6 +226,14 @@ __device__ __forceinline__ v4f mma16(v4f a, v4f b, v4f c) {
   return c;
 }
 __device__ __forceinline__ v4f ld4(const float* p) { return *reinterpret_cast<const v4f*>(p); }
+
+// table[0], table[-1], ...: together and for every lane (left alone, the compiler puts each behind a branch of its own where
+// only some lanes use it, and waits for each)
+__device__ __forceinline__ void load_decays(float (&d)[4], const float* table) {
+#pragma unroll
+  for (int v = 0; v < 4; ++v) d[v] = table[-v];
+  asm volatile("" : "+v"(d[0]), "+v"(d[1]), "+v"(d[2]), "+v"(d[3]));
+}
 
 template <int DP>
 struct Lds {
@@ -401,11 +411,16 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
   double dr = 0.0;
   uint4 fk[R::NP], fq[SUMS ? 1 : R::NP];
   v4f vf[4];
+  // one branch for all rows: behind a join of two paths the next loads wait for those in flight
+  const bool whole = rk.whole && cv.whole && (SUMS || rq.whole);
+  auto fetch_as = [&](auto WHOLE, int base, int cnt) {
+    rk.template fetch<WHOLE.value>(fk, base, cnt);
+    if constexpr (!SUMS) rq.template fetch<WHOLE.value>(fq, base, cnt);
+    cv.template fetch<WHOLE.value>(vf, base, cnt);
+  };
   auto fetch = [&](int base) {
-    const int cnt = n - base < kC ? n - base : kC;
-    rk.fetch(fk, base, cnt);
-    if constexpr (!SUMS) rq.fetch(fq, base, cnt);
-    cv.fetch(vf, base, cnt);
+    if (n - base >= kC && whole) fetch_as(std::true_type(), base, kC);
+    else fetch_as(std::false_type(), base, n - base < kC ? n - base : kC);
   };
   if (ch0 * kC < n) fetch(ch0 * kC);
   for (int ch = ch0; ch < ch1; ++ch) {
@@ -445,10 +460,11 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
 #pragma unroll
           for (int s = 0; s < KS; ++s) acc = mma16(ld4(&Ks[16 * jt + c][16 * s + q4]), ld4(&Qs[16 * it + c][16 * s + q4]), acc);
           const int lag0 = 16 * (it - jt) + c - q4;
+          float d[4];
+          load_decays(d, &lds.dev[kC + lag0]);
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            const float d = lds.dev[kC + lag0 - v];
-            acc[v] = lag0 >= v ? acc[v] * (d * oscale) : 0.f;  // (a select: what lies above the diagonal may be infinite)
+            acc[v] = lag0 >= v ? acc[v] * (d[v] * oscale) : 0.f;  // (a select: what lies above the diagonal may be infinite)
           }
           *reinterpret_cast<v4f*>(&Ps[16 * it + c][16 * jt + q4]) = acc;
         }
@@ -683,11 +699,12 @@ struct Rows {
     whole = D == DP;
     off = (uint32_t)((rev ? kC - 1 - r : r) * (int32_t)st + c * 2);
   }
-  // rows [base, base + cnt) (virtual positions); others read as zero
+  // rows [base, base + cnt) (virtual positions); others read as zero.  WHOLE: a whole chunk and `whole`
+  template <bool WHOLE>
   __device__ __forceinline__ void fetch(uint4 (&x)[NP], int base, int cnt) const {
     const int r = threadIdx.x / (DP / 8);
     const char* at = src + base * step;
-    if (cnt == kC && whole) {  // (no lane left out)
+    if constexpr (WHOLE) {  // (no lane left out)
 #pragma unroll
       for (int j = 0; j < NP; ++j, at += RT * step) x[j] = *reinterpret_cast<const uint4*>(at + off);
       return;
@@ -790,12 +807,17 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
   }
   double dr = 0.0;
   uint4 fk[R::NP], fv[R::NP], fq[SUMS ? 1 : R::NP], fx[!SUMS && LAG ? R::NP : 1];
+  // one branch for all rows: behind a join of two paths the next loads wait for those in flight
+  const bool whole = rk.whole && rv.whole;
+  auto fetch_as = [&](auto WHOLE, int base, int cnt) {
+    rk.template fetch<WHOLE.value>(fk, base, cnt);
+    rv.template fetch<WHOLE.value>(fv, base, cnt);
+    if constexpr (!SUMS) rq.template fetch<WHOLE.value>(fq, base, cnt);
+    if constexpr (!SUMS && LAG) rx.template fetch<WHOLE.value>(fx, base, cnt);
+  };
   auto fetch = [&](int base) {
-    const int cnt = n - base < kC ? n - base : kC;
-    rk.fetch(fk, base, cnt);
-    rv.fetch(fv, base, cnt);
-    if constexpr (!SUMS) rq.fetch(fq, base, cnt);
-    if constexpr (!SUMS && LAG) rx.fetch(fx, base, cnt);
+    if (n - base >= kC && whole) fetch_as(std::true_type(), base, kC);
+    else fetch_as(std::false_type(), base, n - base < kC ? n - base : kC);
   };
   if (ch0 * kC < n) fetch(ch0 * kC);
   for (int ch = ch0; ch < ch1; ++ch) {
@@ -831,10 +853,11 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
           }
           float x[4];
           const int lag0 = 16 * (it - jt) + c - q4;
+          float d[4];
+          load_decays(d, &lds.dev[kC + lag0]);
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            const float d = lds.dev[kC + lag0 - v];
-            x[v] = lag0 >= v ? acc[v] * (d * oscale) : 0.f;  // (a select: what lies above the diagonal may be infinite)
+            x[v] = lag0 >= v ? acc[v] * (d[v] * oscale) : 0.f;  // (a select: what lies above the diagonal may be infinite)
             if constexpr (LAG) drc = lag0 > v ? fmaf((float)(lag0 - v) * x[v], ax[v], drc) : drc;
           }
           uint2 p1, p2;
