@@ -568,13 +568,14 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
           S[t] = carry * S[t];
         }
       }
-      const float* dl = &lds.dev[kC + cnt - 1 - q4 - 51];  // (51: the largest position of this lane's values)
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         v4f vw, vl;
+        float d[4];
+        load_decays(d, &lds.dev[kC + cnt - 1 - q4 - 16 * s]);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          vw[u] = v0[s][u] * (SUMS ? dl[51 - 16 * s - u] * ahead : dl[51 - 16 * s - u]);
+          vw[u] = v0[s][u] * (SUMS ? d[u] * ahead : d[u]);
           if constexpr (LAG) vl[u] = vw[u] * (float)(left + cnt - 1 - q4 - 16 * s - u);  // (0 behind the last valid position)
         }
 #pragma unroll
@@ -954,14 +955,13 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
             if (gi == p->G - 1) store4(out + t * ost + b0 * 2, o);
           }
         }
-      } else if (cnt == kC) {  // a whole chunk
+      } else if (cnt == kC && rv.whole) {  // a whole chunk
         const int64_t step = rev ? -ost : ost;
         char* at = const_cast<char*>(chunk_src(out, ost, n, rev)) + base * step;
 #pragma unroll
         for (int it = 0; it < 4; ++it, at += 16 * step)
 #pragma unroll
-          for (int k = 0; k < CW; ++k)
-            if (col0 + 16 * k + q4 < Db) store4(at + ooff + 32 * k, O[k][it]);
+          for (int k = 0; k < CW; ++k) store4(at + ooff + 32 * k, O[k][it]);
       } else {
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
