@@ -339,6 +339,14 @@ __device__ __forceinline__ v4f add_part(const Pass* p, v4f o, int64_t at, int gi
   }
   return o;
 }
+template <typename T>
+__device__ __forceinline__ void store_row4(char* row, const v4f& o) {
+  union { T e[4]; uint4 u4; uint2 u2; } x;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) x.e[v] = ic_from_f<T>(o[v]);
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(row) = x.u4;
+  else *reinterpret_cast<uint2*>(row) = x.u2;
+}
 template <int NW>
 __device__ __forceinline__ void write_drate(const Pass* p, double* red, double dr, int bh, int seg) {
   for (int o = 32; o; o >>= 1) dr += __shfl_xor(dr, o, 64);
@@ -406,6 +414,23 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
       if constexpr (LAG) {
         if (p->seg) load_state(L, s0 + dd, ia, ib, Da, Db, col, q4);
       }
+    }
+  }
+  const int b0 = 16 * w + q4;  // this lane's four columns of an output row
+  char* out = nullptr;
+  int64_t ost = 0, xst = 0;
+  uint32_t ooff = 0;
+  bool ovec = false, owhole = false;  // (uniform) 16- or 8-byte stores are allowed; no lane outside the row either
+  const T* x0 = nullptr;
+  if constexpr (!SUMS) {
+    ost = p->out.st * (int)sizeof(T);
+    out = (char*)const_cast<T*>(row_base<T>(p->out, b, h));
+    ooff = (uint32_t)((rev ? kC - 1 - c : c) * (int32_t)ost + b0 * (int)sizeof(T));
+    ovec = p->out.vec;
+    owhole = ovec && Db == DP;
+    if constexpr (LAG) {
+      xst = p->x.st;
+      x0 = row_base<T>(p->x, b, h);
     }
   }
   double dr = 0.0;
@@ -512,12 +537,10 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
             }
           }
         if constexpr (LAG) {
-          const int64_t xst = (rev ? -1 : 1) * p->x.st;
-          const T* x0 = row_base<T>(p->x, b, h) + (int64_t)(rev ? n - 1 : 0) * p->x.st;
 #pragma unroll
           for (int it = 0; it < 4; ++it) {
             const int i = 16 * it + c;
-            const T* x = x0 + (base + (i < cnt ? i : 0)) * xst;
+            const T* x = x0 + (base + (i < cnt ? i : 0)) * xst;  // (the lag-weighted pass is no reversed one)
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
               const float xv = ic_to_f(x[16 * w + q4 + v < Db ? 16 * w + q4 + v : 0]);
@@ -529,31 +552,32 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
       }
     }
     if constexpr (!SUMS) {
-      const int b0 = 16 * w + q4;  // this lane's four columns of a row
-      const int64_t ob = (int64_t)b * p->out.sb + (int64_t)(h / p->out.group) * p->out.sh;
-      const int gi = SHARED ? h % p->G : 0;
+      if (!SHARED && cnt == kC && owhole) {
+        const int64_t step = rev ? -ost : ost;
+        char* at = const_cast<char*>(chunk_src(out, ost, n, rev)) + base * step;
 #pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const int i = base + 16 * it + c;
-        if (i >= T_ || b0 >= Db) continue;
-        const bool live = i < n;
-        const int64_t t = rev && live ? n - 1 - i : i;
-        v4f o = live ? O[it] : v4f{0.f, 0.f, 0.f, 0.f};
-        if constexpr (SHARED) {
-          o = add_part(p, o, ((int64_t)(bh / p->G) * T_ + t) * Db + b0, gi, b0, Db);
-          if (gi < p->G - 1) continue;
-        }
-        T* row = (T*)p->out.p + ob + t * p->out.st + b0;
-        if (p->out.vec) {
-          union { T e[4]; uint4 u4; uint2 u2; } x;
+        for (int it = 0; it < 4; ++it, at += 16 * step) store_row4<T>(at + ooff, O[it]);
+      } else {
+        const int gi = SHARED ? h % p->G : 0;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) x.e[v] = ic_from_f<T>(o[v]);
-          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(row) = x.u4;
-          else *reinterpret_cast<uint2*>(row) = x.u2;
-        } else {
+        for (int it = 0; it < 4; ++it) {
+          const int i = base + 16 * it + c;
+          if (i >= T_ || b0 >= Db) continue;
+          const bool live = i < n;
+          const int64_t t = rev && live ? n - 1 - i : i;
+          v4f o = live ? O[it] : v4f{0.f, 0.f, 0.f, 0.f};
+          if constexpr (SHARED) {
+            o = add_part(p, o, ((int64_t)(bh / p->G) * T_ + t) * Db + b0, gi, b0, Db);
+            if (gi < p->G - 1) continue;
+          }
+          char* row = out + t * ost + b0 * (int)sizeof(T);
+          if (ovec) {
+            store_row4<T>(row, o);
+          } else {
 #pragma unroll
-          for (int v = 0; v < 4; ++v)
-            if (b0 + v < Db) row[v] = ic_from_f<T>(o[v]);
+            for (int v = 0; v < 4; ++v)
+              if (b0 + v < Db) ((T*)row)[v] = ic_from_f<T>(o[v]);
+          }
         }
       }
     }
