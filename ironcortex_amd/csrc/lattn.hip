@@ -12,8 +12,8 @@
 // So ONE kernel serves the forward (one pass) and the backward (three).  Against a kernel that forms all three gradients of a
 // chunk at once it multiplies 12 tiles instead of 10, and needs neither the state at every chunk's border in memory nor two
 // states in registers.  Gradients of shared key / value heads: a workgroup takes their query heads in turn and keeps the sum
-// in fp32 rows that only its own lanes touch (against a partial gradient for each query head and a joining launch: 550
-// instead of 564 us for a forward and backward of 8 x 4096 positions, 8 / 4 bf16 heads of 128, and half the workspace).
+// in fp32 rows that only its own lanes touch (against a partial gradient for each query head and a joining launch: 14 of
+// 564 us less for a forward and backward of 8 x 4096 positions, 8 / 4 bf16 heads of 128, and half the workspace).
 // d rate: -d o / d rate weighs every pair by its lag.  The dq pass carries the lag-weighted state L = sum lag e^{-r lag}
 // k v^T next to S, and sums q_i . (lag-weighted dq_i): every term counted once with its own lag, where a difference of
 // position-weighted q . dq and k . dk would cancel to T times the rounding error.
@@ -27,13 +27,14 @@
 //
 // Measured (microseconds; floors are the rows' bytes at the 4.76 TB/s of a large copy and the products at the 153 / 1201
 // TFLOP/s of large fp32 / bf16 matrix products):
-//   one document of 65536 positions, 8 bf16 heads of 128: sums 68 (3.9 TB/s), scan 18, pass 175 (3.1 TB/s); floor 113, and
-//     169 with k and v read twice.  Of the pass's time the matrix instructions are busy for 24%, vector arithmetic for 28%,
-//     half its waves' time waits (rows from memory, LDS round trips between the barriers).  Four waves a SIMD instead of two
-//     (one column tile a wave, 128 registers) spill: 240 us.
-//   forward and backward of 8 x 4096 positions, 8 / 4 bf16 heads of 128: forward 35 + 24 + 94; backward sums 81, scan 24, dq
-//     and d rate 195, dk and dv 215, d rate's sum 5.
-//   forward and backward of 16 x 1024 positions, 4 fp32 heads of 64: forward 14 + 8 + 28; backward 30 + 8 + 52 + 55 + 4; the
+//   one document of 65536 positions, 8 bf16 heads of 128: sums 69 (3.9 TB/s), scan 15, pass 163 (3.3 TB/s); floor 113, and
+//     169 with k and v read twice.  Of the pass's time the matrix instructions are busy for 30%, vector arithmetic for 35%,
+//     30% of its waves' time waits (LDS round trips between the barriers, rows from memory).  Four waves a SIMD instead of two
+//     (one column tile a wave, 128 registers) spill: 240 us.  K and V without bank conflicts in the products of rows (a third
+//     of the LDS time has them) cost a register that is not there: 165 us.
+//   forward and backward of 8 x 4096 positions, 8 / 4 bf16 heads of 128: forward 36 + 25 + 88; backward sums 80, scan 25, dq
+//     and d rate 182, dk and dv 210, d rate's sum 5.
+//   forward and backward of 16 x 1024 positions, 4 fp32 heads of 64: forward 14 + 9 + 27; backward 27 + 9 + 50 + 52 + 4; the
 //     products alone take 54 at the fp32 rate, and 2 chunks a workgroup leave half of a pass to its ends.
 #include <type_traits>
 
@@ -1097,7 +1098,7 @@ __global__ __launch_bounds__(DP * 4) void k_lattn_sums(SumArgs a) {
 }
 
 // segment sums -> start states: seg[s] <- state in front of segment s.  A thread owns an element of a state; memory-bound but for
-// the ends of its chain (64 segments of 8 heads of 128 x 128: 67 MB in 18 us, 3.7 TB/s; with eight sums in flight 22.5 us).
+// the ends of its chain (64 segments of 8 heads of 128 x 128: 67 MB in 15 us, 4.4 TB/s; with eight sums in flight 22.5 us).
 struct ScanState {
   Span sp;
   float* seg;
