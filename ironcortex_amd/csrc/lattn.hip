@@ -107,6 +107,22 @@ __device__ __forceinline__ int valid_of(const Geo& g, int b) {
 
 // e^{-rate * n}, n >= 0; n = 0 is 1 for every rate
 __device__ __forceinline__ float decay(float l2, int n) { return n == 0 ? 1.f : exp2f(l2 * (float)n); }
+// A state carried over n positions: e^{-rate n} x, as x + (e^{-rate n} - 1) x where more than half of it stays.  The factor itself,
+// rounded next to 1 and applied at every chunk, would leave a slowly decaying state off by that rounding times the number of
+// chunks; where little stays, the sum would cancel.
+struct Carry {
+  float f;
+  bool add;
+};
+__device__ __forceinline__ Carry carry_of(float rate, int n) {
+  const float x = n == 0 ? 0.f : -rate * (float)n, loss = expm1f(x);
+  Carry c;
+  c.add = loss > -0.5f;
+  c.f = c.add ? loss : expf(x);
+  return c;
+}
+__device__ __forceinline__ float carried(float x, Carry c) { return fmaf(c.f, x, c.add ? x : 0.f); }
+__device__ __forceinline__ v4f carried(const v4f& x, Carry c) { return v4f{carried(x[0], c), carried(x[1], c), carried(x[2], c), carried(x[3], c)}; }
 
 template <typename T>
 __device__ __forceinline__ const T* row_base(const Mat& m, int b, int h) {
@@ -381,7 +397,8 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
   const int bh = b * g.H + h;
   const Span sp = SUMS ? sm->sp : p->sp;
   const int n = valid_of(g, b), T_ = g.T;
-  const float l2 = -g.rate[h] * 1.44269504088896340736f;
+  const float rate = g.rate[h], l2 = -rate * 1.44269504088896340736f;
+  const Carry whole = carry_of(rate, kC);
   const int Da = SUMS ? sm->Da : p->Da, Db = SUMS ? sm->Db : p->Db;
   const int rev = SUMS ? sm->rev : p->rev;
   const float vscale = SUMS ? sm->vscale : p->vscale, oscale = SUMS ? 1.f : p->oscale;
@@ -438,14 +455,14 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
   uint4 fk[R::NP], fq[SUMS ? 1 : R::NP];
   v4f vf[4];
   // one branch for all rows: behind a join of two paths the next loads wait for those in flight
-  const bool whole = rk.whole && cv.whole && (SUMS || rq.whole);
+  const bool all = rk.whole && cv.whole && (SUMS || rq.whole);
   auto fetch_as = [&](auto WHOLE, int base, int cnt) {
     rk.template fetch<WHOLE.value>(fk, base, cnt);
     if constexpr (!SUMS) rq.template fetch<WHOLE.value>(fq, base, cnt);
     cv.template fetch<WHOLE.value>(vf, base, cnt);
   };
   auto fetch = [&](int base) {
-    if (n - base >= kC && whole) fetch_as(std::true_type(), base, kC);
+    if (n - base >= kC && all) fetch_as(std::true_type(), base, kC);
     else fetch_as(std::false_type(), base, n - base < kC ? n - base : kC);
   };
   if (ch0 * kC < n) fetch(ch0 * kC);
@@ -526,17 +543,21 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
             }
         } else
 #pragma unroll
-        for (int it = 0; it < 4; ++it)
+        for (int it = 0; it < 4; ++it) {
+          v4f o = v4f{0.f, 0.f, 0.f, 0.f}, e = o;  // (sums of their own: see the state's below)
 #pragma unroll
           for (int s = 0; s <= it; ++s) {
             v4f bp = ld4(&Ps[16 * it + c][16 * s + q4]);
-            O[it] = mma16(v0[s], bp, O[it]);
+            o = mma16(v0[s], bp, o);
             if constexpr (LAG) {
 #pragma unroll
               for (int u = 0; u < 4; ++u) bp[u] *= (float)(16 * (it - s) + c - q4 - u);  // (0 above the diagonal stays 0)
-              E[it] = mma16(v0[s], bp, E[it]);
+              e = mma16(v0[s], bp, e);
             }
           }
+          O[it] += o;
+          if constexpr (LAG) E[it] += e;
+        }
         if constexpr (LAG) {
 #pragma unroll
           for (int it = 0; it < 4; ++it) {
@@ -585,31 +606,39 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
     if (cnt > 0) {  // the state behind the chunk; a segment's sums weigh every position from the segment's end, with no carry
       const int left = SUMS ? nend - base - cnt : 0;
       const float ahead = SUMS ? decay(l2, left) : 1.f;
-      if constexpr (!SUMS) {
-        const float carry = lds.dec[kC + cnt - off];
+      const Carry over = SUMS || cnt - off == kC ? whole : carry_of(rate, cnt - off);
+      constexpr int HS = LAG && DP == 128 ? 1 : 2;
+      // A half chunk's own sum first, then one addition: a matrix instruction rounds after each of its products, and added to the
+      // state one by one each of the chunk's 64 would be rounded at the state's size (1024 positions of slow decay: state off by
+      // 5.1e-7 in the mean square, so 1.4e-7).
 #pragma unroll
-        for (int t = 0; t < KS; ++t) {
-          if constexpr (LAG) L[t] = carry * (L[t] + (float)cnt * S[t]);
-          S[t] = carry * S[t];
-        }
-      }
+      for (int s0 = 0; s0 < 4; s0 += HS) {
+        v4f vw[HS];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        v4f vw, vl;
-        float d[4];
-        load_decays(d, &lds.dev[kC + cnt - 1 - q4 - 16 * s]);
+        for (int s = 0; s < HS; ++s) {
+          float d[4];
+          load_decays(d, &lds.dev[kC + cnt - 1 - q4 - 16 * (s0 + s)]);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          vw[u] = v0[s][u] * (SUMS ? d[u] * ahead : d[u]);
-          if constexpr (LAG) vl[u] = vw[u] * (float)(left + cnt - 1 - q4 - 16 * s - u);  // (0 behind the last valid position)
+          for (int u = 0; u < 4; ++u) vw[s][u] = v0[s0 + s][u] * (SUMS ? d[u] * ahead : d[u]);
         }
 #pragma unroll
         for (int t = 0; t < KS; ++t) {
-          v4f ak;
+          v4f ds = v4f{0.f, 0.f, 0.f, 0.f}, dl = ds;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) ak[u] = Ks[16 * s + q4 + u][16 * t + c];
-          S[t] = mma16(ak, vw, S[t]);
-          if constexpr (LAG) L[t] = mma16(ak, vl, L[t]);
+          for (int s = 0; s < HS; ++s) {
+            v4f ak;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) ak[u] = Ks[16 * (s0 + s) + q4 + u][16 * t + c];
+            ds = mma16(ak, vw[s], ds);
+            if constexpr (LAG) {
+              v4f vl;
+#pragma unroll
+              for (int u = 0; u < 4; ++u) vl[u] = vw[s][u] * (float)(left + cnt - 1 - q4 - 16 * (s0 + s) - u);  // (0 behind the last valid position)
+              dl = mma16(ak, vl, dl);
+            }
+          }
+          if constexpr (LAG) L[t] = SUMS || s0 ? L[t] + dl : carried(L[t] + (float)cnt * S[t], over) + dl;
+          S[t] = SUMS || s0 ? S[t] + ds : carried(S[t], over) + ds;
         }
       }
       __syncthreads();
@@ -778,7 +807,8 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
   const int bh = b * g.H + h;
   const Span sp = SUMS ? sm->sp : p->sp;
   const int n = valid_of(g, b), T = g.T;
-  const float l2 = -g.rate[h] * 1.44269504088896340736f;
+  const float rate = g.rate[h], l2 = -rate * 1.44269504088896340736f;
+  const Carry whole = carry_of(rate, kC);
   const int Da = SUMS ? sm->Da : p->Da, Db = SUMS ? sm->Db : p->Db;
   const int rev = SUMS ? sm->rev : p->rev;
   const float vscale = SUMS ? sm->vscale : p->vscale, oscale = SUMS ? 1.f : p->oscale;
@@ -834,7 +864,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
   double dr = 0.0;
   uint4 fk[R::NP], fv[R::NP], fq[SUMS ? 1 : R::NP], fx[!SUMS && LAG ? R::NP : 1];
   // one branch for all rows: behind a join of two paths the next loads wait for those in flight
-  const bool whole = rk.whole && rv.whole;
+  const bool all = rk.whole && rv.whole;
   auto fetch_as = [&](auto WHOLE, int base, int cnt) {
     rk.template fetch<WHOLE.value>(fk, base, cnt);
     rv.template fetch<WHOLE.value>(fv, base, cnt);
@@ -842,7 +872,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
     if constexpr (!SUMS && LAG) rx.template fetch<WHOLE.value>(fx, base, cnt);
   };
   auto fetch = [&](int base) {
-    if (n - base >= kC && whole) fetch_as(std::true_type(), base, kC);
+    if (n - base >= kC && all) fetch_as(std::true_type(), base, kC);
     else fetch_as(std::false_type(), base, n - base < kC ? n - base : kC);
   };
   if (ch0 * kC < n) fetch(ch0 * kC);
@@ -1005,13 +1035,13 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
       const int left = SUMS ? nend - base - cnt : 0;
       const float ahead = SUMS ? decay(l2, left) : 1.f;
       if constexpr (!SUMS) {
-        const float carry = lds.dec[kC + cnt - off];
+        const Carry over = cnt - off == kC ? whole : carry_of(rate, cnt - off);
 #pragma unroll
         for (int k = 0; k < CW; ++k)
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            if constexpr (LAG) L[k][t] = carry * (L[k][t] + (float)cnt * S[k][t]);
-            S[k][t] = carry * S[k][t];
+            if constexpr (LAG) L[k][t] = carried(L[k][t] + (float)cnt * S[k][t], over);
+            S[k][t] = carried(S[k][t], over);
           }
       }
 #pragma unroll
@@ -1114,13 +1144,13 @@ __global__ __launch_bounds__(256) void k_lattn_scan(ScanArgs a) {
   const int dd = z.Da * z.Db, e = blockIdx.y * 256 + threadIdx.x, bh = blockIdx.x;
   if (e >= dd || z.sp.nseg <= 1) return;
   const int b = bh / a.g.H, h = bh - b * a.g.H, n = valid_of(a.g, b), len = z.sp.cps * kC;
-  const float l2 = -a.g.rate[h] * 1.44269504088896340736f;
+  const float rate = a.g.rate[h];
   const int nst = z.lag ? 2 : 1;
   float* at = z.seg + (size_t)bh * z.sp.nseg * nst * dd + e;
   float S = z.init ? z.init[(size_t)bh * dd + (size_t)(e / z.Db) * z.ia + (size_t)(e % z.Db) * z.ib] : 0.f, L = 0.f;
   const size_t next = (size_t)nst * dd;
   constexpr int U = 16;  // sums in flight: the chain of states would wait for each of them in turn otherwise
-  const float whole = decay(l2, len);
+  const Carry whole = carry_of(rate, len);
   for (int s0 = 0; s0 < z.sp.nseg; s0 += U, at += U * next) {
     float ls[U], ll[U];
 #pragma unroll
@@ -1137,9 +1167,9 @@ __global__ __launch_bounds__(256) void k_lattn_scan(ScanArgs a) {
         cnt = cnt < 0 ? 0 : cnt < len ? cnt : len;
         at[u * next] = S;
         if (z.lag) at[u * next + dd] = L;
-        const float carry = cnt == len && !(z.rev && s == 0) ? whole : decay(l2, cnt > 0 && z.rev && s == 0 ? cnt - 1 : cnt);
-        L = carry * (L + (float)cnt * S) + ll[u];
-        S = carry * S + ls[u];
+        const Carry over = cnt == len && !(z.rev && s == 0) ? whole : carry_of(rate, cnt > 0 && z.rev && s == 0 ? cnt - 1 : cnt);
+        L = carried(L + (float)cnt * S, over) + ll[u];
+        S = carried(S, over) + ls[u];
       }
     }
   }
