@@ -656,15 +656,17 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
 // Rows that allow 16-byte accesses (others take the body above).
 // The same map on bf16 matrix instructions (16x16x32: sixteen times the fp32 rate).  Products of rows (q . k) are exact
 // there.  Operands that are computed in fp32 -- the decayed products P, the state, the decay-weighted values -- are split
-// into bf16 parts (x = x1 + x2 [+ x3], each the rounded rest of the one before, 8 bits apiece): two where the sum ends in a
-// bf16 output (2^-17 of a term at most, against the output's own 2^-9), three where it ends in an fp32 one, the state that
-// is carried on and d rate (with two the state was off by 2.4e-6 in the mean square, with fp32 products by 2e-7).
+// into three bf16 parts (x = x1 + x2 + x3, each the rounded rest of the one before, 8 bits apiece), all of fp32's 24 bits.
 // Rows lie in LDS as they come; column operands (k^T, v^T) are read with the transposing LDS load
 // (16 lanes x 8 bytes of four rows -> four rows of one column per lane).  A 32-deep operand of a lane is therefore k-indices
 // 4 q .. 4 q + 3 of either 16-row half, on both sides of a product; products of rows use contiguous eights instead.
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef short s4v __attribute__((ext_vector_type(4)));
-constexpr int kPw = kC + 8;
+constexpr int kParts = 3;
+// P in LDS, three parts: rows of 32 positions in the upper half (the others lie above the diagonal), of 64 in the lower; 16 bytes
+// of padding a row
+constexpr int kPn = 32 * (32 + 8) + 32 * (64 + 8);
+__device__ __forceinline__ int p_row(int i) { return i < 32 ? 40 * i : 72 * i - 1024; }
 
 // padding: 32 bytes a row spread the 8 rows of a transposing read over the 64 banks, 16 bytes the 16 rows of a 16-byte read
 template <int W>
@@ -675,8 +677,8 @@ template <int DP, bool LAG>
 struct Lds16 {
   RowTile<DP + 16> K, V;
   RowTile<DP + 8> Q;
-  RowTile<LAG ? DP + 8 : 8> X;
-  uint16_t P1[kC][kPw], P2[kC][kPw];
+  RowTile<LAG ? DP + 8 : 1> X;
+  uint16_t P[kParts][kPn];
   float dec[2 * kC + 1], dev[2 * kC + 1];  // dec[kC + lag] = e^{-r lag}, 0 for lag < 0; dev = dec * vscale
   double red[DP / 16];
 };
@@ -780,7 +782,7 @@ struct Rows {
 
 // O += P v by elements and without the products above the diagonal: for the chunks whose values are not all finite
 template <int CW, int W>
-__device__ __forceinline__ void add_rows_at_or_before(v4f (&O)[CW][4], const uint16_t (*P1)[kPw], const uint16_t (*P2)[kPw], const uint16_t (*V)[W], int cnt, int c, int b0) {
+__device__ __forceinline__ void add_rows_at_or_before(v4f (&O)[CW][4], const uint16_t (*P)[kPn], const uint16_t (*V)[W], int cnt, int c, int b0) {
 #pragma unroll 1
   for (int j = 0; j < cnt; ++j) {
     const int at = 32 * (j >> 5) + 8 * ((j >> 2) & 3) + 4 * ((j >> 4) & 1) + (j & 3);
@@ -788,7 +790,8 @@ __device__ __forceinline__ void add_rows_at_or_before(v4f (&O)[CW][4], const uin
     for (int it = 0; it < 4; ++it) {
       const int i = 16 * it + c;
       if (j > i) continue;
-      const float pj = __uint_as_float((uint32_t)P1[i][at] << 16) + __uint_as_float((uint32_t)P2[i][at] << 16);
+      const int e = p_row(i) + at;
+      const float pj = __uint_as_float((uint32_t)P[0][e] << 16) + (__uint_as_float((uint32_t)P[1][e] << 16) + __uint_as_float((uint32_t)P[2][e] << 16));
 #pragma unroll
       for (int k = 0; k < CW; ++k)
 #pragma unroll
@@ -797,11 +800,10 @@ __device__ __forceinline__ void add_rows_at_or_before(v4f (&O)[CW][4], const uin
   }
 }
 
-// A wave owns CW tiles of 16 value columns; a workgroup has DP / (16 CW) waves.  UP: parts of the values in the state's update.
-template <int DP, int CW, bool LAG, bool SUMS, bool SHARED, int UP, typename LDS>
+// A wave owns CW tiles of 16 value columns; a workgroup has DP / (16 CW) waves.
+template <int DP, int CW, bool LAG, bool SUMS, bool SHARED, typename LDS>
 __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const Sums* sm, LDS& lds, int b, int h, int seg) {
   constexpr int NW = DP / (16 * CW), NT = DP / 16, KS = DP / 32, MT = (10 + NW - 1) / NW;
-  constexpr int RP = LAG ? 3 : 2;  // parts of the state where it is read
   using R = Rows<DP, CW>;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, q4 = (lane >> 4) * 4;
   const int bh = b * g.H + h;
@@ -857,8 +859,8 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
     // the two 16x16 tiles of P above the diagonal that a 32-deep product reads stay zero
     for (int i = threadIdx.x; i < 128; i += 64 * NW) {
       const int it = (i >> 6) << 1, r = i & 15, at = 32 * (it >> 1) + 8 * ((i >> 4) & 3) + 4;
-      *reinterpret_cast<uint64_t*>(&lds.P1[16 * it + r][at]) = 0;
-      *reinterpret_cast<uint64_t*>(&lds.P2[16 * it + r][at]) = 0;
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) *reinterpret_cast<uint64_t*>(&lds.P[k][p_row(16 * it + r) + at]) = 0;
     }
   }
   double dr = 0.0;
@@ -916,13 +918,14 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
             x[v] = lag0 >= v ? acc[v] * (d[v] * oscale) : 0.f;  // (a select: what lies above the diagonal may be infinite)
             if constexpr (LAG) drc = lag0 > v ? fmaf((float)(lag0 - v) * x[v], ax[v], drc) : drc;
           }
-          uint2 p1, p2;
-          p1.x = take2(x[0], x[1]);
-          p1.y = take2(x[2], x[3]);
-          p2 = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
-          const int at = 32 * (jt >> 1) + 2 * q4 + 4 * (jt & 1);  // the order in which a 32-deep operand of P is read
-          *reinterpret_cast<uint2*>(&lds.P1[16 * it + c][at]) = p1;
-          *reinterpret_cast<uint2*>(&lds.P2[16 * it + c][at]) = p2;
+          const int at = p_row(16 * it + c) + 32 * (jt >> 1) + 2 * q4 + 4 * (jt & 1);  // the order in which a 32-deep operand of P is read
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) {
+            uint2 y;
+            y.x = k + 1 < kParts ? take2(x[0], x[1]) : pack2(x[0], x[1]);
+            y.y = k + 1 < kParts ? take2(x[2], x[3]) : pack2(x[2], x[3]);
+            *reinterpret_cast<uint2*>(&lds.P[k][at]) = y;
+          }
         }
         v4f E[LAG ? CW : 1][4];
 #pragma unroll
@@ -934,7 +937,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
           }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          b8 sp[CW][RP], lp[LAG ? CW : 1][RP];
+          b8 sp[CW][kParts], lp[LAG ? CW : 1][kParts];
 #pragma unroll
           for (int k = 0; k < CW; ++k) {
             split(S[k][2 * s], S[k][2 * s + 1], sp[k]);
@@ -944,7 +947,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
           for (int it = 0; it < 4; ++it) {
             const b8 bq = lds8x2(&lds.Q.r[16 * it + c][32 * s + q4]);
 #pragma unroll
-            for (int i = 0; i < RP; ++i)
+            for (int i = 0; i < kParts; ++i)
 #pragma unroll
               for (int k = 0; k < CW; ++k) {
                 O[k][it] = mma32(sp[k][i], bq, O[k][it]);
@@ -980,17 +983,18 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
         }
         __syncthreads();
         if (!finite) {
-          add_rows_at_or_before(O, lds.P1, lds.P2, lds.V.r, cnt, c, col0 + q4);
+          add_rows_at_or_before(O, lds.P, lds.V.r, cnt, c, col0 + q4);
         } else
 #pragma unroll
         for (int it = 0; it < 4; ++it)
 #pragma unroll
           for (int s = 0; s <= it / 2; ++s) {
-            const b8 x1 = lds16(&lds.P1[16 * it + c][32 * s + 2 * q4]), x2 = lds16(&lds.P2[16 * it + c][32 * s + 2 * q4]);
 #pragma unroll
-            for (int k = 0; k < CW; ++k) O[k][it] = mma32(vf[k][s], x1, O[k][it]);
+            for (int i = 0; i < kParts; ++i) {
+              const b8 bp = lds16(&lds.P[i][p_row(16 * it + c) + 32 * s + 2 * q4]);
 #pragma unroll
-            for (int k = 0; k < CW; ++k) O[k][it] = mma32(vf[k][s], x2, O[k][it]);
+              for (int k = 0; k < CW; ++k) O[k][it] = mma32(vf[k][s], bp, O[k][it]);
+            }
           }
       }
     }
@@ -1034,19 +1038,10 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
     if (cnt > 0) {  // the state behind the chunk; a segment's sums weigh every position from the segment's end, with no carry
       const int left = SUMS ? nend - base - cnt : 0;
       const float ahead = SUMS ? decay(l2, left) : 1.f;
-      if constexpr (!SUMS) {
-        const Carry over = cnt - off == kC ? whole : carry_of(rate, cnt - off);
-#pragma unroll
-        for (int k = 0; k < CW; ++k)
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if constexpr (LAG) L[k][t] = carried(L[k][t] + (float)cnt * S[k][t], over);
-            S[k][t] = carried(S[k][t], over);
-          }
-      }
+      const Carry over = SUMS || cnt - off == kC ? whole : carry_of(rate, cnt - off);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        b8 vp[CW][UP], lp[LAG ? CW : 1][UP];
+        b8 vp[CW][kParts], lp[LAG ? CW : 1][kParts];
         const float* dl = &lds.dev[kC + cnt - 1 - q4 - 51];  // (51: the largest position of this lane's values)
 #pragma unroll
         for (int k = 0; k < CW; ++k) {
@@ -1064,12 +1059,16 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
         for (int t = 0; t < NT; ++t) {
           const b8 ak = lds_col(lds.K.r, 32 * s, 16 * t, lane);
 #pragma unroll
-          for (int i = 0; i < UP; ++i)
+          for (int k = 0; k < CW; ++k) {  // (a half chunk's own sum first, as for fp32 rows)
+            v4f ds = v4f{0.f, 0.f, 0.f, 0.f}, dl = ds;
 #pragma unroll
-            for (int k = 0; k < CW; ++k) {
-              S[k][t] = mma32(ak, vp[k][i], S[k][t]);
-              if constexpr (LAG) L[k][t] = mma32(ak, lp[k][i], L[k][t]);
+            for (int i = kParts - 1; i >= 0; --i) {
+              ds = mma32(ak, vp[k][i], ds);
+              if constexpr (LAG) dl = mma32(ak, lp[k][i], dl);
             }
+            if constexpr (LAG) L[k][t] = SUMS || s ? L[k][t] + dl : carried(L[k][t] + (float)cnt * S[k][t], over) + dl;
+            S[k][t] = SUMS || s ? S[k][t] + ds : carried(S[k][t], over) + ds;
+          }
         }
       }
       __syncthreads();
@@ -1092,14 +1091,13 @@ template <int DP, bool LAG, bool W16>
 constexpr int cw_of() { return W16 && DP == 128 && !LAG ? 2 : 1; }
 
 // LAG: the pass that carries the lag-weighted state, a launch of its own (its registers and LDS would bound the others).
-// UP: the reversed passes take two parts where only bf16 rows come of their state (three for dstate).
-template <typename T, int DP, bool LAG, bool W16, bool SHARED, int UP>
+template <typename T, int DP, bool LAG, bool W16, bool SHARED>
 __global__ __launch_bounds__((DP * 4 / cw_of<DP, LAG, W16>()), (DP == 64 && !LAG ? 3 : 2)) void k_lattn(PassArgs a) {
   __shared__ __align__(16) std::conditional_t<W16, Lds16<DP, LAG>, Lds<DP>> lds;
   const Pass* p = &a.p[blockIdx.y];
   const int seg = blockIdx.x % p->sp.nseg, u = blockIdx.x / p->sp.nseg;
   auto body = [&](int b, int h) __attribute__((always_inline)) {
-    if constexpr (W16) lattn_body16<DP, cw_of<DP, LAG, W16>(), LAG, false, SHARED, UP>(a.g, p, nullptr, lds, b, h, seg);
+    if constexpr (W16) lattn_body16<DP, cw_of<DP, LAG, W16>(), LAG, false, SHARED>(a.g, p, nullptr, lds, b, h, seg);
     else lattn_body<T, DP, LAG, false, SHARED>(a.g, p, nullptr, lds, b, h, seg);
   };
   if constexpr (SHARED) {
@@ -1111,7 +1109,7 @@ __global__ __launch_bounds__((DP * 4 / cw_of<DP, LAG, W16>()), (DP == 64 && !LAG
   }
 }
 // (the last segment's sum is not needed)
-template <typename T, int DP, bool LAG, bool W16, int UP>
+template <typename T, int DP, bool LAG, bool W16>
 __global__ __launch_bounds__(DP * 4) void k_lattn_sums(SumArgs a) {
   __shared__ __align__(16) std::conditional_t<W16, LdsSums16<DP>, LdsSums<DP>> lds;
   const Sums& z = a.s[blockIdx.y];
@@ -1119,8 +1117,8 @@ __global__ __launch_bounds__(DP * 4) void k_lattn_sums(SumArgs a) {
   if ((int)blockIdx.x >= a.g.B * a.g.H * n) return;
   const int seg = blockIdx.x % n, bh = blockIdx.x / n, b = bh / a.g.H, h = bh - b * a.g.H;
   if constexpr (W16) {
-    if (LAG && blockIdx.y == 0) lattn_body16<DP, 1, LAG, true, false, 3>(a.g, nullptr, &z, lds, b, h, seg);
-    else lattn_body16<DP, 1, false, true, false, UP>(a.g, nullptr, &z, lds, b, h, seg);
+    if (LAG && blockIdx.y == 0) lattn_body16<DP, 1, LAG, true, false>(a.g, nullptr, &z, lds, b, h, seg);
+    else lattn_body16<DP, 1, false, true, false>(a.g, nullptr, &z, lds, b, h, seg);
   } else {
     if (LAG && blockIdx.y == 0) lattn_body<T, DP, LAG, true, false>(a.g, nullptr, &z, lds, b, h, seg);
     else lattn_body<T, DP, false, true, false>(a.g, nullptr, &z, lds, b, h, seg);
@@ -1381,7 +1379,7 @@ extern "C" int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream) {
     SumArgs s{};
     s.g = g;
     s.s[0] = Sums{k, v, sp, a->Dk, a->Dv, 0, 1.f, a->ws};
-#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16, 3>), dim3(bh * (sp.nseg - 1)), dim3(DP * 4), 0, st, s))
+#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, false, W16>), dim3(bh * (sp.nseg - 1)), dim3(DP * 4), 0, st, s))
 #define IC_BODY_T(T) IC_LATTN_DP(dp, T, IC_BODY)
     IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
@@ -1402,7 +1400,7 @@ extern "C" int ic_lattn_fwd(const ic_lattn_args* a, ic_stream_t stream) {
   f.init = a->state; f.ia = a->Dv; f.ib = 1;
   f.fin = a->state_out;
   if (sp.nseg > 1) { f.seg = a->ws; f.sga = a->Dv; f.sgb = 1; f.nst = 1; }
-#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_fwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false, W16, false, 3>), dim3(bh * sp.nseg), dim3(DP * 4 / cw_of<DP, false, W16>()), 0, st, p))
+#define IC_BODY(T, DP) IC_TIMED(IC_KID_lattn_fwd, st, hipLaunchKernelGGL((k_lattn<T, DP, false, W16, false>), dim3(bh * sp.nseg), dim3(DP * 4 / cw_of<DP, false, W16>()), 0, st, p))
   IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
   IC_LAUNCH_CHECK("ic_lattn_fwd");
@@ -1445,11 +1443,10 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
     s.g = g;
     s.s[0] = Sums{v, k, sq, Dv, Dk, 0, 1.f, seg_s};
     s.s[1] = Sums{q, o, skv, Dk, Dv, 1, a->scale, seg_r};
-#define IC_SUMS(T, DP, LAG, UP) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, LAG, W16, UP>), dim3(bh * (nmax - 1), 2), dim3(DP * 4), 0, st, s))
-#define IC_BODY(T, DP)                                          \
-  if (lag && (ba->dstate || !W16)) { IC_SUMS(T, DP, true, 3); } \
-  else if (lag) { IC_SUMS(T, DP, true, (W16 ? 2 : 3)); }        \
-  else { IC_SUMS(T, DP, false, 3); }
+#define IC_SUMS(T, DP, LAG) IC_TIMED(IC_KID_lattn_sums, st, hipLaunchKernelGGL((k_lattn_sums<T, DP, LAG, W16>), dim3(bh * (nmax - 1), 2), dim3(DP * 4), 0, st, s))
+#define IC_BODY(T, DP)                    \
+  if (lag) { IC_SUMS(T, DP, true); }      \
+  else { IC_SUMS(T, DP, false); }
     IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
 #undef IC_SUMS
@@ -1496,23 +1493,19 @@ extern "C" int ic_lattn_bwd(const ic_lattn_bwd_args* ba, ic_stream_t stream) {
   PassArgs pkv = p;
   pkv.p[0] = p.p[1];
   pkv.p[1] = p.p[2];
-#define IC_LATTN_BWD(T, DP, LAG, SHARED, UP, GRID, ARGS) \
-  IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, LAG, W16, SHARED, UP>), GRID, dim3(DP * 4 / cw_of<DP, LAG, W16>()), 0, st, ARGS))
-#define IC_LATTN_KV(T, DP, UP)                                               \
-  if (G == 1) { IC_LATTN_BWD(T, DP, false, false, UP, dim3(nkv, 2), pkv); }  \
-  else { IC_LATTN_BWD(T, DP, false, true, UP, dim3(nkv, 2), pkv); }
-#define IC_BODY(T, DP)                                                              \
-  if (!lag && G == 1) {                                                             \
-    IC_LATTN_BWD(T, DP, false, false, 3, dim3(nq > nkv ? nq : nkv, 3), p);          \
-  } else {                                                                          \
-    if (lag) { IC_LATTN_BWD(T, DP, true, false, 3, dim3(nq), p); }                  \
-    else { IC_LATTN_BWD(T, DP, false, false, 3, dim3(nq), p); }                     \
-    if (ba->dstate || !W16) { IC_LATTN_KV(T, DP, 3) }                               \
-    else { IC_LATTN_KV(T, DP, (W16 ? 2 : 3)) }                                      \
+#define IC_LATTN_BWD(T, DP, LAG, SHARED, GRID, ARGS) \
+  IC_TIMED(IC_KID_lattn_bwd, st, hipLaunchKernelGGL((k_lattn<T, DP, LAG, W16, SHARED>), GRID, dim3(DP * 4 / cw_of<DP, LAG, W16>()), 0, st, ARGS))
+#define IC_BODY(T, DP)                                                           \
+  if (!lag && G == 1) {                                                          \
+    IC_LATTN_BWD(T, DP, false, false, dim3(nq > nkv ? nq : nkv, 3), p);          \
+  } else {                                                                       \
+    if (lag) { IC_LATTN_BWD(T, DP, true, false, dim3(nq), p); }                  \
+    else { IC_LATTN_BWD(T, DP, false, false, dim3(nq), p); }                     \
+    if (G == 1) { IC_LATTN_BWD(T, DP, false, false, dim3(nkv, 2), pkv); }        \
+    else { IC_LATTN_BWD(T, DP, false, true, dim3(nkv, 2), pkv); }                \
   }
   IC_LATTN_T(a->dtype, wide, IC_BODY_T);
 #undef IC_BODY
-#undef IC_LATTN_KV
 #undef IC_LATTN_BWD
   IC_LAUNCH_CHECK("ic_lattn_bwd");
   if (lag) {

@@ -101,3 +101,10 @@ def check_exactness(dtype, B, H, Hk, T, D):
 @pytest.mark.parametrize("B,H,Hk,T,D", [(96, 8, 8, 1024, 64), (48, 8, 4, 1024, 128)])
 def test_rows_on_fp32_products_are_as_exact_as_fp32_allows(dtype, B, H, Hk, T, D):
     check_exactness(dtype, B, H, Hk, T, D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hk,T,D", [(96, 8, 8, 1024, 64), (48, 8, 4, 1024, 128), (96, 8, 4, 1024, 32)])
+def test_bf16_rows_are_as_exact_as_fp32_products(B, H, Hk, T, D):
+    """Three bf16 parts of an fp32 operand hold all of its 24 bits, two of them 16."""
+    check_exactness("bf16", B, H, Hk, T, D)
