@@ -717,8 +717,8 @@ int ic_rope_bwd(const ic_rope_bwd_args* b, ic_stream_t stream);
  *   S_t = e^{-rate_h} S_{t-1} + k_t v_t^T,   o_t = scale * q_t^T S_t          (S_{-1} = state, zero if NULL)
  * for the positions t < valid_len[b]; rows behind that are written as zeros and leave the state alone.  Cost linear in T:
  * chunks of 64 positions on the matrix cores (fp32 accumulation), the state between chunks in fp32.
- * Rows may be strided (elements, fewer than 2^22 from position to position; the channels of a row are contiguous); query head
- * h reads key / value head h / (H / Hk).  A value that is not finite reaches its own and later positions and the state, no
+ * Rows may be strided (elements; from position to position 0 or more and fewer than 2^22; the channels of a row are contiguous);
+ * query head h reads key / value head h / (H / Hk).  A value that is not finite reaches its own and later positions and the state, no
  * earlier output; in the backward it may reach the gradients of every row of its chunk. */
 typedef struct ic_lattn_args {
   int32_t B, H, Hk, T;        /* H % Hk == 0; B*H <= 2^22 */

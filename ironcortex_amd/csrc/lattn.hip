@@ -1252,9 +1252,9 @@ int check_lattn(const ic_lattn_args* a, const char* who) {
   return IC_OK;
 }
 
-// 64 rows of a matrix lie within 2^31 bytes (the kernels' offsets inside a chunk)
+// 64 rows of a matrix lie within 2^31 bytes behind the first one (the kernels' offsets inside a chunk, unsigned)
 int check_stride(int64_t st, const char* who, const char* n) {
-  IC_REQUIRE(st > -kMaxStride && st < kMaxStride, "%s: %s has %lld elements from position to position (below %lld)", who, n, (long long)st, (long long)kMaxStride);
+  IC_REQUIRE(st >= 0 && st < kMaxStride, "%s: %s has %lld elements from position to position (0 to below %lld)", who, n, (long long)st, (long long)kMaxStride);
   return IC_OK;
 }
 
