@@ -1096,6 +1096,11 @@ class QKNormRopeFn(torch.autograd.Function):
         part = torch.empty(ROPE_PARTS * q.shape[3], device=q.device)
         vals, outs, gws, keep = [], [], [], []
         for x, w, g in ((q, wq, gq), (k, wk, gk)):  # ic_rope_grad
+            if x is None:
+                vals += (0,) * 9
+                outs.append(None)
+                gws.append(None)
+                continue
             g, gx, gw = _rows4(g), x.new_empty_strided(x.shape, _dense_order(x)), torch.empty_like(w)
             vals += (g.data_ptr(), gx.data_ptr(), gw.data_ptr(), *g.stride()[:3], *gx.stride()[:3])
             outs.append(gx)
@@ -1123,8 +1128,14 @@ def rope(q, k=None, *, cos=None, sin=None, positions=None, freqs=None, layout: s
     Returns dense [B,H,T,D] rows: the rotated q, or (q, k).  Gradients reach q and k."""
     _check_qk("rope", q, k)
     ang, hold = _angles("rope", q, cos, sin, positions, freqs, layout, scale)
-    if q.numel() == 0 or (k is not None and k.numel() == 0):
-        return (q.clone(), k.clone()) if k is not None else q.clone()
+    if q.numel() == 0:
+        return q.clone() if k is None else (q.clone(), k.clone() if k.numel() == 0 else _rope(k, None, ang, hold))
+    if k is not None and k.numel() == 0:  # (no heads)
+        return _rope(q, None, ang, hold), k.clone()
+    return _rope(q, k, ang, hold)
+
+
+def _rope(q, k, ang, hold):
     q, k = _rows4(q), None if k is None else _rows4(k)
     yq, yk = RopeFn.apply(q, k, ang, *hold) if _wants_grad(q, k) else _rope_run(ang, hold, q, k)
     return yq if k is None else (yq, yk)
@@ -1143,12 +1154,19 @@ def qk_norm_rope(q, k, q_weight, k_weight, *, eps: float = 1e-5, cos=None, sin=N
     if q.shape[1] + k.shape[1] > ROPE_PARTS:
         raise ValueError(f"qk_norm_rope: {q.shape[1]} + {k.shape[1]} heads (at most {ROPE_PARTS})")
     ang, hold = _angles("qk_norm_rope", q, cos, sin, positions, freqs, layout, scale)
-    if q.numel() == 0 or k.numel() == 0:
-        return q * q_weight.to(q.dtype), k * k_weight.to(k.dtype)
-    q, k, q_weight, k_weight = _rows4(q), _rows4(k), q_weight.contiguous(), k_weight.contiguous()
-    if _wants_grad(q, k, q_weight, k_weight):
-        return QKNormRopeFn.apply(q, k, q_weight, k_weight, ang, float(eps), *hold)
-    return _rope_run(ang, hold, q, k, q_weight, k_weight, float(eps))
+    if q.numel() and k.numel():
+        return _qk_norm_rope(q, k, q_weight, k_weight, ang, hold, float(eps))
+    return tuple(_qk_norm_rope(x, None, w, None, ang, hold, float(eps))[0] if x.numel() else x * w.to(x.dtype)  # (no heads, or no rows at all)
+                 for x, w in ((q, q_weight), (k, k_weight)))
+
+
+def _qk_norm_rope(q, k, wq, wk, ang, hold, eps):
+    q, wq = _rows4(q), wq.contiguous()
+    if k is not None:
+        k, wk = _rows4(k), wk.contiguous()
+    if _wants_grad(q, k, wq, wk):
+        return QKNormRopeFn.apply(q, k, wq, wk, ang, eps, *hold)
+    return _rope_run(ang, hold, q, k, wq, wk, eps)
 
 
 # ---------------------------------------------------------------- linear attention with a decay for each head
