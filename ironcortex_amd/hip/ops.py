@@ -1180,7 +1180,17 @@ _pack_lattn, _pack_lattn_bwd, _pack_lattn_step = packer("ic_lattn_args")[0], pac
 def _rows_near(t: torch.Tensor) -> torch.Tensor:
     """_rows4 whose positions lie near enough to each other."""
     t = _rows4(t)
-    return t if t.stride(2) < LATTN_MAX_STRIDE else t.contiguous()
+    if t.stride(2) < LATTN_MAX_STRIDE:
+        return t
+    return t.contiguous() if t.shape[2] > 1 else t[:, :, 0].unsqueeze(2)  # (one position: any stride will do)
+
+
+def _near_order(t: torch.Tensor) -> tuple:
+    """_dense_order, or [B,H,T,D] where that would put the positions too far from each other (dimensions that t shows several
+    times come innermost in it)."""
+    s = _dense_order(t)
+    B, H, T, D = t.shape
+    return s if s[2] < LATTN_MAX_STRIDE else (H * T * D, T * D, D, 1)
 
 
 def _lattn_values(q, k, v, rate, valid_len, state, scale, out=None, state_out=None, ws=None) -> tuple:
@@ -1212,7 +1222,7 @@ def _lattn_ws(q, k, v, backward: int) -> Optional[torch.Tensor]:
 def _lattn_run(q, k, v, rate, state, valid_len, scale):
     B, H, T, Dk = q.shape
     Dv = v.shape[3]
-    out = q.new_empty((B, T, H, Dv)).transpose(1, 2)
+    out = q.new_empty((B, T, H, Dv)).transpose(1, 2) if H * Dv < LATTN_MAX_STRIDE else q.new_empty((B, H, T, Dv))
     state_out = rate.new_empty((B, H, Dk, Dv))
     ws = _lattn_ws(q, k, v, 0)
     _launch("ic_lattn_fwd", _pack_lattn(*_lattn_values(q, k, v, rate, valid_len, state, scale, out, state_out, ws)), q.device)
@@ -1240,7 +1250,7 @@ class LinearAttnFn(torch.autograd.Function):
         drate = torch.empty_like(rate) if ctx.needs_input_grad[3] else None
         dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
         ws = _lattn_ws(q, k, v, 1)
-        dq, dk, dv = (t.new_empty_strided(t.shape, _dense_order(t)) for t in (q, k, v))
+        dq, dk, dv = (t.new_empty_strided(t.shape, _near_order(t)) for t in (q, k, v))
         _launch("ic_lattn_bwd", _pack_lattn_bwd(
             *_lattn_values(q, k, v, rate, valid_len, state, ctx.scale, ws=ws), gout.data_ptr(), *gout.stride()[:3], _addr(gstate),
             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], _addr(drate), _addr(dstate)), q.device)
@@ -1272,8 +1282,8 @@ def linear_attention(q, k, v, rate, *, scale: float = 1.0, state=None, valid_len
     q [B,H,T,Dk], k [B,Hk,T,Dk], v [B,Hk,T,Dv] in fp32, bf16 or fp16 (any strides; Dk, Dv <= 128); query head h reads key /
     value head h // (H // Hk).  rate [H] fp32 >= 0.  state [B,H,Dk,Dv] fp32: S before the first position (None: zero).
     valid_len [B]: positions >= valid_len[b] are padding (zeros out, the state passes them by, whatever they hold).
-    Returns (out [B,H,T,Dv] in q's type, its memory in [B,T,H,Dv] order; the state behind the last valid position, fp32:
-    the next call's `state`, or linear_attention_step's).  Gradients reach q, k, v, rate and state."""
+    Returns (out [B,H,T,Dv] in q's type, its memory in [B,T,H,Dv] order ([B,H,T,Dv] from H * Dv = 2^22 on); the state behind the
+    last valid position, fp32: the next call's `state`, or linear_attention_step's).  Gradients reach q, k, v, rate and state."""
     if q.dim() != 4:
         raise ValueError(f"linear_attention: q is {tuple(q.shape)}, needs [B,H,T,Dk]")
     _check_linear("linear_attention", q, k, v, rate, state, 4, LATTN_MAX_D)

@@ -81,3 +81,67 @@ def test_rope_of_one_side_without_heads(norm):
             assert float(gw.abs().max()) == 0.0
         with torch.no_grad():
             assert torch.equal(call(*place(none))[at], got[at].detach())
+
+
+def far_apart(device, which):
+    """Inputs whose outputs or gradients would lie 2^22 elements and more from position to position in their usual order."""
+    g = torch.Generator(device=device).manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=g, device=device)  # noqa: E731
+    if which == "many heads":  # H * Dv = 2^22
+        return r(1, 3, 1 << 16, 2).transpose(1, 2), r(1, 3, 1 << 16, 2).transpose(1, 2), r(1, 3, 1, 64).transpose(1, 2).expand(1, 1 << 16, 3, 64)
+    if which == "one position":  # H * Dk = 2^22, a view whose only position has that stride
+        return r(1, 1, 1 << 16, 64).transpose(1, 2), r(1, 1, 1, 64).transpose(1, 2), r(1, 1, 1, 2).transpose(1, 2)
+    # keys of one sequence shown to all: their gradient's dense order has the sequences inside the positions
+    k = r(1, 3, 64, 128).transpose(1, 2).expand(512, 64, 3, 128)
+    return r(512, 3, 64, 128).transpose(1, 2), k, r(512, 3, 64, 1).transpose(1, 2)
+
+
+FAR = ["many heads", "one position", "shared keys"]
+
+
+@pytest.mark.parametrize("which", FAR)
+def test_linear_attention_lays_out_what_it_makes_within_its_own_limits(which, monkeypatch):
+    from ironcortex_amd import hip
+    from ironcortex_amd.hip import ops
+    got = []
+
+    def launch(name, blob, device):
+        a = hip.CLASSES["ic_lattn_args" if name == "ic_lattn_fwd" else "ic_lattn_bwd_args"].from_buffer_copy(blob)
+        f = a.f if name == "ic_lattn_bwd" else a
+        got.extend([f.q_st, f.k_st, f.v_st] + ([f.o_st] if f is a else [a.do_st, a.dq_st, a.dk_st, a.dv_st]))
+
+    monkeypatch.setattr(ops, "_launch", launch)
+    monkeypatch.setattr(ops, "_same_device", lambda *a, **kw: None)
+    q, k, v = (x.detach().requires_grad_(True) for x in far_apart("cpu", which))
+    H = q.shape[1]
+    o, _ = ops.linear_attention(q, k, v, torch.ones(H))
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), torch.ones(o.shape))
+    assert len(got) == 11 and all(0 <= s < ops.LATTN_MAX_STRIDE for s in got), got
+    assert all(x.numel() == 1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())) for x in (o, dq, dk, dv))  # dense
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", FAR)
+def test_linear_attention_of_rows_far_apart_equals_a_piece_of_them(which):
+    """A few heads (sequences) of such a call give the same rows and gradients as in a call of their own."""
+    from ironcortex_amd.hip import ops
+    q, k, v = (x.detach().requires_grad_(True) for x in far_apart(DEV, which))
+    B, H, T, _ = q.shape
+    rate = torch.rand(H, device=DEV) * 0.5
+    o, s = ops.linear_attention(q, k, v, rate)
+    go = torch.randn(o.shape, device=DEV)
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), go)
+    nb, nh = (2, H) if B > 1 else (1, 5)
+    qs = q.detach()[:nb, H - nh:].clone().requires_grad_(True)
+    ks, vs = (x.detach()[:nb, -min(nh, x.shape[1]):].clone().requires_grad_(True) for x in (k, v))
+    o2, s2 = ops.linear_attention(qs, ks, vs, rate[H - nh:])
+    assert torch.equal(o[:nb, H - nh:].detach(), o2.detach()) and torch.equal(s[:nb, H - nh:].detach(), s2.detach())
+    dq2, dk2, dv2 = torch.autograd.grad(o2, (qs, ks, vs), go[:nb, H - nh:])
+    assert torch.equal(dq[:nb, H - nh:], dq2)
+    if k.shape[1] == H:
+        assert torch.equal(dk[:nb, H - nh:], dk2) and torch.equal(dv[:nb, H - nh:], dv2)
+    else:  # gradients of a head shared by all: every query head adds to them
+        want = (q.detach().double() * (go.double() * v.detach().double()).sum(-1, keepdim=True)).sum(1, keepdim=True)  # (one position)
+        size = (q.detach().double() * (go.double() * v.detach().double()).sum(-1, keepdim=True)).abs().sum(1, keepdim=True)
+        # a sum over H heads, one rounding each, grows like its root: 4 sqrt(H) u of the sizes
+        assert bool(((dk.double() - want).abs() <= 4 * H ** 0.5 * 2.0 ** -24 * size).all())
