@@ -9,9 +9,11 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import sys
 from typing import Callable, Dict, List, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ENUMS, check, lib, new, packer, ptr, stream_handle
@@ -954,6 +956,21 @@ def _same_device(who: str, first: torch.Tensor, **others) -> None:
     for n, t in others.items():
         if t is not None and t.device != first.device:
             raise RuntimeError(f"{who}: {n} is on {t.device}, the rows are on {first.device}")
+
+
+def not_eager(*ts: Optional[torch.Tensor]) -> str:
+    """What keeps a launch from standing for an operation on these tensors, or "": what records operations (torch.jit.trace,
+    torch.fx) does not see it, torch.func's transforms have no rule for it, and it hands no tangent on."""
+    if torch._C._are_functorch_transforms_active():
+        return "under a transform of torch.func"
+    if torch._C._is_tracing():
+        return "under torch.jit.trace"
+    fx = sys.modules.get("torch.fx.experimental.proxy_tensor")
+    if fx is not None and fx.get_proxy_mode() is not None:
+        return "while torch.fx records"
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        return "on dual numbers (forward-mode differentiation)"
+    return ""
 
 
 def _addr(t: Optional[torch.Tensor]) -> int:

@@ -54,9 +54,9 @@ def rope_rotate_pairs(x: torch.Tensor, cos_th: torch.Tensor, sin_th: torch.Tenso
 def rotate_qk(q: torch.Tensor, k: torch.Tensor, cos_th: torch.Tensor, sin_th: torch.Tensor):
     """rope_rotate_pairs of q and k [B,H,T,hd] by angles [B,T,m] in one launch (ops.rope: the same products, differences and
     sums in the same order, so the same bits); the plain formulation for anything but fp32 on the device (other types
-    promote there) and for angles that carry a gradient."""
-    if (q.is_cuda and q.dtype == k.dtype == cos_th.dtype == torch.float32 and q.shape[-1] <= ops.ROPE_MAX_D
-            and not cos_th.requires_grad):
+    promote there), for angles that carry a gradient, and where operations are recorded, transformed or differentiated forwards."""
+    if (not torch.compiler.is_compiling() and type(q) is torch.Tensor and q.is_cuda and q.dtype == k.dtype == cos_th.dtype == torch.float32
+            and q.shape[-1] <= ops.ROPE_MAX_D and not (cos_th.requires_grad or sin_th.requires_grad) and not ops.not_eager(q, k, cos_th, sin_th)):
         return ops.rope(q, k, cos=cos_th, sin=sin_th)
     c, s, m = cos_th.unsqueeze(1), sin_th.unsqueeze(1), cos_th.shape[-1]
     return rope_rotate_pairs(q, c, s, m), rope_rotate_pairs(k, c, s, m)

@@ -145,3 +145,76 @@ def test_linear_attention_of_rows_far_apart_equals_a_piece_of_them(which):
         size = (q.detach().double() * (go.double() * v.detach().double()).sum(-1, keepdim=True)).abs().sum(1, keepdim=True)
         # a sum over H heads, one rounding each, grows like its root: 4 sqrt(H) u of the sizes
         assert bool(((dk.double() - want).abs() <= 4 * H ** 0.5 * 2.0 ** -24 * size).all())
+
+
+def masked_mixer(seed=0):
+    """A mixer whose context mask takes the plain [T,T] attention behind the rotation; x [2,9,32]; the mask."""
+    from ironcortex_amd.mixer import IronRoPESelfAttention
+    torch.manual_seed(seed)
+    m = IronRoPESelfAttention(32, 2, 64, rope_m=6, fb_m=4).to(DEV)
+    x = torch.randn(2, 9, 32, device=DEV)
+    mask = torch.ones(2, 9, dtype=torch.bool, device=DEV)
+    mask[:, 7:] = False
+    return m, x, mask
+
+
+def plain_rotation(monkeypatch):
+    from ironcortex_amd.hip import ops
+    monkeypatch.setattr(ops, "ROPE_MAX_D", 0)  # (no row is narrow enough for the kernel)
+
+
+@pytest.mark.gpu
+def test_mixer_hands_tangents_on(monkeypatch):
+    import torch.autograd.forward_ad as fw
+    m, x, mask = masked_mixer()
+    t = torch.randn_like(x)
+
+    def jvp():
+        with torch.no_grad(), fw.dual_level():
+            return fw.unpack_dual(m(fw.make_dual(x, t), context_mask=mask)).tangent
+
+    got = jvp()
+    plain_rotation(monkeypatch)
+    assert torch.equal(got, jvp())
+
+
+@pytest.mark.gpu
+def test_mixer_under_torch_func_equals_the_plain_rotation(monkeypatch):
+    from ironcortex_amd.mixer import rotate_qk
+    g = torch.Generator(device=DEV).manual_seed(2)
+    q, k, dq = (torch.randn(3, 2, 5, 8, generator=g, device=DEV) for _ in range(3))
+    th = torch.rand(3, 5, 4, generator=g, device=DEV)
+    c, s = torch.cos(th), torch.sin(th)
+    turn = lambda a: rotate_qk(a, k, c, s)[0]  # noqa: E731
+    one = lambda a, b: rotate_qk(a.unsqueeze(0), b.unsqueeze(0), c[:1], s[:1])[0][0]  # noqa: E731
+    calls = (lambda: torch.func.grad(lambda a: turn(a).sin().sum())(q), lambda: torch.func.jvp(turn, (q,), (dq,)),
+             lambda: torch.func.vmap(one)(q, k), lambda: torch.func.hessian(lambda a: turn(a)[0, 0, 0].sin().sum())(q))
+    got = [f() for f in calls]
+    plain_rotation(monkeypatch)
+    for a, f in zip(got, calls):
+        assert all(torch.equal(x, y) for x, y in zip(a, f()))
+
+
+@pytest.mark.gpu
+def test_mixer_traces_record_the_rotation():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from ironcortex_amd.mixer import rotate_qk
+    g = torch.Generator(device=DEV).manual_seed(2)
+    q, k, q2 = (torch.randn(3, 2, 5, 8, generator=g, device=DEV) for _ in range(3))
+    th = torch.rand(3, 5, 4, generator=g, device=DEV)
+    f = lambda a, b: rotate_qk(a, b, torch.cos(th), torch.sin(th))  # noqa: E731
+    want = f(q2, k)
+    fake = torch._subclasses.FakeTensorMode(allow_non_fake_inputs=True)
+    for h in (torch.jit.trace(f, (q, k), check_trace=False), make_fx(f)(q, k), make_fx(f, tracing_mode="fake", _allow_non_fake_inputs=True)(q, k),
+              make_fx(f, pre_dispatch=True)(q, k), torch.compile(f, backend="eager", fullgraph=True)):
+        got = h(q2, k)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with fake:
+        y, _ = f(fake.from_tensor(q), fake.from_tensor(k))
+    assert y.shape == q.shape and y.device == q.device
+    m, x, mask = masked_mixer()
+    with torch.no_grad():
+        m.requires_grad_(False)
+        h = torch.jit.trace(lambda a: m(a, context_mask=mask), x, check_trace=False)
+        x2 = torch.randn_like(x)
+        assert torch.equal(h(x2), m(x2, context_mask=mask))
