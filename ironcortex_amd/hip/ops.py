@@ -9,10 +9,10 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
-import sys
 from typing import Callable, Dict, List, Optional
 
 import torch
+from torch._ops import _get_dispatch_mode_pre_dispatch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
@@ -958,19 +958,28 @@ def _same_device(who: str, first: torch.Tensor, **others) -> None:
             raise RuntimeError(f"{who}: {n} is on {t.device}, the rows are on {first.device}")
 
 
+_transformed, _traced, _mode, _PROXY = (torch._C._are_functorch_transforms_active, torch._C._is_tracing, torch._C._get_dispatch_mode,
+                                        torch._C._TorchDispatchModeKey.PROXY)  # (every call of an operator asks: 0.4 us)
+
+
 def not_eager(*ts: Optional[torch.Tensor]) -> str:
     """What keeps a launch from standing for an operation on these tensors, or "": what records operations (torch.jit.trace,
     torch.fx) does not see it, torch.func's transforms have no rule for it, and it hands no tangent on."""
-    if torch._C._are_functorch_transforms_active():
+    if _transformed():
         return "under a transform of torch.func"
-    if torch._C._is_tracing():
+    if _traced():
         return "under torch.jit.trace"
-    fx = sys.modules.get("torch.fx.experimental.proxy_tensor")
-    if fx is not None and fx.get_proxy_mode() is not None:
+    if _mode(_PROXY) is not None or _get_dispatch_mode_pre_dispatch(_PROXY) is not None:
         return "while torch.fx records"
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
         return "on dual numbers (forward-mode differentiation)"
     return ""
+
+
+def _eager_only(who: str, *ts: Optional[torch.Tensor]) -> None:
+    why = not_eager(*ts)
+    if why:
+        raise RuntimeError(f"{who}: launches a kernel on its tensors' memory and cannot be used {why}")
 
 
 def _addr(t: Optional[torch.Tensor]) -> int:
@@ -1127,7 +1136,8 @@ class QKNormRopeFn(torch.autograd.Function):
         return (*outs, *gws, None, None) + (None,) * len(hold)
 
 
-def _check_qk(who, q, k) -> None:
+def _check_qk(who, q, k, *others) -> None:
+    _eager_only(who, q, k, *others)
     _same_device(who, q, k=k)
     if q.dim() != 4 or q.dtype not in DTYPES or not 1 <= q.shape[3] <= ROPE_MAX_D:
         raise ValueError(f"{who}: q is {q.dtype} {tuple(q.shape)}, needs fp32, bf16 or fp16 [B,H,T,D] with D <= {ROPE_MAX_D}")
@@ -1142,8 +1152,9 @@ def rope(q, k=None, *, cos=None, sin=None, positions=None, freqs=None, layout: s
     "half" -- turned by their position's angles; the other D - 2m are copied.  Angles come as fp32 tables cos / sin
     ([T,m] or [B,T,m]), or from freqs ([m], radians per position, fp32 or fp64) and integer positions ([T] or [B,T]; None:
     0 .. T-1), whose product is formed in 64 bits.  scale multiplies both cos and sin (the rotated channels).
-    Returns dense [B,H,T,D] rows: the rotated q, or (q, k).  Gradients reach q and k."""
-    _check_qk("rope", q, k)
+    Returns dense [B,H,T,D] rows: the rotated q, or (q, k).  Gradients reach q and k; like every operator from here to
+    linear_attention_step it raises in a trace, under torch.func's transforms and on dual numbers."""
+    _check_qk("rope", q, k, cos, sin, freqs)
     ang, hold = _angles("rope", q, cos, sin, positions, freqs, layout, scale)
     if q.numel() == 0:
         return q.clone() if k is None else (q.clone(), k.clone() if k.numel() == 0 else _rope(k, None, ang, hold))
@@ -1163,7 +1174,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, *, eps: float = 1e-5, cos=None, sin=N
     """rope() of w * x / sqrt(mean_D(x^2) + eps): an RMSNorm of every head's row of q (weight q_weight [D]) and of k
     (k_weight [D]; weights in fp32 or in the rows' type), then the rotation, in one pass over the rows.
     Gradients reach q, k and both weights."""
-    _check_qk("qk_norm_rope", q, k)
+    _check_qk("qk_norm_rope", q, k, q_weight, k_weight, cos, sin, freqs)
     _same_device("qk_norm_rope", q, q_weight=q_weight, k_weight=k_weight)
     for n, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w.dim() != 1 or w.shape[0] != q.shape[3] or w.dtype not in (torch.float32, q.dtype):
@@ -1275,6 +1286,7 @@ class LinearAttnFn(torch.autograd.Function):
 
 
 def _check_linear(who, q, k, v, rate, state, dims: int, most: int):
+    _eager_only(who, q, k, v, rate, state)
     _same_device(who, q, k=k, v=v, rate=rate, state=state)
     want = "[B,H,T,Dk], [B,Hk,T,Dk], [B,Hk,T,Dv]" if dims == 4 else "[B,H,Dk], [B,Hk,Dk], [B,Hk,Dv]"
     say = lambda: f"{who}: q, k, v are {q.dtype} {tuple(q.shape)}, {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}"  # noqa: E731

@@ -218,3 +218,29 @@ def test_mixer_traces_record_the_rotation():
         h = torch.jit.trace(lambda a: m(a, context_mask=mask), x, check_trace=False)
         x2 = torch.randn_like(x)
         assert torch.equal(h(x2), m(x2, context_mask=mask))
+
+
+def test_operators_refuse_traces_transforms_and_dual_numbers(launches):
+    import torch.autograd.forward_ad as fw
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from ironcortex_amd.hip import ops
+    x, w, r, st, f = torch.randn(2, 3, 5, 8), torch.ones(8), torch.ones(3), torch.zeros(2, 3, 8, 8), torch.ones(4)
+    table = torch.ones(5, 4)
+    calls = [lambda a: ops.rope(a, freqs=f), lambda a: ops.rope(x, a, freqs=f)[1], lambda a: ops.qk_norm_rope(a, x, w, w, freqs=f)[0],
+             lambda a: ops.linear_attention(a, x, x, r)[0], lambda a: ops.linear_attention_step(a[:, :, 0], x[:, :, 0], x[:, :, 0], r, st)]
+    with torch.no_grad():
+        for i, f_ in enumerate(calls):
+            for go in (lambda: torch.jit.trace(f_, x, check_trace=False), lambda: make_fx(f_)(x), lambda: make_fx(f_, pre_dispatch=True)(x),
+                       lambda: torch.func.vmap(f_)(torch.stack((x, x))), lambda: torch.func.jvp(f_, (x,), (x,)), lambda: torch.func.grad(lambda a: f_(a).sum())(x)):
+                with pytest.raises(RuntimeError, match="cannot be used|no gradients"):
+                    go()
+        with fw.dual_level():
+            dual = fw.make_dual
+            for f_ in calls + [lambda a: ops.qk_norm_rope(x, x, w, a[0, 0, 0], freqs=f)[0], lambda a: ops.linear_attention(x, x, x, a[0, :, 0, 0])[0],
+                               lambda a: ops.linear_attention(x, x, x, r, state=a[:, :, :1].expand(2, 3, 8, 8))[0], lambda a: ops.rope(x, cos=a[0, 0, :, :4], sin=table),
+                               lambda a: ops.rope(x, freqs=a[0, 0, 0, :4])]:
+                with pytest.raises(RuntimeError, match="cannot be used"):
+                    f_(dual(x, x))
+            assert launches == []
+            ops.rope(x, freqs=f)  # (a level without a tangent)
+    assert launches == ["ic_rope_fwd"]
