@@ -1079,31 +1079,64 @@ def _rope_values(ang, hold, q, k, yq=None, yk=None, wq=None, wk=None, eps: float
     return (B, T, D, m, DTYPES[q.dtype], layout, inverse, pos64, freq64, scale, eps, *src, *_rope_rows(q, yq, wq), *_rope_rows(k, yk, wk))
 
 
-def _rope_run(ang, hold, q, k, wq=None, wk=None, eps: float = 0.0):
-    yq = q.new_empty(q.shape)
-    yk = None if k is None else k.new_empty(k.shape)
-    _launch("ic_rope_fwd", _pack_rope(*_rope_values(ang, hold, q, k, yq, yk, wq, wk, eps)), q.device)
+def _rope_run(ang, hold, q, k, wq=None, wk=None, eps: float = 0.0, inverse: int = 0, order=None):
+    yq, yk = (None if x is None else x.new_empty(x.shape) if order is None else x.new_empty_strided(x.shape, order[i]) for i, x in enumerate((q, k)))
+    _launch("ic_rope_fwd", _pack_rope(*_rope_values(ang, hold, q, k, yq, yk, wq, wk, eps, inverse)), q.device)
     return yq, yk
 
 
+def _in_memory(*ts: Optional[torch.Tensor]) -> bool:
+    """False for tensors that only stand for others (batches of gradients under vmap)."""
+    try:
+        for t in ts:
+            _addr(t)
+    except RuntimeError:
+        return False
+    return True
+
+
+def _rope_plain(ang, hold, x, inverse: int):
+    """What the launch computes, in torch operations: for gradients that are recorded, transformed or dual numbers."""
+    m, layout, _, _, scale, _, tables = ang
+    if tables:
+        c, s = hold
+    else:
+        pos = hold[1] if len(hold) > 1 else torch.arange(x.shape[2], device=x.device)
+        th = pos.unsqueeze(-1).double() * hold[0].double()
+        c, s = torch.cos(th).float(), torch.sin(th).float()
+    c, s = (c * scale).unsqueeze(-3), (s * (-scale if inverse else scale)).unsqueeze(-3)
+    y, half = x.float(), layout == ROPE_LAYOUTS["half"]
+    a, b = (y[..., :m], y[..., m:2 * m]) if half else (y[..., 0:2 * m:2], y[..., 1:2 * m:2])
+    u, v = a * c - b * s, a * s + b * c
+    turned = torch.cat((u, v), -1) if half else torch.stack((u, v), -1).reshape(x.shape[:-1] + (2 * m,))
+    return torch.cat((turned, y[..., 2 * m:]), -1).to(x.dtype)
+
+
 class RopeFn(torch.autograd.Function):
-    """Rotated queries (and keys) in one launch (ic_rope_fwd); the backward is the rotation by the negative angles."""
+    """Rotated queries (and keys) in one launch (ic_rope_fwd).  The backward is the rotation by the negative angles, itself of
+    this kind: a linear map's derivatives of every order."""
 
     @staticmethod
-    def forward(ctx, q, k, ang, *hold):
+    def forward(ctx, q, k, ang, inverse, order, *hold):
         ctx.save_for_backward(*hold)  # (so that angles changed in place raise)
-        ctx.ang = ang
+        ctx.ang, ctx.inverse = ang, inverse
         ctx.order = [_dense_order(t) for t in (q, k) if t is not None]
-        return _rope_run(ang, hold, q, k)
+        return _rope_run(ang, hold, q, k, inverse=inverse, order=order)
 
-    @_once
+    @staticmethod
     def backward(ctx, gq, gk):
         hold = ctx.saved_tensors
-        gq, gk = _rows4(gq), _rows4(gk) if len(ctx.order) > 1 else None
-        oq = gq.new_empty_strided(gq.shape, ctx.order[0])
-        ok = None if gk is None else gk.new_empty_strided(gk.shape, ctx.order[1])
-        _launch("ic_rope_fwd", _pack_rope(*_rope_values(ctx.ang, hold, gq, gk, oq, ok, inverse=1)), gq.device)
-        return (oq, ok, None) + (None,) * len(hold)
+        if len(ctx.order) == 1:
+            gk = None
+        if not_eager(gq, gk) or not _in_memory(gq, gk):
+            oq, ok = (None if g is None else _rope_plain(ctx.ang, hold, g, 1 - ctx.inverse) for g in (gq, gk))
+        else:
+            gq, gk = _rows4(gq), None if gk is None else _rows4(gk)
+            if _wants_grad(gq, gk):
+                oq, ok = RopeFn.apply(gq, gk, ctx.ang, 1 - ctx.inverse, ctx.order, *hold)
+            else:
+                oq, ok = _rope_run(ctx.ang, hold, gq, gk, inverse=1 - ctx.inverse, order=ctx.order)
+        return (oq, ok, None, None, None) + (None,) * len(hold)
 
 
 class QKNormRopeFn(torch.autograd.Function):
@@ -1152,7 +1185,7 @@ def rope(q, k=None, *, cos=None, sin=None, positions=None, freqs=None, layout: s
     "half" -- turned by their position's angles; the other D - 2m are copied.  Angles come as fp32 tables cos / sin
     ([T,m] or [B,T,m]), or from freqs ([m], radians per position, fp32 or fp64) and integer positions ([T] or [B,T]; None:
     0 .. T-1), whose product is formed in 64 bits.  scale multiplies both cos and sin (the rotated channels).
-    Returns dense [B,H,T,D] rows: the rotated q, or (q, k).  Gradients reach q and k; like every operator from here to
+    Returns dense [B,H,T,D] rows: the rotated q, or (q, k).  Gradients, of any order, reach q and k; like every operator from here to
     linear_attention_step it raises in a trace, under torch.func's transforms and on dual numbers."""
     _check_qk("rope", q, k, cos, sin, freqs)
     ang, hold = _angles("rope", q, cos, sin, positions, freqs, layout, scale)
@@ -1165,7 +1198,7 @@ def rope(q, k=None, *, cos=None, sin=None, positions=None, freqs=None, layout: s
 
 def _rope(q, k, ang, hold):
     q, k = _rows4(q), None if k is None else _rows4(k)
-    yq, yk = RopeFn.apply(q, k, ang, *hold) if _wants_grad(q, k) else _rope_run(ang, hold, q, k)
+    yq, yk = RopeFn.apply(q, k, ang, 0, None, *hold) if _wants_grad(q, k) else _rope_run(ang, hold, q, k)
     return yq if k is None else (yq, yk)
 
 

@@ -244,3 +244,72 @@ def test_operators_refuse_traces_transforms_and_dual_numbers(launches):
             assert launches == []
             ops.rope(x, freqs=f)  # (a level without a tangent)
     assert launches == ["ic_rope_fwd"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tables", [False, True])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rope_derivatives_of_second_and_third_order(layout, tables):
+    """y = R x: the gradient of sum(y^3) is 3 R^T y^2, along u its derivative is 6 R^T (y R u), and so on."""
+    from ironcortex_amd.hip import ops
+    g = torch.Generator(device=DEV).manual_seed(6)
+    q, k = (torch.randn(2, 21, h, 16, generator=g, device=DEV).transpose(1, 2).requires_grad_(True) for h in (3, 1))
+    u = torch.randn(2, 3, 21, 16, generator=g, device=DEV)
+    pos, f = torch.randint(0, 1000, (2, 21), generator=g, device=DEV), torch.rand(6, generator=g, device=DEV)
+    th = pos.unsqueeze(-1).double() * f.double()
+    c, s = torch.cos(th).float(), torch.sin(th).float()
+    kw = dict(cos=c, sin=s) if tables else dict(positions=pos, freqs=f)
+
+    def R(x, sign):
+        cc, ss = (c.double().unsqueeze(1) * 1.25, s.double().unsqueeze(1) * 1.25 * sign) if tables else (torch.cos(th).unsqueeze(1) * 1.25, torch.sin(th).unsqueeze(1) * 1.25 * sign)
+        a, b = (x[..., :6], x[..., 6:12]) if layout == "half" else (x[..., 0:12:2], x[..., 1:12:2])
+        ra, rb = a * cc - b * ss, a * ss + b * cc
+        return torch.cat((torch.cat((ra, rb), -1) if layout == "half" else torch.stack((ra, rb), -1).flatten(-2), x[..., 12:]), -1)
+
+    y, yk = ops.rope(q, k, layout=layout, scale=1.25, **kw)
+    g1, gk = torch.autograd.grad(y.pow(3).sum() + yk.pow(3).sum(), (q, k), create_graph=True)
+    g2, = torch.autograd.grad((g1 * u).sum(), q, create_graph=True)
+    g3, = torch.autograd.grad((g2 * u).sum(), q)
+    yd, ud = R(q.detach().double(), 1), R(u.double(), 1)
+    # chains of at most five rotations and four products, 6u of |a| + |b| each: 64 u of the largest value there
+    for got, want in ((g1, 3 * R(yd.square(), -1)), (g2, 6 * R(yd * ud, -1)), (g3, 6 * R(ud * ud, -1)), (gk, 3 * R(R(k.detach().double(), 1).square(), -1))):
+        assert got.shape == want.shape and float((got.detach().double() - want).abs().max()) <= 64 * 2.0 ** -24 * float(want.abs().max())
+    assert g2.stride() == q.stride()  # (laid out like its input)
+
+
+@pytest.mark.gpu
+def test_mixer_second_derivative_equals_the_plain_rotations(monkeypatch):
+    m, x, mask = masked_mixer()
+    x.requires_grad_(True)
+
+    def twice():
+        g, = torch.autograd.grad(m(x, context_mask=mask).sin().sum(), x, create_graph=True)
+        return torch.autograd.grad(g.square().sum(), [x, *m.parameters()], allow_unused=True)
+
+    got = twice()
+    plain_rotation(monkeypatch)
+    for a, b in zip(got, twice()):  # the same products, some sums in another order
+        assert (a is None) == (b is None) and (a is None or float((a - b).abs().max()) <= 64 * 2.0 ** -24 * float(b.abs().max().clamp_min(1.0)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tables", [False, True])
+def test_rope_backward_of_batched_and_dual_gradients(tables):
+    """Gradients under vmap (a vectorised Jacobian) and with tangents: those of the gradients one by one."""
+    import torch.autograd.forward_ad as fw
+    from ironcortex_amd.hip import ops
+    g = torch.Generator(device=DEV).manual_seed(8)
+    q, k = (torch.randn(2, h, 7, 16, generator=g, device=DEV, requires_grad=True) for h in (2, 1))
+    f = torch.rand(4, generator=g, device=DEV)
+    th = torch.arange(7, device=DEV).unsqueeze(-1) * f
+    kw = dict(cos=torch.cos(th), sin=torch.sin(th)) if tables else dict(freqs=f)
+    y = ops.rope(q, k, **kw)
+    gos = [torch.randn(3, *t.shape, generator=g, device=DEV) for t in y]
+    one = [torch.autograd.grad(y, (q, k), [t[i] for t in gos], retain_graph=True) for i in range(3)]
+    many = torch.autograd.grad(y, (q, k), gos, is_grads_batched=True, retain_graph=True)
+    close = lambda a, b: float((a - b).abs().max()) <= 16 * 2.0 ** -24 * float(b.abs().max())  # noqa: E731  (two evaluations, 6u of |a| + |b| each)
+    for i in range(3):
+        assert close(many[0][i], one[i][0]) and close(many[1][i], one[i][1])
+    with fw.dual_level():
+        d = torch.autograd.grad(y, (q, k), [fw.make_dual(t[0], t[1]) for t in gos])
+        assert all(close(fw.unpack_dual(a).primal, p) and close(fw.unpack_dual(a).tangent, t) for a, p, t in zip(d, one[0], one[1]))
