@@ -1151,6 +1151,7 @@ class QKNormRopeFn(torch.autograd.Function):
 
     @_once
     def backward(ctx, gq, gk):
+        _eager_only("qk_norm_rope's backward", gq, gk)
         q, k, wq, wk, *hold = ctx.saved_tensors
         part = torch.empty(ROPE_PARTS * q.shape[3], device=q.device)
         vals, outs, gws, keep = [], [], [], []
@@ -1305,6 +1306,7 @@ class LinearAttnFn(torch.autograd.Function):
         q, k, v, rate, state, valid_len = ctx.saved_tensors
         if gout is None and gstate is None:
             return (None,) * 7
+        _eager_only("linear_attention's backward", gout, gstate)
         B, H, T, Dk = q.shape
         gout = torch.zeros((B, H, T, v.shape[3]), dtype=q.dtype, device=q.device) if gout is None else _rows_near(gout)
         gstate = None if gstate is None else gstate.contiguous()

@@ -313,3 +313,19 @@ def test_rope_backward_of_batched_and_dual_gradients(tables):
     with fw.dual_level():
         d = torch.autograd.grad(y, (q, k), [fw.make_dual(t[0], t[1]) for t in gos])
         assert all(close(fw.unpack_dual(a).primal, p) and close(fw.unpack_dual(a).tangent, t) for a, p, t in zip(d, one[0], one[1]))
+
+
+def test_backward_refuses_dual_gradients(launches):
+    """Norms and linear attention hand no tangent on in their backward either."""
+    import torch.autograd.forward_ad as fw
+    from ironcortex_amd.hip import ops
+    x, w = torch.randn(2, 3, 5, 8, requires_grad=True), torch.ones(8)
+    go = torch.randn(2, 3, 5, 8)
+    for call in (lambda: ops.qk_norm_rope(x, x, w, w, freqs=torch.ones(4))[0], lambda: ops.linear_attention(x, x, x, torch.ones(3))[0]):
+        y = call()
+        with fw.dual_level():
+            dual = fw.make_dual(go, go)
+            with pytest.raises(RuntimeError, match="cannot be used on dual numbers"):
+                torch.autograd.grad(y, x, dual, retain_graph=True)
+        torch.autograd.grad(y, x, go)
+    assert len(launches) == 4
