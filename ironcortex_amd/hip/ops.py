@@ -1125,7 +1125,7 @@ class RopeFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gq, gk):
-        hold = ctx.saved_tensors
+        hold = [t.contiguous() for t in ctx.saved_tensors]  # (hooks may hand them back in another layout)
         if len(ctx.order) == 1:
             gk = None
         if not_eager(gq, gk) or not _in_memory(gq, gk):
@@ -1153,6 +1153,8 @@ class QKNormRopeFn(torch.autograd.Function):
     def backward(ctx, gq, gk):
         _eager_only("qk_norm_rope's backward", gq, gk)
         q, k, wq, wk, *hold = ctx.saved_tensors
+        q, k = _rows4(q), None if k is None else _rows4(k)
+        wq, wk, *hold = (None if t is None else t.contiguous() for t in (wq, wk, *hold))
         part = torch.empty(ROPE_PARTS * q.shape[3], device=q.device)
         vals, outs, gws, keep = [], [], [], []
         for x, w, g in ((q, wq, gq), (k, wk, gk)):  # ic_rope_grad
@@ -1307,6 +1309,8 @@ class LinearAttnFn(torch.autograd.Function):
         if gout is None and gstate is None:
             return (None,) * 7
         _eager_only("linear_attention's backward", gout, gstate)
+        q, k, v = _rows_near(q), _rows_near(k), _rows_near(v)  # (hooks may hand them back in another layout)
+        rate, state, valid_len = (None if t is None else t.contiguous() for t in (rate, state, valid_len))
         B, H, T, Dk = q.shape
         gout = torch.zeros((B, H, T, v.shape[3]), dtype=q.dtype, device=q.device) if gout is None else _rows_near(gout)
         gstate = None if gstate is None else gstate.contiguous()

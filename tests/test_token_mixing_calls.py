@@ -329,3 +329,30 @@ def test_backward_refuses_dual_gradients(launches):
                 torch.autograd.grad(y, x, dual, retain_graph=True)
         torch.autograd.grad(y, x, go)
     assert len(launches) == 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["rope tables", "rope", "norm", "linear"])
+def test_saved_tensors_may_come_back_in_another_layout(which):
+    """Hooks for saved tensors keep values and shapes; the memory's order is theirs (here: the dimensions reversed)."""
+    from ironcortex_amd.hip import ops
+    g = torch.Generator(device=DEV).manual_seed(9)
+    q, k, v = (torch.randn(2, h, 70, 16, generator=g, device=DEV, requires_grad=True) for h in (4, 2, 2))
+    w = [torch.rand(16, generator=g, device=DEV).requires_grad_(True) for _ in (0, 1)]
+    rate, st = torch.rand(4, generator=g, device=DEV).requires_grad_(True), torch.randn(2, 4, 16, 16, generator=g, device=DEV, requires_grad=True)
+    pos, f = torch.randint(0, 500, (2, 70), generator=g, device=DEV), torch.rand(6, generator=g, device=DEV)
+    th = pos.unsqueeze(-1) * f
+    kw = dict(cos=torch.cos(th), sin=torch.sin(th)) if which == "rope tables" else dict(positions=pos, freqs=f)
+    run = {"norm": lambda: (ops.qk_norm_rope(q, k, *w, **kw), [q, k, *w]),
+           "linear": lambda: (ops.linear_attention(q, k, v, rate, state=st, valid_len=torch.tensor([70, 33], device=DEV)), [q, k, v, rate, st])}.get(
+               which, lambda: (ops.rope(q, k, **kw), [q, k]))
+
+    def grads():
+        y, leaves = run()
+        return torch.autograd.grad([t.sin().sum() for t in y], leaves)
+
+    want = grads()
+    turned = lambda t: t.detach().permute(*reversed(range(t.dim()))).contiguous().permute(*reversed(range(t.dim())))  # noqa: E731
+    with torch.autograd.graph.saved_tensors_hooks(turned, lambda t: t):
+        got = grads()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
