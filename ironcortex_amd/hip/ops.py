@@ -1364,8 +1364,9 @@ def linear_attention(q, k, v, rate, *, scale: float = 1.0, state=None, valid_len
     if B * H > LATTN_MAX_HEADS:
         raise ValueError(f"linear_attention: B * H = {B * H} (at most {LATTN_MAX_HEADS})")
     if B * H * T == 0:
+        none = q.sum() + k.sum() + v.sum() + rate[:0].sum()  # zero, and the way by which (zero) gradients reach all of them
         st = torch.zeros(B, H, Dk, v.shape[3], device=q.device) if state is None else state.clone()
-        return q.new_empty(B, H, T, v.shape[3]) + 0 * (q.sum() + k.sum() + v.sum()), st
+        return (q.new_empty(B, H, T, v.shape[3]) + none).to(q.dtype), st + none.float()
     q, k, v, rate, state = _rows_near(q), _rows_near(k), _rows_near(v), rate.contiguous(), None if state is None else state.contiguous()
     if _wants_grad(q, k, v, rate, state):
         return LinearAttnFn.apply(q, k, v, rate, state, valid_len, float(scale))

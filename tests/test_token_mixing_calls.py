@@ -356,3 +356,23 @@ def test_saved_tensors_may_come_back_in_another_layout(which):
     with torch.autograd.graph.saved_tensors_hooks(turned, lambda t: t):
         got = grads()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear_attention_of_no_positions_passes_gradients_on(dtype, launches):
+    """The state as it came, its gradient with it, and zeros for everything else, as from a call with positions."""
+    from ironcortex_amd.hip import ops
+    for B, H, T in ((2, 3, 0), (0, 3, 5), (2, 0, 5)):
+        q, k, v = (torch.randn(B, H, T, 8, dtype=dtype).requires_grad_(True) for _ in range(3))
+        rate, st = torch.full((H,), float("inf"), requires_grad=True), torch.randn(B, H, 8, 8, requires_grad=True)
+        for state in (st, None):
+            o, s = ops.linear_attention(q, k, v, rate, state=state)
+            assert o.shape == (B, H, T, 8) and o.dtype == dtype and s.dtype == torch.float32
+            assert torch.equal(s, torch.zeros_like(st) if state is None else st) and (state is None or s.data_ptr() != st.data_ptr() or not s.numel())
+            leaves = [q, k, v, rate] + ([] if state is None else [st])
+            for y in (o, s):
+                got = torch.autograd.grad(y.float().sum(), leaves, retain_graph=True, allow_unused=True)
+                for x, gx in zip(leaves, got):
+                    assert torch.equal(torch.zeros_like(x) if gx is None else gx, torch.ones_like(st) if x is st and y is s else torch.zeros_like(x))
+                assert got[3] is not None
+    assert launches == []
