@@ -111,17 +111,17 @@ __device__ __forceinline__ float decay(float l2, int n) { return n == 0 ? 1.f : 
 // rounded next to 1 and applied at every chunk, would leave a slowly decaying state off by that rounding times the number of
 // chunks; where little stays, the sum would cancel.
 struct Carry {
-  float f;
-  bool add;
+  float keep, loss;  // 1 and e^{-rate n} - 1, or e^{-rate n} and 0
 };
 __device__ __forceinline__ Carry carry_of(float rate, int n) {
   const float x = n == 0 ? 0.f : -rate * (float)n, loss = expm1f(x);
   Carry c;
-  c.add = loss > -0.5f;
-  c.f = c.add ? loss : expf(x);
+  c.keep = loss > -0.5f ? 1.f : expf(x);
+  c.loss = loss > -0.5f ? loss : 0.f;
   return c;
 }
-__device__ __forceinline__ float carried(float x, Carry c) { return fmaf(c.f, x, c.add ? x : 0.f); }
+// (what is lost is formed from a finite number: an infinite state stays one)
+__device__ __forceinline__ float carried(float x, Carry c) { return fmaf(c.loss, __builtin_amdgcn_fmed3f(x, -3.402823466e38f, 3.402823466e38f), c.keep * x); }
 __device__ __forceinline__ v4f carried(const v4f& x, Carry c) { return v4f{carried(x[0], c), carried(x[1], c), carried(x[2], c), carried(x[3], c)}; }
 
 template <typename T>
@@ -259,6 +259,7 @@ struct Lds {
   float Ps[kC][kC + 4];
   float dec[2 * kC + 1], dev[2 * kC + 1];  // dec[kC + lag] = e^{-r lag}, 0 for lag < 0; dev = dec * vscale
   double red[DP / 16];
+  Carry whole;  // over a chunk
 };
 template <int DP>
 struct LdsSums {
@@ -398,7 +399,6 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
   const Span sp = SUMS ? sm->sp : p->sp;
   const int n = valid_of(g, b), T_ = g.T;
   const float rate = g.rate[h], l2 = -rate * 1.44269504088896340736f;
-  const Carry whole = carry_of(rate, kC);
   const int Da = SUMS ? sm->Da : p->Da, Db = SUMS ? sm->Db : p->Db;
   const int rev = SUMS ? sm->rev : p->rev;
   const float vscale = SUMS ? sm->vscale : p->vscale, oscale = SUMS ? 1.f : p->oscale;
@@ -412,6 +412,9 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
     const float d = i < kC ? 0.f : decay(l2, i - kC);
     lds.dec[i] = d;
     lds.dev[i] = d * vscale;
+  }
+  if constexpr (!SUMS) {
+    if (threadIdx.x == 0) lds.whole = carry_of(rate, kC);
   }
   const int NC = (T_ + kC - 1) / kC;
   const int ch0 = seg * sp.cps, ch1 = ch0 + sp.cps < NC ? ch0 + sp.cps : NC;
@@ -544,7 +547,7 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
         } else
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
-          v4f o = v4f{0.f, 0.f, 0.f, 0.f}, e = o;  // (sums of their own: see the state's below)
+          v4f o = v4f{0.f, 0.f, 0.f, 0.f};  // (a sum of its own: see the state's below)
 #pragma unroll
           for (int s = 0; s <= it; ++s) {
             v4f bp = ld4(&Ps[16 * it + c][16 * s + q4]);
@@ -552,11 +555,10 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
             if constexpr (LAG) {
 #pragma unroll
               for (int u = 0; u < 4; ++u) bp[u] *= (float)(16 * (it - s) + c - q4 - u);  // (0 above the diagonal stays 0)
-              e = mma16(v0[s], bp, e);
+              E[it] = mma16(v0[s], bp, E[it]);
             }
           }
           O[it] += o;
-          if constexpr (LAG) E[it] += e;
         }
         if constexpr (LAG) {
 #pragma unroll
@@ -606,7 +608,8 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
     if (cnt > 0) {  // the state behind the chunk; a segment's sums weigh every position from the segment's end, with no carry
       const int left = SUMS ? nend - base - cnt : 0;
       const float ahead = SUMS ? decay(l2, left) : 1.f;
-      const Carry over = SUMS || cnt - off == kC ? whole : carry_of(rate, cnt - off);
+      Carry over{};
+      if constexpr (!SUMS) over = cnt - off == kC ? lds.whole : carry_of(rate, cnt - off);
       constexpr int HS = LAG && DP == 128 ? 1 : 2;
       // A half chunk's own sum first, then one addition: a matrix instruction rounds after each of its products, and added to the
       // state one by one each of the chunk's 64 would be rounded at the state's size (1024 positions of slow decay: state off by
@@ -681,6 +684,7 @@ struct Lds16 {
   uint16_t P[kParts][kPn];
   float dec[2 * kC + 1], dev[2 * kC + 1];  // dec[kC + lag] = e^{-r lag}, 0 for lag < 0; dev = dec * vscale
   double red[DP / 16];
+  Carry whole;  // over a chunk
 };
 template <int DP>
 struct LdsSums16 {
@@ -810,7 +814,6 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
   const Span sp = SUMS ? sm->sp : p->sp;
   const int n = valid_of(g, b), T = g.T;
   const float rate = g.rate[h], l2 = -rate * 1.44269504088896340736f;
-  const Carry whole = carry_of(rate, kC);
   const int Da = SUMS ? sm->Da : p->Da, Db = SUMS ? sm->Db : p->Db;
   const int rev = SUMS ? sm->rev : p->rev;
   const float vscale = SUMS ? sm->vscale : p->vscale, oscale = SUMS ? 1.f : p->oscale;
@@ -823,6 +826,9 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
     const float d = i < kC ? 0.f : decay(l2, i - kC);
     lds.dec[i] = d;
     lds.dev[i] = d * vscale;
+  }
+  if constexpr (!SUMS) {
+    if (threadIdx.x == 0) lds.whole = carry_of(rate, kC);
   }
   const int col0 = 16 * CW * w;  // this wave's columns
   const int NC = (T + kC - 1) / kC;
@@ -1038,7 +1044,8 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
     if (cnt > 0) {  // the state behind the chunk; a segment's sums weigh every position from the segment's end, with no carry
       const int left = SUMS ? nend - base - cnt : 0;
       const float ahead = SUMS ? decay(l2, left) : 1.f;
-      const Carry over = SUMS || cnt - off == kC ? whole : carry_of(rate, cnt - off);
+      Carry over{};
+      if constexpr (!SUMS) over = cnt - off == kC ? lds.whole : carry_of(rate, cnt - off);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         b8 vp[CW][kParts], lp[LAG ? CW : 1][kParts];

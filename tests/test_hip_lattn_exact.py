@@ -108,3 +108,48 @@ def test_rows_on_fp32_products_are_as_exact_as_fp32_allows(dtype, B, H, Hk, T, D
 def test_bf16_rows_are_as_exact_as_fp32_products(B, H, Hk, T, D):
     """Three bf16 parts of an fp32 operand hold all of its 24 bits, two of them 16."""
     check_exactness("bf16", B, H, Hk, T, D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_slow_decays_over_many_chunks(dtype):
+    """256 chunks of one segment, rates down to 1e-6: a factor rounded next to 1 (off by 2^-26 of it in the mean) and applied 256
+    times would leave a state off by 256 * 1.5e-8 / 2 = 2e-6.  Rounded additions: 2.5e-8 sqrt(512 / 2) = 4e-7, and 1.1e-7 inside the
+    chunks; 6e-7 is asserted of every head."""
+    from ironcortex_amd.hip import ops
+    dt, B, H, T, D = TYPES[dtype], 128, 8, 16384, 16
+    g = torch.Generator(device=DEV).manual_seed(70)
+    k, v = (torch.randn(B, T, H, D, generator=g, device=DEV).to(dt).transpose(1, 2) for _ in (0, 1))
+    rate = torch.exp(torch.linspace(math.log(1e-6), math.log(2e-4), H, device=DEV))
+    s0 = torch.randn(B, H, D, D, generator=g, device=DEV)
+    got = ops.linear_attention(k, k, v, rate, state=s0)[1][:4]
+    t, r = torch.arange(T, device=DEV, dtype=torch.float64), rate.double().view(1, H, 1, 1)
+    want = torch.exp(-r * T) * s0[:4].double()
+    want += (k[:4].double() * torch.exp(-r * (T - 1 - t).view(1, 1, T, 1))).transpose(2, 3) @ v[:4].double()
+    for h in range(H):
+        e = rms(got[:, h] - want[:, h]) / rms(want[:, h])
+        assert e <= 6e-7, f"{dtype} rate {float(rate[h]):.1e}: {e:.2e}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("T", [50, 700])
+def test_an_infinite_state_stays_infinite(T, dtype):
+    """Entries that are not finite stay what they are, whatever the decay; the others are those of a finite state."""
+    from ironcortex_amd.hip import ops
+    dt, B, H, D = TYPES[dtype], 3, 4, 16
+    g = torch.Generator(device=DEV).manual_seed(71)
+    q, k, v = (torch.randn(B, T, H, D, generator=g, device=DEV).to(dt).transpose(1, 2) for _ in range(3))
+    rate = torch.tensor([0.0, 1e-4, 1e-2, 0.05], device=DEV)
+    n = torch.tensor([T, 0, T // 2], device=DEV)
+    s = torch.randn(B, H, D, D, generator=g, device=DEV)
+    bad = s.clone()
+    bad[..., 3, 5], bad[..., 4, 6], bad[..., 7, 7] = float("inf"), float("-inf"), float("nan")
+    o, want = ops.linear_attention(q, k, v, rate, state=s, valid_len=n)
+    o2, got = ops.linear_attention(q, k, v, rate, state=bad, valid_len=n)
+    odd = ~torch.isfinite(bad)
+    assert torch.equal(got[~odd], want[~odd]) and torch.equal(torch.nan_to_num(got[odd], nan=7.0), torch.nan_to_num(bad[odd], nan=7.0))
+    keep = [c for c in range(D) if c not in (5, 6, 7)]
+    assert torch.equal(o2[..., keep], o[..., keep])
+    live = torch.arange(T, device=DEV) < n.view(B, 1)
+    assert not bool(torch.isfinite(o2.transpose(1, 2)[live][..., [5, 6, 7]]).any())
