@@ -1240,10 +1240,14 @@ __global__ __launch_bounds__(256) void k_lattn_step(ic_lattn_step_args a) {
   for (int u = 0; u < 4; ++u) red[r][(threadIdx.x & 7) * 4 + u] = o[u];
   __syncthreads();
   if (threadIdx.x < 32 && oc < a.Dv) {
-    float s = 0.f;
+    float s[kStepRows];  // (in pairs: five roundings on a term's path, one after the other 32)
 #pragma unroll
-    for (int i = 0; i < kStepRows; ++i) s += red[i][threadIdx.x];
-    out[oc] = ic_from_f<T>(s * a.scale);
+    for (int i = 0; i < kStepRows; ++i) s[i] = red[i][threadIdx.x];
+#pragma unroll
+    for (int w = kStepRows / 2; w; w /= 2)
+#pragma unroll
+      for (int i = 0; i < w; ++i) s[i] += s[i + w];
+    out[oc] = ic_from_f<T>(s[0] * a.scale);
   }
 }
 

@@ -153,3 +153,19 @@ def test_an_infinite_state_stays_infinite(T, dtype):
     assert torch.equal(o2[..., keep], o[..., keep])
     live = torch.arange(T, device=DEV) < n.view(B, 1)
     assert not bool(torch.isfinite(o2.transpose(1, 2)[live][..., [5, 6, 7]]).any())
+
+
+@pytest.mark.gpu
+def test_steps_outputs_are_as_exact_as_sums_in_pairs():
+    """64 key channels: the state's two roundings and its factor's (4.6e-8), two channels a thread and five levels of pairs (6.1e-8),
+    the scale (2.5e-8): 8e-8 in the mean square; 9.5e-8 is asserted.  Adding 32 partial sums one after the other leaves 1.2e-7."""
+    from ironcortex_amd.hip import ops
+    B, H, D = 256, 8, 64
+    g = torch.Generator(device=DEV).manual_seed(72)
+    q, k, v = (torch.randn(B, H, D, generator=g, device=DEV) for _ in range(3))
+    rate, s = torch.rand(H, generator=g, device=DEV), torch.randn(B, H, D, D, generator=g, device=DEV)
+    want = torch.exp(-rate.double()).view(1, H, 1, 1) * s.double() + k.double().unsqueeze(-1) * v.double().unsqueeze(-2)
+    want = 0.3 * (q.double().unsqueeze(-2) @ want).squeeze(-2)
+    got = ops.linear_attention_step(q, k, v, rate, s, scale=float(torch.tensor(0.3)))
+    want *= float(torch.tensor(0.3)) / 0.3
+    assert rms(got - want) <= 9.5e-8 * rms(want), f"{rms(got - want) / rms(want):.2e}"
