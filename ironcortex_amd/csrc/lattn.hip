@@ -120,6 +120,11 @@ __device__ __forceinline__ Carry carry_of(float rate, int n) {
   c.loss = loss > -0.5f ? loss : 0.f;
   return c;
 }
+__device__ __forceinline__ Carry uniform(Carry c) {  // the same in all lanes: in scalar registers
+  c.keep = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(c.keep)));
+  c.loss = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(c.loss)));
+  return c;
+}
 // (what is lost is formed from a finite number: an infinite state stays one)
 __device__ __forceinline__ float carried(float x, Carry c) { return fmaf(c.loss, __builtin_amdgcn_fmed3f(x, -3.402823466e38f, 3.402823466e38f), c.keep * x); }
 __device__ __forceinline__ v4f carried(const v4f& x, Carry c) { return v4f{carried(x[0], c), carried(x[1], c), carried(x[2], c), carried(x[3], c)}; }
@@ -1155,7 +1160,13 @@ __global__ __launch_bounds__(256) void k_lattn_scan(ScanArgs a) {
   float S = z.init ? z.init[(size_t)bh * dd + (size_t)(e / z.Db) * z.ia + (size_t)(e % z.Db) * z.ib] : 0.f, L = 0.f;
   const size_t next = (size_t)nst * dd;
   constexpr int U = 16;  // sums in flight: the chain of states would wait for each of them in turn otherwise
-  const Carry whole = carry_of(rate, len);
+  // segments in front of the one that the sequence ends in, that one, and those behind it; in a reversed pass the first position
+  // takes no decay
+  const int p = n / len, r = n - p * len;
+  const Carry none{1.f, 0.f}, whole = uniform(carry_of(rate, len));
+  Carry first = whole, part = none;
+  if (z.rev) first = uniform(carry_of(rate, len - 1));
+  if (r > 0 && p < z.sp.nseg - 1) part = uniform(carry_of(rate, z.rev && p == 0 ? r - 1 : r));  // (nothing starts behind the last one)
   for (int s0 = 0; s0 < z.sp.nseg; s0 += U, at += U * next) {
     float ls[U], ll[U];
 #pragma unroll
@@ -1168,11 +1179,10 @@ __global__ __launch_bounds__(256) void k_lattn_scan(ScanArgs a) {
     for (int u = 0; u < U; ++u) {
       const int s = s0 + u;
       if (s < z.sp.nseg) {
-        int cnt = n - s * len;
-        cnt = cnt < 0 ? 0 : cnt < len ? cnt : len;
+        const int cnt = s < p ? len : s == p ? r : 0;
         at[u * next] = S;
         if (z.lag) at[u * next + dd] = L;
-        const Carry over = cnt == len && !(z.rev && s == 0) ? whole : carry_of(rate, cnt > 0 && z.rev && s == 0 ? cnt - 1 : cnt);
+        const Carry over = s < p ? (s == 0 ? first : whole) : s == p ? part : none;
         L = carried(L + (float)cnt * S, over) + ll[u];
         S = carried(S, over) + ls[u];
       }
