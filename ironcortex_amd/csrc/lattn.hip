@@ -125,9 +125,34 @@ __device__ __forceinline__ Carry uniform(Carry c) {  // the same in all lanes: i
   c.loss = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(c.loss)));
   return c;
 }
-// (what is lost is formed from a finite number: an infinite state stays one)
+// The state carried plus what is new, and with n > 0 positions of lag the lag-weighted one, e^{-rate n} (l + n x) plus what is new:
+// the small terms first, so that the sum is rounded once at the state's size.  (What is lost is formed from a finite number: an
+// infinite state stays one.)
+__device__ __forceinline__ float carried(float x, Carry c, float more) {
+  return fmaf(c.keep, x, fmaf(c.loss, __builtin_amdgcn_fmed3f(x, -3.402823466e38f, 3.402823466e38f), more));
+}
 __device__ __forceinline__ float carried(float x, Carry c) { return fmaf(c.loss, __builtin_amdgcn_fmed3f(x, -3.402823466e38f, 3.402823466e38f), c.keep * x); }
 __device__ __forceinline__ v4f carried(const v4f& x, Carry c) { return v4f{carried(x[0], c), carried(x[1], c), carried(x[2], c), carried(x[3], c)}; }
+__device__ __forceinline__ float carried_lag(float l, float x, Carry c, int n, float more) { return carried(l, c, fmaf((float)n * (c.keep + c.loss), x, more)); }
+__device__ __forceinline__ v4f carried(const v4f& x, Carry c, const v4f& more) {
+  v4f y;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) y[v] = carried(x[v], c, more[v]);
+  return y;
+}
+__device__ __forceinline__ v4f carried_lag(const v4f& l, const v4f& x, Carry c, int n, const v4f& more) {
+  v4f y;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) y[v] = carried_lag(l[v], x[v], c, n, more[v]);
+  return y;
+}
+// a + f b
+__device__ __forceinline__ v4f fma4(float f, const v4f& b, const v4f& a) {
+  v4f y;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) y[v] = fmaf(f, b[v], a[v]);
+  return y;
+}
 
 template <typename T>
 __device__ __forceinline__ const T* row_base(const Mat& m, int b, int h) {
@@ -537,7 +562,7 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
         for (int it = 0; it < 4; ++it) {
           const float f = lds.dec[kC + 16 * it + c + 1 - off] * oscale;
           O[it] = f * O[it];
-          if constexpr (LAG) E[it] = f * E[it] + (float)(16 * it + c + 1) * O[it];
+          if constexpr (LAG) E[it] = fma4((float)(16 * it + c + 1), O[it], f * E[it]);
         }
         __syncthreads();
         if (!finite) {
@@ -645,8 +670,8 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
               dl = mma16(ak, vl, dl);
             }
           }
-          if constexpr (LAG) L[t] = SUMS || s0 ? L[t] + dl : carried(L[t] + (float)cnt * S[t], over) + dl;
-          S[t] = SUMS || s0 ? S[t] + ds : carried(S[t], over) + ds;
+          if constexpr (LAG) L[t] = SUMS || s0 ? L[t] + dl : carried_lag(L[t], S[t], over, cnt, dl);
+          S[t] = SUMS || s0 ? S[t] + ds : carried(S[t], over, ds);
         }
       }
       __syncthreads();
@@ -973,7 +998,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
           for (int k = 0; k < CW; ++k) {
             O[k][it] = f * O[k][it];
             if constexpr (LAG) {  // what the lag-weighted state adds to d rate
-              E[k][it] = f * E[k][it] + (float)(16 * it + c + 1) * O[k][it];
+              E[k][it] = fma4((float)(16 * it + c + 1), O[k][it], f * E[k][it]);
               const uint16_t* x = &lds.X.r[16 * it + c][col0 + 16 * k + q4];
 #pragma unroll
               for (int v = 0; v < 4; ++v) drc = fmaf(E[k][it][v], __uint_as_float((uint32_t)x[v] << 16), drc);
@@ -1078,8 +1103,10 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
               ds = mma32(ak, vp[k][i], ds);
               if constexpr (LAG) dl = mma32(ak, lp[k][i], dl);
             }
-            if constexpr (LAG) L[k][t] = SUMS || s ? L[k][t] + dl : carried(L[k][t] + (float)cnt * S[k][t], over) + dl;
-            S[k][t] = SUMS || s ? S[k][t] + ds : carried(S[k][t], over) + ds;
+            if constexpr (LAG) L[k][t] = SUMS || s ? L[k][t] + dl : carried_lag(L[k][t], S[k][t], over, cnt, dl);
+            if (SUMS || s) S[k][t] += ds;
+            else if (CW == 1) S[k][t] = carried(S[k][t], over, ds);
+            else S[k][t] = carried(S[k][t], over) + ds;  // (in one sum the two tiles a wave spill: a pass of 302 instead of 202 us)
           }
         }
       }
@@ -1183,8 +1210,8 @@ __global__ __launch_bounds__(256) void k_lattn_scan(ScanArgs a) {
         at[u * next] = S;
         if (z.lag) at[u * next + dd] = L;
         const Carry over = s < p ? (s == 0 ? first : whole) : s == p ? part : none;
-        L = carried(L + (float)cnt * S, over) + ll[u];
-        S = carried(S, over) + ls[u];
+        L = carried_lag(L, S, over, cnt, ll[u]);
+        S = carried(S, over, ls[u]);
       }
     }
   }
