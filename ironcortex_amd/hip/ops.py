@@ -12,7 +12,6 @@ import os
 from typing import Callable, Dict, List, Optional
 
 import torch
-from torch._ops import _get_dispatch_mode_pre_dispatch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
@@ -958,8 +957,10 @@ def _same_device(who: str, first: torch.Tensor, **others) -> None:
             raise RuntimeError(f"{who}: {n} is on {t.device}, the rows are on {first.device}")
 
 
-_transformed, _traced, _mode, _PROXY = (torch._C._are_functorch_transforms_active, torch._C._is_tracing, torch._C._get_dispatch_mode,
-                                        torch._C._TorchDispatchModeKey.PROXY)  # (every call of an operator asks: 0.4 us)
+# (every call of an operator asks these: 0.3 us)
+_transformed, _traced, _mode, _included = (torch._C._are_functorch_transforms_active, torch._C._is_tracing, torch._C._get_dispatch_mode,
+                                           torch._C._dispatch_tls_is_dispatch_key_included)
+_PROXY, _PRE_DISPATCH = torch._C._TorchDispatchModeKey.PROXY, torch._C.DispatchKey.PreDispatch
 
 
 def not_eager(*ts: Optional[torch.Tensor]) -> str:
@@ -969,7 +970,7 @@ def not_eager(*ts: Optional[torch.Tensor]) -> str:
         return "under a transform of torch.func"
     if _traced():
         return "under torch.jit.trace"
-    if _mode(_PROXY) is not None or _get_dispatch_mode_pre_dispatch(_PROXY) is not None:
+    if _mode(_PROXY) is not None or _included(_PRE_DISPATCH):
         return "while torch.fx records"
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
         return "on dual numbers (forward-mode differentiation)"
@@ -1007,7 +1008,12 @@ def _dense_order(t: torch.Tensor) -> tuple:
 
 
 def _wants_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if not torch.is_grad_enabled():
+        return False
+    for t in ts:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def _angles(who, q, cos, sin, positions, freqs, layout, scale):
@@ -1080,7 +1086,10 @@ def _rope_values(ang, hold, q, k, yq=None, yk=None, wq=None, wk=None, eps: float
 
 
 def _rope_run(ang, hold, q, k, wq=None, wk=None, eps: float = 0.0, inverse: int = 0, order=None):
-    yq, yk = (None if x is None else x.new_empty(x.shape) if order is None else x.new_empty_strided(x.shape, order[i]) for i, x in enumerate((q, k)))
+    if order is None:
+        yq, yk = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
+    else:
+        yq, yk = q.new_empty_strided(q.shape, order[0]), None if k is None else k.new_empty_strided(k.shape, order[1])
     _launch("ic_rope_fwd", _pack_rope(*_rope_values(ang, hold, q, k, yq, yk, wq, wk, eps, inverse)), q.device)
     return yq, yk
 
@@ -1125,17 +1134,18 @@ class RopeFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gq, gk):
-        hold = [t.contiguous() for t in ctx.saved_tensors]  # (hooks may hand them back in another layout)
-        if len(ctx.order) == 1:
+        hold, ang, order, inverse = ctx.saved_tensors, ctx.ang, ctx.order, 1 - ctx.inverse
+        hold = [t.contiguous() for t in hold]  # (hooks may hand them back in another layout)
+        if len(order) == 1:
             gk = None
         if not_eager(gq, gk) or not _in_memory(gq, gk):
-            oq, ok = (None if g is None else _rope_plain(ctx.ang, hold, g, 1 - ctx.inverse) for g in (gq, gk))
+            oq, ok = (None if g is None else _rope_plain(ang, hold, g, inverse) for g in (gq, gk))
         else:
             gq, gk = _rows4(gq), None if gk is None else _rows4(gk)
             if _wants_grad(gq, gk):
-                oq, ok = RopeFn.apply(gq, gk, ctx.ang, 1 - ctx.inverse, ctx.order, *hold)
+                oq, ok = RopeFn.apply(gq, gk, ang, inverse, order, *hold)
             else:
-                oq, ok = _rope_run(ctx.ang, hold, gq, gk, inverse=1 - ctx.inverse, order=ctx.order)
+                oq, ok = _rope_run(ang, hold, gq, gk, None, None, 0.0, inverse, order)
         return (oq, ok, None, None, None) + (None,) * len(hold)
 
 
@@ -1154,7 +1164,7 @@ class QKNormRopeFn(torch.autograd.Function):
         _eager_only("qk_norm_rope's backward", gq, gk)
         q, k, wq, wk, *hold = ctx.saved_tensors
         q, k = _rows4(q), None if k is None else _rows4(k)
-        wq, wk, *hold = (None if t is None else t.contiguous() for t in (wq, wk, *hold))
+        wq, wk, hold = wq.contiguous(), None if wk is None else wk.contiguous(), [t.contiguous() for t in hold]
         part = torch.empty(ROPE_PARTS * q.shape[3], device=q.device)
         vals, outs, gws, keep = [], [], [], []
         for x, w, g in ((q, wq, gq), (k, wk, gk)):  # ic_rope_grad
@@ -1173,7 +1183,8 @@ class QKNormRopeFn(torch.autograd.Function):
 
 
 def _check_qk(who, q, k, *others) -> None:
-    _eager_only(who, q, k, *others)
+    if not_eager(q, k, *others):
+        _eager_only(who, q, k, *others)
     _same_device(who, q, k=k)
     if q.dim() != 4 or q.dtype not in DTYPES or not 1 <= q.shape[3] <= ROPE_MAX_D:
         raise ValueError(f"{who}: q is {q.dtype} {tuple(q.shape)}, needs fp32, bf16 or fp16 [B,H,T,D] with D <= {ROPE_MAX_D}")
@@ -1310,7 +1321,7 @@ class LinearAttnFn(torch.autograd.Function):
             return (None,) * 7
         _eager_only("linear_attention's backward", gout, gstate)
         q, k, v = _rows_near(q), _rows_near(k), _rows_near(v)  # (hooks may hand them back in another layout)
-        rate, state, valid_len = (None if t is None else t.contiguous() for t in (rate, state, valid_len))
+        rate, state, valid_len = rate.contiguous(), None if state is None else state.contiguous(), None if valid_len is None else valid_len.contiguous()
         B, H, T, Dk = q.shape
         gout = torch.zeros((B, H, T, v.shape[3]), dtype=q.dtype, device=q.device) if gout is None else _rows_near(gout)
         gstate = None if gstate is None else gstate.contiguous()
@@ -1325,7 +1336,8 @@ class LinearAttnFn(torch.autograd.Function):
 
 
 def _check_linear(who, q, k, v, rate, state, dims: int, most: int):
-    _eager_only(who, q, k, v, rate, state)
+    if not_eager(q, k, v, rate, state):
+        _eager_only(who, q, k, v, rate, state)
     _same_device(who, q, k=k, v=v, rate=rate, state=state)
     want = "[B,H,T,Dk], [B,Hk,T,Dk], [B,Hk,T,Dv]" if dims == 4 else "[B,H,Dk], [B,Hk,Dk], [B,Hk,Dv]"
     say = lambda: f"{who}: q, k, v are {q.dtype} {tuple(q.shape)}, {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}"  # noqa: E731
