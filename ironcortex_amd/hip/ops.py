@@ -965,7 +965,10 @@ _PROXY, _PRE_DISPATCH = torch._C._TorchDispatchModeKey.PROXY, torch._C.DispatchK
 
 def not_eager(*ts: Optional[torch.Tensor]) -> str:
     """What keeps a launch from standing for an operation on these tensors, or "": what records operations (torch.jit.trace,
-    torch.fx) does not see it, torch.func's transforms have no rule for it, and it hands no tangent on."""
+    torch.fx) does not see it, torch.func's transforms have no rule for it, and it hands no tangent on.  (torch.compile leaves its
+    graph for a launch.)"""
+    if torch.compiler.is_compiling():
+        return ""
     if _transformed():
         return "under a transform of torch.func"
     if _traced():

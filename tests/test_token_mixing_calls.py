@@ -376,3 +376,39 @@ def test_linear_attention_of_no_positions_passes_gradients_on(dtype, launches):
                     assert torch.equal(torch.zeros_like(x) if gx is None else gx, torch.ones_like(st) if x is st and y is s else torch.zeros_like(x))
                 assert got[3] is not None
     assert launches == []
+
+
+def compiled_calls(device):
+    from ironcortex_amd.hip import ops
+    f, w, r, st = torch.ones(4, device=device), torch.ones(8, device=device), torch.ones(3, device=device), torch.zeros(2, 3, 8, 8, device=device)
+
+    def step(q):
+        with torch.no_grad():
+            return ops.linear_attention_step(q[:, :, 0], q[:, :, 1], q[:, :, 2], r, st.clone()) * 2
+
+    return {"rope": lambda q: ops.rope(q, freqs=f) * 2, "norm": lambda q: ops.qk_norm_rope(q, q, w, w, freqs=f)[0] * 2,
+            "linear": lambda q: ops.linear_attention(q, q, q, r)[0] * 2, "step": step}
+
+
+@pytest.mark.parametrize("which", ["rope", "norm", "linear", "step"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_compiled_programs_leave_their_graph_for_a_launch(which, grad, launches):
+    x = torch.randn(2, 3, 5, 8, requires_grad=grad)
+    torch._dynamo.reset()
+    y = torch.compile(compiled_calls("cpu")[which], backend="eager")(x)
+    if y.requires_grad:
+        y.sum().backward()
+    assert len(launches) == (2 if grad and which != "step" else 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["rope", "norm", "linear", "step"])
+def test_compiled_programs_give_the_same(which):
+    x = torch.randn(2, 3, 5, 8, device=DEV, requires_grad=True)
+    f = compiled_calls(DEV)[which]
+    want = f(x)
+    torch._dynamo.reset()
+    got = torch.compile(f, backend="eager")(x)
+    assert torch.equal(got, want) and got.requires_grad == want.requires_grad == (which != "step")
+    if which != "step":
+        assert torch.equal(*(torch.autograd.grad(y.sin().sum(), x)[0] for y in (got, want)))
