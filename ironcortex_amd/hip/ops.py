@@ -957,23 +957,28 @@ def _same_device(who: str, first: torch.Tensor, **others) -> None:
             raise RuntimeError(f"{who}: {n} is on {t.device}, the rows are on {first.device}")
 
 
-# (every call of an operator asks these: 0.3 us)
-_transformed, _traced, _mode, _included = (torch._C._are_functorch_transforms_active, torch._C._is_tracing, torch._C._get_dispatch_mode,
-                                           torch._C._dispatch_tls_is_dispatch_key_included)
-_PROXY, _PRE_DISPATCH = torch._C._TorchDispatchModeKey.PROXY, torch._C.DispatchKey.PreDispatch
+_tls_keys = torch._C._dispatch_tls_local_include_set
+_PLAIN_KEYS = {k.raw_repr() for k in (torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect),  # (in inference mode)
+                                      torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect).add(torch._C.DispatchKey.ADInplaceOrView))}
+
+
+def _plain_call() -> bool:
+    """Nothing records, transforms, batches or differentiates forwards here: what every call and backward pass asks first (one
+    look at the thread's dispatch keys, where each of them leaves its own)."""
+    return forward_ad._current_level < 0 and _tls_keys().raw_repr() in _PLAIN_KEYS
 
 
 def not_eager(*ts: Optional[torch.Tensor]) -> str:
     """What keeps a launch from standing for an operation on these tensors, or "": what records operations (torch.jit.trace,
     torch.fx) does not see it, torch.func's transforms have no rule for it, and it hands no tangent on.  (torch.compile leaves its
     graph for a launch.)"""
-    if torch.compiler.is_compiling():
+    if _plain_call() or torch.compiler.is_compiling():
         return ""
-    if _transformed():
+    if torch._C._are_functorch_transforms_active():
         return "under a transform of torch.func"
-    if _traced():
+    if torch._C._is_tracing():
         return "under torch.jit.trace"
-    if _mode(_PROXY) is not None or _included(_PRE_DISPATCH):
+    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None or torch._C._dispatch_tls_is_dispatch_key_included(torch._C.DispatchKey.PreDispatch):
         return "while torch.fx records"
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
         return "on dual numbers (forward-mode differentiation)"
@@ -1137,19 +1142,27 @@ class RopeFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gq, gk):
-        hold, ang, order, inverse = ctx.saved_tensors, ctx.ang, ctx.order, 1 - ctx.inverse
-        hold = [t.contiguous() for t in hold]  # (hooks may hand them back in another layout)
-        if len(order) == 1:
+        hold = ctx.saved_tensors
+        if not (hold[0].is_contiguous() and hold[-1].is_contiguous()):  # (hooks may hand them back in another layout)
+            hold = [t.contiguous() for t in hold]
+        if len(ctx.order) == 1:
             gk = None
+        if torch.is_grad_enabled() or not _plain_call():
+            return RopeFn._backward_of_any_kind(ctx, hold, gq, gk)
+        gq, gk = _rows4(gq), None if gk is None else _rows4(gk)
+        oq, ok = _rope_run(ctx.ang, hold, gq, gk, None, None, 0.0, 1 - ctx.inverse, ctx.order)
+        return (oq, ok, None, None, None) + (None,) * len(hold)
+
+    @staticmethod
+    def _backward_of_any_kind(ctx, hold, gq, gk):
+        """... where it may be differentiated itself, or runs on gradients that a kernel cannot read."""
         if not_eager(gq, gk) or not _in_memory(gq, gk):
-            oq, ok = (None if g is None else _rope_plain(ang, hold, g, inverse) for g in (gq, gk))
+            out = [None if g is None else _rope_plain(ctx.ang, hold, g, 1 - ctx.inverse) for g in (gq, gk)]
         else:
             gq, gk = _rows4(gq), None if gk is None else _rows4(gk)
-            if _wants_grad(gq, gk):
-                oq, ok = RopeFn.apply(gq, gk, ang, inverse, order, *hold)
-            else:
-                oq, ok = _rope_run(ang, hold, gq, gk, None, None, 0.0, inverse, order)
-        return (oq, ok, None, None, None) + (None,) * len(hold)
+            args = (gq, gk, ctx.ang, 1 - ctx.inverse, ctx.order, *hold)
+            out = RopeFn.apply(*args) if _wants_grad(gq, gk) else _rope_run(ctx.ang, hold, gq, gk, inverse=1 - ctx.inverse, order=ctx.order)
+        return (*out, None, None, None) + (None,) * len(hold)
 
 
 class QKNormRopeFn(torch.autograd.Function):
@@ -1164,10 +1177,12 @@ class QKNormRopeFn(torch.autograd.Function):
 
     @_once
     def backward(ctx, gq, gk):
-        _eager_only("qk_norm_rope's backward", gq, gk)
-        q, k, wq, wk, *hold = ctx.saved_tensors
+        if not _plain_call():
+            _eager_only("qk_norm_rope's backward", gq, gk)
+        q, k, wq, wk, *hold = ctx.saved_tensors  # (which hooks may hand back in another layout)
+        if not (hold[0].is_contiguous() and hold[-1].is_contiguous() and wq.is_contiguous() and (wk is None or wk.is_contiguous())):
+            wq, wk, hold = wq.contiguous(), None if wk is None else wk.contiguous(), [t.contiguous() for t in hold]
         q, k = _rows4(q), None if k is None else _rows4(k)
-        wq, wk, hold = wq.contiguous(), None if wk is None else wk.contiguous(), [t.contiguous() for t in hold]
         part = torch.empty(ROPE_PARTS * q.shape[3], device=q.device)
         vals, outs, gws, keep = [], [], [], []
         for x, w, g in ((q, wq, gq), (k, wk, gk)):  # ic_rope_grad
@@ -1186,7 +1201,7 @@ class QKNormRopeFn(torch.autograd.Function):
 
 
 def _check_qk(who, q, k, *others) -> None:
-    if not_eager(q, k, *others):
+    if not _plain_call():
         _eager_only(who, q, k, *others)
     _same_device(who, q, k=k)
     if q.dim() != 4 or q.dtype not in DTYPES or not 1 <= q.shape[3] <= ROPE_MAX_D:
@@ -1322,7 +1337,8 @@ class LinearAttnFn(torch.autograd.Function):
         q, k, v, rate, state, valid_len = ctx.saved_tensors
         if gout is None and gstate is None:
             return (None,) * 7
-        _eager_only("linear_attention's backward", gout, gstate)
+        if not _plain_call():
+            _eager_only("linear_attention's backward", gout, gstate)
         q, k, v = _rows_near(q), _rows_near(k), _rows_near(v)  # (hooks may hand them back in another layout)
         rate, state, valid_len = rate.contiguous(), None if state is None else state.contiguous(), None if valid_len is None else valid_len.contiguous()
         B, H, T, Dk = q.shape
@@ -1339,7 +1355,7 @@ class LinearAttnFn(torch.autograd.Function):
 
 
 def _check_linear(who, q, k, v, rate, state, dims: int, most: int):
-    if not_eager(q, k, v, rate, state):
+    if not _plain_call():
         _eager_only(who, q, k, v, rate, state)
     _same_device(who, q, k=k, v=v, rate=rate, state=state)
     want = "[B,H,T,Dk], [B,Hk,T,Dk], [B,Hk,T,Dv]" if dims == 4 else "[B,H,Dk], [B,Hk,Dk], [B,Hk,Dv]"
