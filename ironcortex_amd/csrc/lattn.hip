@@ -12,8 +12,8 @@
 // So ONE kernel serves the forward (one pass) and the backward (three).  Against a kernel that forms all three gradients of a
 // chunk at once it multiplies 12 tiles instead of 10, and needs neither the state at every chunk's border in memory nor two
 // states in registers.  Gradients of shared key / value heads: a workgroup takes their query heads in turn and keeps the sum
-// in fp32 rows that only its own lanes touch (against a partial gradient for each query head and a joining launch: 14 of
-// 564 us less for a forward and backward of 8 x 4096 positions, 8 / 4 bf16 heads of 128, and half the workspace).
+// in fp32 rows that only its own lanes touch (against a partial gradient for each query head and a joining launch: 14 us less
+// of a forward and backward of 8 x 4096 positions, 8 / 4 bf16 heads of 128, and half the workspace).
 // d rate: -d o / d rate weighs every pair by its lag.  The dq pass carries the lag-weighted state L = sum lag e^{-r lag}
 // k v^T next to S, and sums q_i . (lag-weighted dq_i): every term counted once with its own lag, where a difference of
 // position-weighted q . dq and k . dk would cancel to T times the rounding error.
@@ -27,15 +27,25 @@
 //
 // Measured (microseconds; floors are the rows' bytes at the 4.76 TB/s of a large copy and the products at the 153 / 1201
 // TFLOP/s of large fp32 / bf16 matrix products):
-//   one document of 65536 positions, 8 bf16 heads of 128: sums 69 (3.9 TB/s), scan 15, pass 163 (3.3 TB/s); floor 113, and
-//     169 with k and v read twice.  Of the pass's time the matrix instructions are busy for 30%, vector arithmetic for 35%,
-//     30% of its waves' time waits (LDS round trips between the barriers, rows from memory).  Four waves a SIMD instead of two
-//     (one column tile a wave, 128 registers) spill: 240 us.  K and V without bank conflicts in the products of rows (a third
-//     of the LDS time has them) cost a register that is not there: 165 us.
-//   forward and backward of 8 x 4096 positions, 8 / 4 bf16 heads of 128: forward 36 + 25 + 88; backward sums 80, scan 25, dq
-//     and d rate 182, dk and dv 210, d rate's sum 5.
-//   forward and backward of 16 x 1024 positions, 4 fp32 heads of 64: forward 14 + 9 + 27; backward 27 + 9 + 50 + 52 + 4; the
+//   one document of 65536 positions, 8 bf16 heads of 128: sums 74 (3.6 TB/s), scan 18, pass 209 (2.6 TB/s); floor 113, and
+//     169 with k and v read twice.  Of the pass's time the matrix instructions are busy for 28%, vector arithmetic for 41%, 35%
+//     of its waves' time waits (LDS round trips between the barriers, rows from memory).  Four waves a SIMD instead of two (one column tile a wave, 128 registers) spill: 240 us, when operands of two parts
+//     took 163.  K and V without bank conflicts in the products of rows (a third of the LDS time has them) cost a register that
+//     is not there.
+//   forward and backward of 8 x 4096 positions, 8 / 4 bf16 heads of 128: forward 38 + 28 + 105; backward sums 92, scan 28, dq
+//     and d rate 190 (matrix 29%, vector 45%, waves waiting 41%, 222 MB), dk and dv 249 (22%, 38%, 46%, 484 MB), d rate's sum 5.
+//   forward and backward of 16 x 1024 positions, 4 fp32 heads of 64: forward 14 + 10 + 27; backward 31 + 10 + 51 + 54 + 4; the
 //     products alone take 54 at the fp32 rate, and 2 chunks a workgroup leave half of a pass to its ends.
+// Registers: a pass of 128 channels fills all 256, with a few in scratch memory (vector / scalar ones the compiler reports: bf16
+// forward 2 / 51, dk and dv of shared heads 8 / 166, dq with d rate 2 / 75; fp32 and fp16 up to 9 / 154).
+//
+// fp16 rows take the fp32 kernels: products of rows would be exact on 16-bit matrix instructions of their type, but the state,
+// P and the decayed values leave its range (65504, and below 2^-24), and bf16 parts would have to be cut from the rows as well.
+//
+// Exactness: sums are formed where they are small and added to the state or the row once (an fp32 matrix instruction rounds after
+// every product), a carried state is rounded once or twice a chunk.  Mean square errors of the sizes above: states 1.0e-7 to
+// 1.3e-7, fp32 rows 1.9e-7, 4e-4 of the bf16 values rounded otherwise than the exact ones, d rate 1.5e-7 (bf16), 2.0e-7 (fp16) and
+// 2.4e-7 (fp32) of the root of its terms' squares; a plain evaluation in fp32 has 1.5e-7, 2.1e-7 and 3e-7 to 6e-7.
 #include <type_traits>
 
 #include "ic_types.h"
@@ -689,7 +699,9 @@ __device__ __forceinline__ void lattn_body(const Geo& g, const Pass* p, const Su
 // Rows that allow 16-byte accesses (others take the body above).
 // The same map on bf16 matrix instructions (16x16x32: sixteen times the fp32 rate).  Products of rows (q . k) are exact
 // there.  Operands that are computed in fp32 -- the decayed products P, the state, the decay-weighted values -- are split
-// into three bf16 parts (x = x1 + x2 + x3, each the rounded rest of the one before, 8 bits apiece), all of fp32's 24 bits.
+// into three bf16 parts (x = x1 + x2 + x3, each the rounded rest of the one before, 8 bits apiece), all of fp32's 24 bits.  Two
+// parts are 13% faster (wide training pass of the figures above: 564 us), but 16 bits are fewer than the sums' 24: 3e-3 of the bf16
+// results were rounded otherwise than the exact ones, states off by 2.4e-6.
 // Rows lie in LDS as they come; column operands (k^T, v^T) are read with the transposing LDS load
 // (16 lanes x 8 bytes of four rows -> four rows of one column per lane).  A 32-deep operand of a lane is therefore k-indices
 // 4 q .. 4 q + 3 of either 16-row half, on both sides of a product; products of rows use contiguous eights instead.
@@ -1124,7 +1136,7 @@ __device__ __forceinline__ void lattn_body16(const Geo& g, const Pass* p, const 
 }
 
 // bf16 rows, 128 channels: two column tiles a wave, so that 4 waves own the columns and two workgroups fit a compute unit
-// (74 KB of LDS, <= 256 registers): the one's barriers under the other's products.  One tile a wave where the lag-weighted
+// (77 KB of LDS, <= 256 registers): the one's barriers under the other's products.  One tile a wave where the lag-weighted
 // state doubles the registers.
 template <int DP, bool LAG, bool W16>
 constexpr int cw_of() { return W16 && DP == 128 && !LAG ? 2 : 1; }
@@ -1165,7 +1177,7 @@ __global__ __launch_bounds__(DP * 4) void k_lattn_sums(SumArgs a) {
 }
 
 // segment sums -> start states: seg[s] <- state in front of segment s.  A thread owns an element of a state; memory-bound but for
-// the ends of its chain (64 segments of 8 heads of 128 x 128: 67 MB in 15 us, 4.4 TB/s; with eight sums in flight 22.5 us).
+// the ends of its chain (64 segments of 8 heads of 128 x 128: 67 MB in 17 us, 3.9 TB/s; with eight sums in flight 7 us more).
 struct ScanState {
   Span sp;
   float* seg;
@@ -1227,7 +1239,7 @@ __global__ __launch_bounds__(64) void k_lattn_drate(const double* part, float* d
 }
 
 // One position.  Memory-bound: the state is read and written once (256 sequences, 16 heads of 128 x 128: 537 MB in 114 us, 4.7 TB/s,
-// a large copy's rate; a call for 4 heads of 64 x 64 costs its launch, 10 us).  A workgroup owns (sequence, head, 32 value columns):
+// a large copy's rate; a call for 4 heads of 64 x 64 costs its launch, 11 us).  A workgroup owns (sequence, head, 32 value columns):
 // 8 lanes x 4 columns, 32 rows of threads over the key channels; the output's sum over them goes through LDS.
 constexpr int kStepRows = 32;
 template <typename T>
@@ -1336,7 +1348,7 @@ Span span_of(int T, int64_t have, int slots) {
   }
   return g;
 }
-// Workgroups at a time: 32 channels 38 KB of LDS, 64 channels 53 KB and 168 registers (232 with the lag-weighted state), 128
+// Workgroups at a time: 32 channels 40 KB of LDS, 64 channels 53 KB and 168 registers (256 with the lag-weighted state), 128
 // channels 75 KB and 256 registers for bf16 rows, 86 KB for others.  (bf16 rows that take the fp32 kernels for want of
 // 16-byte accesses are planned like the rest of their type.)
 int slots_of(const ic_lattn_args* a, bool lag) {

@@ -10,7 +10,7 @@
 // Measured (bytes read and written once / time; a large copy reaches 4.76 TB/s): rotation of 131072 positions of 8 + 2 bf16
 // heads of 128 channels, half of each turned, 671 MB in 136 us = 4.9 TB/s; norms and rotation, forward and backward, of
 // 32768 positions of 16 + 4 bf16 heads of 128, 839 MB in 190 us = 4.4 TB/s; 16 x 266 positions of 4 + 4 fp32 heads of 64,
-// forward and backward, 9 + 9 us, where the call and the autograd engine around them take 100.
+// forward and backward, 9 + 9 us, where the call and the autograd engine around them take 110.
 #include "ic_types.h"
 
 namespace {
